@@ -13,7 +13,7 @@ LIB_PATH = os.path.join(HERE, "_build", "libann_b200.so")
 
 ANN_OK, ANN_EINVAL, ANN_ECUDA, ANN_ENOTSUP, ANN_EDEVICE, ANN_ENCCL, ANN_EIO = 0, 1, 2, 3, 4, 5, 6
 COMM_ID_BYTES = 128
-ANN_DEVERR_TOKEN_ID, ANN_DEVERR_WAIT_TIMEOUT = 0x1, 0x2
+ANN_DEVERR_TOKEN_ID, ANN_DEVERR_WAIT_TIMEOUT, ANN_DEVERR_CACHE_RANGE = 0x1, 0x2, 0x4
 MAX_RANK = 8
 
 
@@ -71,12 +71,21 @@ SIGNATURES = {
                                     ctypes.c_char_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                     ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64], ctypes.c_int),
 }
+SIGNATURES.update({
+    "ann_rotary_frequencies": ([_S, _P] + [ctypes.c_double] * 5, ctypes.c_int),
+    "ann_kv_cache_append_q8_f32": ([_S] + [_P] * 8 + [_u32, _i32], ctypes.c_int),
+    "ann_kv_cache_read_q8_f32": ([_S] + [_P] * 7 + [_u32, _i32], ctypes.c_int),
+    "ann_attention_decode_q8_f32": ([_S] + [_P] * 7 + [ctypes.c_float, _u32, _u32, _i32, _i32], ctypes.c_int),
+    "ann_pack_weight_q4_f32": ([_S] + [_P] * 3 + [_u32], ctypes.c_int),
+    "ann_linear_q4_f32": ([_S] + [_P] * 6 + [_u32, _i32], ctypes.c_int),
+})
 for _sfx, _ft in _f.items():
     SIGNATURES.update({
         f"ann_embedding_lookup_{_sfx}": ([_S, _P, _P, _P], ctypes.c_int),
         f"ann_rms_norm_{_sfx}": ([_S, _P, _P, _P, _ft], ctypes.c_int),
         f"ann_embedding_rms_norm_{_sfx}": ([_S, _P, _P, _P, _P, _ft], ctypes.c_int),
         f"ann_rope_{_sfx}": ([_S, _P, _P, _P, _P, _i32, _u32], ctypes.c_int),
+        f"ann_rotary_{_sfx}": ([_S] + [_P] * 6 + [_i32, _i32, _ft, _i32], ctypes.c_int),
         f"ann_rope_inplace_{_sfx}": ([_S, _P, _P, _P, _P, _i32, _u32], ctypes.c_int),
         f"ann_attention_scores_{_sfx}": ([_S, _P, _P, _P, _u32, _i32], ctypes.c_int),
         f"ann_scale_{_sfx}": ([_S, _P, _ft, _P], ctypes.c_int),

@@ -37,6 +37,7 @@ int take_prefill_f64_error(cudaStream_t s, uint32_t* bits);
 int take_softmax_error(cudaStream_t s, uint32_t* bits);
 int take_multicast_error(cudaStream_t s, uint32_t* bits);
 int take_attention_tc_error(cudaStream_t s, uint32_t* bits);
+int take_kv_q8_error(cudaStream_t s, uint32_t* bits);
 
 // ---------------------------------------------------------------------------
 // Views: ann_view with byte pitches -> element strides, validated.
@@ -72,6 +73,14 @@ inline bool same_extents(const Dims& a, const Dims& b) {
     if (a.rank != b.rank) return false;
     for (int i = 0; i < a.rank; ++i)
         if (a.ext[i] != b.ext[i]) return false;
+    return true;
+}
+
+// An output in which no two elements share an address through a zero pitch.
+inline bool writable(const Dims& d) {
+    if (d.numel() == 0) return true;
+    for (int a = 0; a < d.rank; ++a)
+        if (d.ext[a] > 1 && d.str[a] == 0) return false;
     return true;
 }
 

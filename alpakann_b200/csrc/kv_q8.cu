@@ -1,0 +1,363 @@
+// kv_q8.cu -- a KV cache held in 8 bits: append and read-back.
+//
+// A cache value is a whole number n in [-127, 127]; it stands for n * s, with
+// one fp32 scale s per KV head and block of `block` tokens:
+//   k_cache, v_cache int8 [B, Hkv, Tcap, D] (or BTHD), scales [B, Hkv, ceil(Tcap / block)].
+//
+// append: s' = max(s of the block's earlier rows, max|x| / 127 over the new
+// rows in the block); a new value becomes the whole number nearest to the exact
+// quotient x / s' (ties to even); where s' grew, the block's earlier values are
+// rounded anew from n * s / s'. The rounding is exact, not that of a 32-bit
+// quotient, so any implementation of this definition gives the same integers.
+// A NaN or infinity in a new row makes its block's scale NaN or infinite, so
+// the block reads back as NaN / infinity instead of as wrong finite values.
+//
+// Both are bound by HBM: append reads 4 bytes and writes 1 per value, the
+// read-back reads 1 and writes 4.
+#include <algorithm>
+
+#include "common.cuh"
+#include "reduce.cuh"
+
+namespace ann {
+namespace {
+
+__device__ unsigned int g_kv_q8_error;
+
+constexpr int kThreads = 256;
+
+struct CacheTensor {
+    int8_t* q;
+    float* scale;
+    int64_t q_b, q_h, q_t, q_d;  // element strides
+    int64_t s_b, s_h, s_j;
+};
+
+struct AppendArgs {
+    CacheTensor c[2];
+    const float* x[2];
+    int64_t x_b[2], x_t[2], x_h[2], x_d[2];
+    const int32_t* pos;
+    const int32_t* counts;  // may be null: every row
+    int64_t pos_s, counts_s;
+    int64_t Tn, H, D, cap, block, touched;  // touched: blocks a sequence's rows can reach
+    int vec;                                // rows of 4 aligned values
+};
+
+// The whole number nearest to x / s, exactly, ties to even; |x| <= 127 s up to
+// the rounding of s. t is within 2^-16 of the quotient, so rint(t) is off by one
+// at most; r = x - n s is exact in 32 bits (a multiple of half an ulp of s, at
+// most 2^24 of them), and comparing it with s / 2 puts n right.
+__device__ __forceinline__ int nearest(float x, float s, float inv) {
+    float n = rintf(x * inv);
+    float const r = fmaf(-n, s, x), half = 0.5f * s;
+    bool const odd = static_cast<int>(n) & 1;
+    if (r > half || (r == half && odd)) n += 1.0f;
+    if (r < -half || (r == -half && odd)) n -= 1.0f;
+    return max(-127, min(127, static_cast<int>(n)));
+}
+// The same in 64 bits, for scales so small that the 32-bit remainder is not
+// exact, and for requantised values n_old * s_old / s.
+__device__ __forceinline__ int nearest64(double x, double s) {
+    return static_cast<int>(fmin(fmax(rint(x / s), -127.0), 127.0));
+}
+
+__global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
+    __shared__ unsigned int red[kThreads / 32];
+    int64_t unit = blockIdx.x;
+    int64_t const jb = unit % a.touched;
+    unit /= a.touched;
+    int const kv = static_cast<int>(unit & 1);
+    unit >>= 1;
+    int64_t const h = unit % a.H, b = unit / a.H;
+
+    int64_t const start = a.pos[b * a.pos_s];
+    int64_t count = a.Tn;
+    if (a.counts != nullptr) count = min(a.Tn, max(int64_t{0}, static_cast<int64_t>(a.counts[b * a.counts_s])));
+    int64_t const first = max(start, int64_t{0}), end = min(start + count, a.cap);
+    if (threadIdx.x == 0 && count > 0 && (start < 0 || start + count > a.cap))
+        atomicOr(&g_kv_q8_error, ANN_DEVERR_CACHE_RANGE);
+    int64_t const j = first / a.block + jb;
+    int64_t const lo = max(first, j * a.block), hi = min(end, (j + 1) * a.block);
+    if (lo >= hi) return;
+
+    CacheTensor const& c = kv ? a.c[1] : a.c[0];
+    float const* x = (kv ? a.x[1] : a.x[0]) + b * (kv ? a.x_b[1] : a.x_b[0]) + h * (kv ? a.x_h[1] : a.x_h[0]);
+    int64_t const x_t = kv ? a.x_t[1] : a.x_t[0], x_d = kv ? a.x_d[1] : a.x_d[0];
+    x += (lo - start) * x_t;
+    int8_t* q = c.q + b * c.q_b + h * c.q_h;
+    float* scale = c.scale + b * c.s_b + h * c.s_h + j * c.s_j;
+    int const rows = static_cast<int>(hi - lo), D = static_cast<int>(a.D);
+
+    // max |x| on the bit patterns: ordered like the values, infinity above every
+    // number and NaN above infinity.
+    unsigned int top = 0;
+    if (a.vec) {
+        int const dv = D / 4;
+        for (int i = threadIdx.x; i < rows * dv; i += kThreads) {
+            int const r = i / dv, d = i - r * dv;
+            uint4 const v = *reinterpret_cast<uint4 const*>(x + r * x_t + 4 * d);
+            top = max(max(max(top, v.x & 0x7fffffffu), v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
+        }
+    } else {
+        for (int i = threadIdx.x; i < rows * D; i += kThreads) {
+            int const r = i / D, d = i - r * D;
+            top = max(top, __float_as_uint(x[r * x_t + d * x_d]) & 0x7fffffffu);
+        }
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+    bool const begun = j * a.block < lo;  // the block holds earlier rows
+    float const old = begun ? fabsf(*scale) : 0.0f;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) top = max(top, red[w]);
+    unsigned int const want = __float_as_uint(__fdiv_rn(__uint_as_float(top), 127.0f));
+    float const s = __uint_as_float(max(want, __float_as_uint(old)));
+    if (threadIdx.x == 0) *scale = s;  // every thread has read the old one before the barrier above
+
+    bool const finite = __float_as_uint(s) < 0x7f800000u && s > 0.0f;
+    if (begun && __float_as_uint(s) != __float_as_uint(old)) {
+        int64_t const t0 = j * a.block;
+        int const early = static_cast<int>(lo - t0);
+        for (int i = threadIdx.x; i < early * D; i += kThreads) {
+            int const r = i / D, d = i - r * D;
+            int8_t* p = q + (t0 + r) * c.q_t + d * c.q_d;
+            *p = static_cast<int8_t>(finite ? nearest64(static_cast<double>(*p) * old, s) : 0);
+        }
+    }
+    bool const tiny = s < 1e-30f;  // 64-bit rounding below: the remainder's ulp argument needs normal numbers
+    float const inv = 1.0f / s;
+    auto round1 = [&](float v) {
+        if (!finite) return 0;
+        return tiny ? nearest64(v, s) : nearest(v, s, inv);
+    };
+    if (a.vec) {
+        int const dv = D / 4;
+        for (int i = threadIdx.x; i < rows * dv; i += kThreads) {
+            int const r = i / dv, d = i - r * dv;
+            float4 const v = *reinterpret_cast<float4 const*>(x + r * x_t + 4 * d);
+            char4 const n = make_char4(round1(v.x), round1(v.y), round1(v.z), round1(v.w));
+            *reinterpret_cast<char4*>(q + (lo + r) * c.q_t + 4 * d) = n;
+        }
+    } else {
+        for (int i = threadIdx.x; i < rows * D; i += kThreads) {
+            int const r = i / D, d = i - r * D;
+            q[(lo + r) * c.q_t + d * c.q_d] = static_cast<int8_t>(round1(x[r * x_t + d * x_d]));
+        }
+    }
+}
+
+struct ReadArgs {
+    CacheTensor c[2];
+    float* out[2];
+    int64_t o_b[2], o_h[2], o_t[2], o_d[2];
+    const int32_t* lengths;  // may be null: every row
+    int64_t len_s;
+    int64_t H, D, Tout, block, chunks;  // chunks of kReadItems items per (batch, head)
+    int vec;
+};
+
+constexpr int kReadItems = kThreads * 8;
+
+template <bool VEC>
+__global__ void __launch_bounds__(kThreads) read_kernel(ReadArgs a) {
+    int64_t unit = blockIdx.x;
+    int64_t const chunk = unit % a.chunks;
+    unit /= a.chunks;
+    int const kv = static_cast<int>(unit & 1);
+    unit >>= 1;
+    int64_t const h = unit % a.H, b = unit / a.H;
+    int64_t rows = a.Tout;
+    if (a.lengths != nullptr) rows = min(rows, max(int64_t{0}, static_cast<int64_t>(a.lengths[b * a.len_s])));
+    CacheTensor const& c = kv ? a.c[1] : a.c[0];
+    int8_t const* q = c.q + b * c.q_b + h * c.q_h;
+    float const* scale = c.scale + b * c.s_b + h * c.s_h;
+    float* out = (kv ? a.out[1] : a.out[0]) + b * (kv ? a.o_b[1] : a.o_b[0]) + h * (kv ? a.o_h[1] : a.o_h[0]);
+    int64_t const o_t = kv ? a.o_t[1] : a.o_t[0], o_d = kv ? a.o_d[1] : a.o_d[0];
+    int64_t const per = VEC ? a.D / 4 : a.D;  // items per row
+    int64_t const total = rows * per, base = chunk * kReadItems + threadIdx.x;
+#pragma unroll 4
+    for (int u = 0; u < 8; ++u) {
+        int64_t const i = base + u * kThreads;
+        if (i >= total) break;
+        int64_t const t = i / per, d = i - t * per;
+        float const s = scale[t / a.block * c.s_j];
+        if constexpr (VEC) {
+            char4 const n = *reinterpret_cast<char4 const*>(q + t * c.q_t + 4 * d);
+            *reinterpret_cast<float4*>(out + t * o_t + 4 * d) = make_float4(n.x * s, n.y * s, n.z * s, n.w * s);
+        } else {
+            out[t * o_t + d * o_d] = static_cast<float>(q[t * c.q_t + d * c.q_d]) * s;
+        }
+    }
+}
+
+// The two caches and their scales, checked against each other.
+int cache_tensors(const char* what, const ann_view* const qv[2], const ann_view* const sv[2], uint32_t block, int layout,
+                  Dims q[2], Dims s[2]) {
+    if (layout != ANN_LAYOUT_BTHD && layout != ANN_LAYOUT_BHTD) return fail(ANN_EINVAL, "%s: invalid kv layout.", what);
+    if (block == 0) return fail(ANN_EINVAL, "%s requires tokensPerScale > 0.", what);
+    for (int k = 0; k < 2; ++k) {
+        ANN_TRY(to_dims(qv[k], 1, what, q[k]));
+        ANN_TRY(to_dims(sv[k], sizeof(float), what, s[k]));
+    }
+    if (q[0].rank != 4 || q[1].rank != 4) return fail(ANN_EINVAL, "%s expects rank-4 caches.", what);
+    if (!same_extents(q[0], q[1])) return fail(ANN_EINVAL, "%s: K and V cache extents differ.", what);
+    int const tok = layout == ANN_LAYOUT_BTHD ? 1 : 2, head = 3 - tok;
+    for (int k = 0; k < 2; ++k)
+        if (s[k].rank != 3 || s[k].ext[0] != q[k].ext[0] || s[k].ext[1] != q[k].ext[head] ||
+            s[k].ext[2] != ceil_div(q[k].ext[tok], block))
+            return fail(ANN_EINVAL, "%s: scales %s do not match the cache %s with %u tokens a scale.", what,
+                        extents_str(s[k]).c_str(), extents_str(q[k]).c_str(), block);
+    return ANN_OK;
+}
+
+CacheTensor tensor_of(const Dims& q, const Dims& s, int layout) {
+    int const tok = layout == ANN_LAYOUT_BTHD ? 1 : 2, head = 3 - tok;
+    return CacheTensor{static_cast<int8_t*>(q.data), static_cast<float*>(s.data), q.str[0], q.str[head], q.str[tok],
+                       q.str[3], s.str[0], s.str[1], s.str[2]};
+}
+
+// A rank-1 int32 view with one entry per sequence.
+int per_sequence(const ann_view* v, const char* what, int64_t B, const int32_t*& p, int64_t& stride) {
+    Dims d;
+    ANN_TRY(to_dims(v, sizeof(int32_t), what, d));
+    if (d.rank != 1 || d.ext[0] != B) return fail(ANN_EINVAL, "%s must be rank 1 with one entry per sequence.", what);
+    p = static_cast<const int32_t*>(d.data);
+    stride = d.str[0];
+    return ANN_OK;
+}
+
+bool rows4(const Dims& x, size_t elem) {  // unit stride, 4 elements aligned in every row
+    if (x.str[3] != 1 || x.ext[3] % 4 != 0 || !aligned(x.data, 4 * elem)) return false;
+    return x.str[0] % 4 == 0 && x.str[1] % 4 == 0 && x.str[2] % 4 == 0;
+}
+
+int append(ann_stream stream, const ann_view* kn, const ann_view* vn, const ann_view* kc, const ann_view* vc,
+           const ann_view* ks, const ann_view* vs, const ann_view* pos_v, const ann_view* counts_v, uint32_t block,
+           int layout) {
+    char const* what = "kvCacheAppendQ8";
+    Dims x[2], q[2], s[2];
+    ANN_TRY(to_dims(kn, sizeof(float), what, x[0]));
+    ANN_TRY(to_dims(vn, sizeof(float), what, x[1]));
+    const ann_view* const qv[2] = {kc, vc};
+    const ann_view* const sv[2] = {ks, vs};
+    ANN_TRY(cache_tensors(what, qv, sv, block, layout, q, s));
+    int const tok = layout == ANN_LAYOUT_BTHD ? 1 : 2, head = 3 - tok;
+    if (x[0].rank != 4 || !same_extents(x[0], x[1]))
+        return fail(ANN_EINVAL, "kvCacheAppendQ8 expects rank-4 BTHD rows of K and V of the same extents.");
+    if (x[0].ext[0] != q[0].ext[0] || x[0].ext[2] != q[0].ext[head] || x[0].ext[3] != q[0].ext[3])
+        return fail(ANN_EINVAL, "kvCacheAppendQ8: rows %s do not match the cache %s.", extents_str(x[0]).c_str(),
+                    extents_str(q[0]).c_str());
+    for (int k = 0; k < 2; ++k)
+        if (!writable(q[k]) || !writable(s[k])) return fail(ANN_EINVAL, "kvCacheAppendQ8: a cache axis has a zero pitch.");
+    AppendArgs a{};
+    int64_t const B = x[0].ext[0];
+    ANN_TRY(per_sequence(pos_v, "kvCacheAppendQ8 positions", B, a.pos, a.pos_s));
+    if (counts_v != nullptr) ANN_TRY(per_sequence(counts_v, "kvCacheAppendQ8 counts", B, a.counts, a.counts_s));
+    a.Tn = x[0].ext[1];
+    a.H = x[0].ext[2];
+    a.D = x[0].ext[3];
+    a.cap = q[0].ext[tok];
+    a.block = block;
+    if (x[0].numel() == 0 || a.cap == 0) return ANN_OK;
+    int64_t const per_block = std::min<int64_t>(block, a.cap) * a.D;
+    if (per_block > INT32_MAX) return fail(ANN_ENOTSUP, "kvCacheAppendQ8: a block of one head exceeds 2^31 values.");
+    a.vec = 1;
+    for (int k = 0; k < 2; ++k) {
+        a.c[k] = tensor_of(q[k], s[k], layout);
+        a.x[k] = static_cast<const float*>(x[k].data);
+        a.x_b[k] = x[k].str[0];
+        a.x_t[k] = x[k].str[1];
+        a.x_h[k] = x[k].str[2];
+        a.x_d[k] = x[k].str[3];
+        if (!rows4(x[k], sizeof(float)) || !rows4(q[k], 1)) a.vec = 0;
+    }
+    // Rows start anywhere in a block: at most this many blocks hold some of them.
+    a.touched = std::min(ceil_div(a.cap, block), ceil_div(a.Tn - 1, block) + 1);
+    int64_t const grid = B * a.H * 2 * a.touched;
+    if (grid > INT32_MAX) return fail(ANN_ENOTSUP, "kvCacheAppendQ8: grid too large.");
+    append_kernel<<<static_cast<unsigned>(grid), kThreads, 0, as_stream(stream)>>>(a);
+    return check_launch(what);
+}
+
+int read_back(ann_stream stream, const ann_view* kc, const ann_view* vc, const ann_view* ks, const ann_view* vs,
+              const ann_view* ko, const ann_view* vo, const ann_view* len_v, uint32_t block, int layout) {
+    char const* what = "kvCacheReadQ8";
+    Dims q[2], s[2], o[2];
+    const ann_view* const qv[2] = {kc, vc};
+    const ann_view* const sv[2] = {ks, vs};
+    ANN_TRY(cache_tensors(what, qv, sv, block, layout, q, s));
+    ANN_TRY(to_dims(ko, sizeof(float), what, o[0]));
+    ANN_TRY(to_dims(vo, sizeof(float), what, o[1]));
+    int const tok = layout == ANN_LAYOUT_BTHD ? 1 : 2, head = 3 - tok;
+    for (int k = 0; k < 2; ++k) {
+        if (o[k].rank != 4 || o[k].ext[0] != q[k].ext[0] || o[k].ext[head] != q[k].ext[head] ||
+            o[k].ext[3] != q[k].ext[3] || o[k].ext[tok] > q[k].ext[tok])
+            return fail(ANN_EINVAL, "kvCacheReadQ8: output %s does not match the cache %s.", extents_str(o[k]).c_str(),
+                        extents_str(q[k]).c_str());
+        if (!writable(o[k])) return fail(ANN_EINVAL, "kvCacheReadQ8: an output axis has a zero pitch.");
+    }
+    if (!same_extents(o[0], o[1])) return fail(ANN_EINVAL, "kvCacheReadQ8: K and V output extents differ.");
+    ReadArgs a{};
+    if (len_v != nullptr) ANN_TRY(per_sequence(len_v, "kvCacheReadQ8 lengths", q[0].ext[0], a.lengths, a.len_s));
+    a.H = q[0].ext[head];
+    a.D = q[0].ext[3];
+    a.Tout = o[0].ext[tok];
+    a.block = block;
+    if (o[0].numel() == 0) return ANN_OK;
+    a.vec = 1;
+    for (int k = 0; k < 2; ++k) {
+        a.c[k] = tensor_of(q[k], s[k], layout);
+        a.out[k] = static_cast<float*>(o[k].data);
+        a.o_b[k] = o[k].str[0];
+        a.o_h[k] = o[k].str[head];
+        a.o_t[k] = o[k].str[tok];
+        a.o_d[k] = o[k].str[3];
+        if (!rows4(o[k], sizeof(float)) || !rows4(q[k], 1)) a.vec = 0;
+    }
+    a.chunks = ceil_div(a.Tout * (a.vec ? a.D / 4 : a.D), kReadItems);
+    int64_t const grid = q[0].ext[0] * a.H * 2 * a.chunks;
+    if (grid > INT32_MAX) return fail(ANN_ENOTSUP, "kvCacheReadQ8: grid too large.");
+    if (a.vec)
+        read_kernel<true><<<static_cast<unsigned>(grid), kThreads, 0, as_stream(stream)>>>(a);
+    else
+        read_kernel<false><<<static_cast<unsigned>(grid), kThreads, 0, as_stream(stream)>>>(a);
+    return check_launch(what);
+}
+
+}  // namespace
+
+int take_kv_q8_error(cudaStream_t s, uint32_t* bits) {
+    unsigned int value = 0, zero = 0;
+    if (cudaMemcpyFromSymbolAsync(&value, g_kv_q8_error, sizeof value, 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
+        cudaMemcpyToSymbolAsync(g_kv_q8_error, &zero, sizeof zero, 0, cudaMemcpyHostToDevice, s) != cudaSuccess ||
+        cudaStreamSynchronize(s) != cudaSuccess)
+        return fail(ANN_ECUDA, "device error word: %s", cudaGetErrorString(cudaGetLastError()));
+    *bits |= value;
+    return ANN_OK;
+}
+
+}  // namespace ann
+
+extern "C" {
+
+int ann_kv_cache_append_q8_f32(ann_stream s, const ann_view* k_new, const ann_view* v_new, const ann_view* k_cache,
+                               const ann_view* v_cache, const ann_view* k_scale, const ann_view* v_scale,
+                               const ann_view* positions, const ann_view* counts, uint32_t tokens_per_scale,
+                               int32_t kv_layout) {
+    ANN_API_BEGIN
+    return ann::append(s, k_new, v_new, k_cache, v_cache, k_scale, v_scale, positions, counts, tokens_per_scale,
+                       kv_layout);
+    ANN_API_END
+}
+
+int ann_kv_cache_read_q8_f32(ann_stream s, const ann_view* k_cache, const ann_view* v_cache, const ann_view* k_scale,
+                             const ann_view* v_scale, const ann_view* k_out, const ann_view* v_out,
+                             const ann_view* lengths, uint32_t tokens_per_scale, int32_t kv_layout) {
+    ANN_API_BEGIN
+    return ann::read_back(s, k_cache, v_cache, k_scale, v_scale, k_out, v_out, lengths, tokens_per_scale, kv_layout);
+    ANN_API_END
+}
+
+}  // extern "C"

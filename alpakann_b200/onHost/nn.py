@@ -288,6 +288,140 @@ def attentionPrefillMirror(queue, exec, Q, K, V, out, outMirror, scale=None, que
                                               int(kvLayout), 1 if causal else 0))
 
 
+# ---- decode on compressed data -----------------------------------------------
+# No reference counterpart: rotary positions with a position per token, the KV
+# cache in 8 bits, linear layers with 4-bit weights.
+class RotaryPairs(enum.IntEnum):
+    """Elements of a head vector that rotary turns together."""
+    interleaved = 0  # (2p, 2p + 1), as rope
+    halves = 1       # (p, p + P), P = number of frequencies
+
+
+def _typed(name, dtypes, **tensors):
+    """Element types of a call, and one CUDA device for all of it."""
+    for what, t in tensors.items():
+        want = dtypes.get(what, torch.float32)
+        if t is not None and t.dtype != want and not (want == torch.int32 and t.dtype == torch.uint32):
+            raise TypeError(f"{name}: {what} must be {want}, got {t.dtype}")
+    dev = None
+    for what, t in tensors.items():
+        if t is None or t.device == dev:
+            continue
+        if dev is not None:
+            raise ValueError(f"{name}: {what} is on {t.device}, other tensors on {dev}")
+        dev = t.device
+        if dev.type != "cuda":
+            raise ValueError(f"{name} needs CUDA tensors, got {what} on {dev}")
+    return dev
+
+
+def _call(name, queue, dev, *args):
+    """The C call on `queue`, or on the current stream of the tensors' device."""
+    f = getattr(lib, name)
+    if isinstance(queue, torch.cuda.Stream) and queue.device != dev:
+        raise ValueError(f"{name}: the stream is on {queue.device}, the tensors on {dev}")
+    stream = torch.cuda.current_stream(dev).cuda_stream if queue is None else handle(queue)
+    if torch.cuda.current_device() == dev.index:
+        check(f(stream, *args))
+    else:
+        with torch.cuda.device(dev):
+            check(f(stream, *args))
+
+
+def _ref(t):
+    return None if t is None else ref(t)
+
+
+def rotaryFrequencies(queue, exec, frequencies, base=10000.0, factor=1.0, trainedLength=0, lowTurns=1.0,
+                      highTurns=32.0):
+    """frequencies[p] = base^(-p/P) into a float64 vector of P pairs. For contexts
+    `factor` times the trained ones: every frequency divided by factor
+    (trainedLength 0), or by parts: those that turn more than highTurns times
+    over trainedLength tokens are kept, those below lowTurns divided, the ones
+    between blended linearly."""
+    dev = _typed("rotaryFrequencies", {"frequencies": torch.float64}, frequencies=frequencies)
+    _call("ann_rotary_frequencies", queue, dev, ref(frequencies), float(base), float(factor), float(trainedLength),
+          float(lowTurns), float(highTurns))
+
+
+def rotary(queue, exec, q, k, positions, frequencies, outQ, outK, pairs=RotaryPairs.interleaved, layout=BTHD,
+           magnitude=1.0, inverse=False):
+    """q and k (k and outK may be None) turned by the angles positions *
+    frequencies into outQ and outK, which may be q and k themselves. positions:
+    int32 [B,T] or [T]; frequencies: float64, P <= D/2 pairs; elements from 2P
+    on are copied. inverse applies the transposed rotation: the gradients of q
+    and k from those of outQ and outK."""
+    sfx = suffix(q, k, outQ, outK)
+    dev = _typed("rotary", {"q": q.dtype, "k": q.dtype, "outQ": q.dtype, "outK": q.dtype, "positions": torch.int32,
+                            "frequencies": torch.float64},
+                 q=q, k=k, positions=positions, frequencies=frequencies, outQ=outQ, outK=outK)
+    _call(f"ann_rotary_{sfx}", queue, dev, ref(q), _ref(k), ref(positions), ref(frequencies), ref(outQ), _ref(outK),
+          int(pairs), int(layout), float(magnitude), 1 if inverse else 0)
+
+
+_CACHE_TYPES = {"kCache": torch.int8, "vCache": torch.int8, "positions": torch.int32, "counts": torch.int32,
+                "lengths": torch.int32}
+
+
+def kvCacheAppendQ8(queue, exec, kNew, vNew, kCache, vCache, kScale, vScale, positions, tokensPerScale, counts=None,
+                    kvLayout=BHTD):
+    """New K/V rows (float32 BTHD [B,Tn,Hkv,D]) into int8 caches [B,Hkv,Tcap,D]
+    at tokens [positions[b], positions[b] + counts[b]) (int32 [B]; counts
+    defaults to Tn). kScale, vScale: float32 [B, Hkv, ceil(Tcap /
+    tokensPerScale)], one scale per head and block of tokens; a block whose
+    scale grows has its earlier tokens rounded anew."""
+    dev = _typed("kvCacheAppendQ8", _CACHE_TYPES, kNew=kNew, vNew=vNew, kCache=kCache, vCache=vCache, kScale=kScale,
+                 vScale=vScale, positions=positions, counts=counts)
+    _call("ann_kv_cache_append_q8_f32", queue, dev, ref(kNew), ref(vNew), ref(kCache), ref(vCache), ref(kScale),
+          ref(vScale), ref(positions), _ref(counts), int(tokensPerScale), int(kvLayout))
+
+
+def kvCacheReadQ8(queue, exec, kCache, vCache, kScale, vScale, kOut, vOut, tokensPerScale, lengths=None,
+                  kvLayout=BHTD):
+    """The float32 rows that an 8-bit cache stands for, for the tokens before
+    lengths[b] (int32 [B], default all of kOut); rows behind are left as they
+    were. Feeds attentionPrefill with a cached prefix."""
+    dev = _typed("kvCacheReadQ8", _CACHE_TYPES, kCache=kCache, vCache=vCache, kScale=kScale, vScale=vScale, kOut=kOut,
+                 vOut=vOut, lengths=lengths)
+    _call("ann_kv_cache_read_q8_f32", queue, dev, ref(kCache), ref(vCache), ref(kScale), ref(vScale), ref(kOut),
+          ref(vOut), _ref(lengths), int(tokensPerScale), int(kvLayout))
+
+
+def attentionDecodeQ8(queue, exec, Q, kCache, vCache, kScale, vScale, out, tokensPerScale, lengths=None, scale=None,
+                      queriesPerKvGroup=1, kvLayout=BHTD, causal=True):
+    """attentionDecode over an 8-bit cache (kvCacheAppendQ8): Q, out float32
+    [B,Tq,Hq,D], the last Tq tokens of sequences of lengths[b] keys (int32 [B],
+    default the whole cache). causal: query i sees the keys before
+    lengths[b] - Tq + 1 + i; a query that sees none gives zeros. scale defaults
+    to 1/sqrt(D)."""
+    dev = _typed("attentionDecodeQ8", _CACHE_TYPES, Q=Q, kCache=kCache, vCache=vCache, kScale=kScale, vScale=vScale,
+                 out=out, lengths=lengths)
+    if scale is None:
+        scale = 1.0 / math.sqrt(Q.shape[3])
+    _call("ann_attention_decode_q8_f32", queue, dev, ref(Q), ref(kCache), ref(vCache), ref(kScale), ref(vScale),
+          _ref(lengths), ref(out), float(scale), int(queriesPerKvGroup), int(tokensPerScale), int(kvLayout),
+          1 if causal else 0)
+
+
+def packWeightQ4(queue, exec, weight, packed, scales, groupSize):
+    """A float32 weight [K,N] (row-major [in, out]) in 4 bits: packed int32
+    [K/8,N], eight inputs a word, scales float32 [ceil(K/groupSize),N]. Once,
+    when the weights are loaded."""
+    dev = _typed("packWeightQ4", {"packed": torch.int32}, weight=weight, packed=packed, scales=scales)
+    _call("ann_pack_weight_q4_f32", queue, dev, ref(weight), ref(packed), ref(scales), int(groupSize))
+
+
+def linearQ4(queue, exec, input, packed, scales, output, groupSize, bias=None, activation=Activation.none,
+             residual=None):
+    """output = activation(input . W + bias) + residual with W in 4 bits
+    (packWeightQ4): linear, linearBias and outputProjectionResidual for the few
+    rows of a decode step. residual may be output."""
+    dev = _typed("linearQ4", {"packed": torch.int32}, input=input, packed=packed, scales=scales, output=output,
+                 bias=bias, residual=residual)
+    _call("ann_linear_q4_f32", queue, dev, ref(input), ref(packed), ref(scales), _ref(bias), _ref(residual),
+          ref(output), int(groupSize), int(activation))
+
+
 def raise_shape(msg):
     from .._capi import ANN_EINVAL, AnnShapeError
     raise AnnShapeError(ANN_EINVAL, msg)

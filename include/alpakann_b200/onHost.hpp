@@ -21,6 +21,7 @@
 
 #include <array>
 #include <cmath>
+#include <cstddef>
 #include <cstdint>
 #include <cstdio>
 #include <cstdlib>
@@ -841,6 +842,120 @@ void attentionPrefillMirror(auto& queue, auto /*exec*/, auto const& Q, auto cons
     else
         d::check(ann_attention_prefill_mirror_f64(d::stream_of(queue), &q, &k, &v, &o, outMirror, scale,
                                                   queriesPerKvGroup, static_cast<int32_t>(kvLayout), causal ? 1 : 0));
+}
+
+// ---- decode on compressed data (no reference counterpart; include/ann_b200.h) ----
+// Optional views are pointers, nullptr = not given.
+enum class RotaryPairs { interleaved = ANN_ROTARY_INTERLEAVED, halves = ANN_ROTARY_HALVES };
+
+namespace detail {
+// An optional view and its descriptor (nullptr stays NULL).
+struct OptionalView {
+    ann_view view{};
+    bool given = false;
+    OptionalView(std::nullptr_t) {}
+    template <typename V>
+    OptionalView(V const* v) : given(v != nullptr) {
+        if (given) view = alpaka::nn::b200::detail::to_ann(*v);
+    }
+    ann_view const* get() const { return given ? &view : nullptr; }
+};
+template <typename E, typename V>
+constexpr bool holds = std::is_same_v<alpaka::nn::b200::detail::elem_of<V>, E>;
+// int32 or uint32 words of the same bits
+template <typename V>
+constexpr bool holds_words = holds<int32_t, V> || holds<uint32_t, V>;
+}  // namespace detail
+
+// frequencies (double, rank 1) of rotary, scaled for contexts `factor` times the
+// trained ones: everywhere (trainedLength 0) or by parts.
+void rotaryFrequencies(auto& queue, auto /*exec*/, auto& frequencies, double base = 10000.0, double factor = 1.0,
+                       double trainedLength = 0.0, double lowTurns = 1.0, double highTurns = 32.0) {
+    namespace d = alpaka::nn::b200::detail;
+    static_assert(detail::holds<double, std::remove_cvref_t<decltype(frequencies)>>, "frequencies are double");
+    auto f = d::to_ann(frequencies);
+    d::check(ann_rotary_frequencies(d::stream_of(queue), &f, base, factor, trainedLength, lowTurns, highTurns));
+}
+
+// q and k turned by positions (int32 [B,T] or [T]) * frequencies into outQ and
+// outK, which may be q and k; inverse = the transposed rotation (gradient).
+template <typename T_Type>
+void rotary(auto& queue, auto /*exec*/, auto const& q, auto const& k, auto const& positions, auto const& frequencies,
+            auto& outQ, auto& outK, RotaryPairs pairs = RotaryPairs::interleaved,
+            alpaka::nn::RopeLayout layout = alpaka::nn::RopeLayout::BTHD, T_Type magnitude = T_Type(1),
+            bool inverse = false) {
+    namespace d = alpaka::nn::b200::detail;
+    d::require_float<T_Type>();
+    static_assert(detail::holds_words<std::remove_cvref_t<decltype(positions)>>, "positions are int32");
+    static_assert(detail::holds<double, std::remove_cvref_t<decltype(frequencies)>>, "frequencies are double");
+    auto a = d::to_ann(q), b = d::to_ann(k), p = d::to_ann(positions), f = d::to_ann(frequencies);
+    auto oa = d::to_ann(outQ), ob = d::to_ann(outK);
+    auto const pr = static_cast<int32_t>(pairs), lay = static_cast<int32_t>(layout);
+    if constexpr (d::is_f32<T_Type>)
+        d::check(ann_rotary_f32(d::stream_of(queue), &a, &b, &p, &f, &oa, &ob, pr, lay, magnitude, inverse ? 1 : 0));
+    else
+        d::check(ann_rotary_f64(d::stream_of(queue), &a, &b, &p, &f, &oa, &ob, pr, lay, magnitude, inverse ? 1 : 0));
+}
+
+// New rows (float BTHD) into int8 caches with a scale per head and block of tokens.
+void kvCacheAppendQ8(auto& queue, auto /*exec*/, auto const& kNew, auto const& vNew, auto& kCache, auto& vCache,
+                     auto& kScale, auto& vScale, auto const& positions, uint32_t tokensPerScale,
+                     detail::OptionalView counts = nullptr,
+                     alpaka::nn::AttentionKvLayout kvLayout = alpaka::nn::AttentionKvLayout::BHTD) {
+    namespace d = alpaka::nn::b200::detail;
+    static_assert(detail::holds<int8_t, std::remove_cvref_t<decltype(kCache)>>, "the caches are int8");
+    static_assert(detail::holds_words<std::remove_cvref_t<decltype(positions)>>, "positions are int32");
+    auto kn = d::to_ann(kNew), vn = d::to_ann(vNew), kc = d::to_ann(kCache), vc = d::to_ann(vCache);
+    auto ks = d::to_ann(kScale), vs = d::to_ann(vScale), p = d::to_ann(positions);
+    d::check(ann_kv_cache_append_q8_f32(d::stream_of(queue), &kn, &vn, &kc, &vc, &ks, &vs, &p, counts.get(),
+                                        tokensPerScale, static_cast<int32_t>(kvLayout)));
+}
+
+// The float rows that an 8-bit cache stands for.
+void kvCacheReadQ8(auto& queue, auto /*exec*/, auto const& kCache, auto const& vCache, auto const& kScale,
+                   auto const& vScale, auto& kOut, auto& vOut, uint32_t tokensPerScale,
+                   detail::OptionalView lengths = nullptr,
+                   alpaka::nn::AttentionKvLayout kvLayout = alpaka::nn::AttentionKvLayout::BHTD) {
+    namespace d = alpaka::nn::b200::detail;
+    static_assert(detail::holds<int8_t, std::remove_cvref_t<decltype(kCache)>>, "the caches are int8");
+    auto kc = d::to_ann(kCache), vc = d::to_ann(vCache), ks = d::to_ann(kScale), vs = d::to_ann(vScale);
+    auto ko = d::to_ann(kOut), vo = d::to_ann(vOut);
+    d::check(ann_kv_cache_read_q8_f32(d::stream_of(queue), &kc, &vc, &ks, &vs, &ko, &vo, lengths.get(), tokensPerScale,
+                                      static_cast<int32_t>(kvLayout)));
+}
+
+// attentionDecode over an 8-bit cache; Q, out float BTHD, the last Tq tokens.
+void attentionDecodeQ8(auto& queue, auto /*exec*/, auto const& Q, auto const& kCache, auto const& vCache,
+                       auto const& kScale, auto const& vScale, auto& out, uint32_t tokensPerScale,
+                       detail::OptionalView lengths, float scale, uint32_t queriesPerKvGroup = 1u,
+                       alpaka::nn::AttentionKvLayout kvLayout = alpaka::nn::AttentionKvLayout::BHTD,
+                       bool causal = true) {
+    namespace d = alpaka::nn::b200::detail;
+    static_assert(detail::holds<int8_t, std::remove_cvref_t<decltype(kCache)>>, "the caches are int8");
+    auto q = d::to_ann(Q), kc = d::to_ann(kCache), vc = d::to_ann(vCache), ks = d::to_ann(kScale);
+    auto vs = d::to_ann(vScale), o = d::to_ann(out);
+    d::check(ann_attention_decode_q8_f32(d::stream_of(queue), &q, &kc, &vc, &ks, &vs, lengths.get(), &o, scale,
+                                         queriesPerKvGroup, tokensPerScale, static_cast<int32_t>(kvLayout),
+                                         causal ? 1 : 0));
+}
+
+// A float weight [in, out] in 4 bits with a scale per group of inputs and column.
+void packWeightQ4(auto& queue, auto /*exec*/, auto const& weight, auto& packed, auto& scales, uint32_t groupSize) {
+    namespace d = alpaka::nn::b200::detail;
+    static_assert(detail::holds_words<std::remove_cvref_t<decltype(packed)>>, "packed weights are 32-bit words");
+    auto w = d::to_ann(weight), p = d::to_ann(packed), s = d::to_ann(scales);
+    d::check(ann_pack_weight_q4_f32(d::stream_of(queue), &w, &p, &s, groupSize));
+}
+
+// output = activation(input . W + bias) + residual with W in 4 bits.
+void linearQ4(auto& queue, auto /*exec*/, auto const& input, auto const& packed, auto const& scales, auto& output,
+              uint32_t groupSize, detail::OptionalView bias = nullptr, Activation activation = Activation::none,
+              detail::OptionalView residual = nullptr) {
+    namespace d = alpaka::nn::b200::detail;
+    static_assert(detail::holds_words<std::remove_cvref_t<decltype(packed)>>, "packed weights are 32-bit words");
+    auto x = d::to_ann(input), p = d::to_ann(packed), s = d::to_ann(scales), o = d::to_ann(output);
+    d::check(ann_linear_q4_f32(d::stream_of(queue), &x, &p, &s, bias.get(), residual.get(), &o, groupSize,
+                               static_cast<int32_t>(activation)));
 }
 
 }  // namespace alpaka::nn::onHost::nn

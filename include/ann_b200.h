@@ -55,6 +55,7 @@ extern "C" {
 /* Device error word bits (ann_take_device_error). */
 #define ANN_DEVERR_TOKEN_ID 0x1u     /* embeddingLookup saw an id >= vocabulary rows      */
 #define ANN_DEVERR_WAIT_TIMEOUT 0x2u /* a kernel gave up waiting for its own copies (1 s) */
+#define ANN_DEVERR_CACHE_RANGE 0x4u  /* kvCacheAppendQ8 saw a row outside the cache       */
 
 typedef void* ann_stream; /* cudaStream_t */
 typedef struct ann_comm_s* ann_comm; /* one rank of the node's NCCL communicator */
@@ -462,6 +463,104 @@ int ann_signal_barrier(ann_stream stream, uint32_t* signals, uint32_t* const* pe
                        int32_t rank, uint32_t epoch, uint64_t timeout_ns);
 int ann_signal_barrier_dev(ann_stream stream, uint32_t* signals, uint32_t* const* peer_signals, int32_t nranks,
                            int32_t rank, uint32_t* epoch_word, uint64_t timeout_ns);
+
+/* ---- decode on compressed data ------------------------------------------------
+ * No reference counterpart: rotary positions with a position per token, the KV
+ * cache in 8 bits and linear layers with 4-bit weights, for decode steps bound
+ * by the cache's and the weights' bytes. Outputs must not have a zero pitch on
+ * an axis longer than one; inputs may (a broadcast view). No call allocates
+ * device memory or waits, so each can be captured in a CUDA graph.
+ *
+ * rotary: for pair p of a head vector at position t, a = t * frequencies[p] in
+ * 64 bits, (x0, x1) -> magnitude * (x0 cos a - x1 sin a, x0 sin a + x1 cos a).
+ * Pairs are elements (2p, 2p+1) (ANN_ROTARY_INTERLEAVED, rope's) or (p, p + P)
+ * (ANN_ROTARY_HALVES), P = len(frequencies) <= D/2; elements from 2P on are
+ * copied. q, k, out_q, out_k: BTHD or BHTD by `layout`; k and out_k are both
+ * NULL or both given, with their own head count; out may be the input itself
+ * (in place) but must not overlap it otherwise. positions: int32 [B,T], or [T]
+ * for every sequence; any value, negative ones turn backwards. frequencies:
+ * rank-1 float64 in either type of call. inverse != 0 applies the transposed
+ * rotation: the gradient of rotary with respect to its input, given the
+ * gradient of its output (same magnitude). ANN_EINVAL for an odd head
+ * dimension or other extents. */
+#define ANN_ROTARY_INTERLEAVED 0
+#define ANN_ROTARY_HALVES 1
+int ann_rotary_f32(ann_stream stream, const ann_view* q, const ann_view* k, const ann_view* positions,
+                   const ann_view* frequencies, const ann_view* out_q, const ann_view* out_k, int32_t pairs,
+                   int32_t layout, float magnitude, int32_t inverse);
+int ann_rotary_f64(ann_stream stream, const ann_view* q, const ann_view* k, const ann_view* positions,
+                   const ann_view* frequencies, const ann_view* out_q, const ann_view* out_k, int32_t pairs,
+                   int32_t layout, double magnitude, int32_t inverse);
+/* frequencies[p] = base^(-p/P), P = len(frequencies), scaled for contexts
+ * `factor` times the trained ones: divided by factor everywhere when
+ * trained_length is 0 (factor 1: unscaled), else by parts (Peng et al., "YaRN",
+ * 2023, section 3.2): with r = trained_length * f / (2 pi) full turns over the
+ * trained length and w = clamp((r - low_turns) / (high_turns - low_turns), 0, 1),
+ * f' = f * (w + (1 - w) / factor). */
+int ann_rotary_frequencies(ann_stream stream, const ann_view* frequencies, double base, double factor,
+                           double trained_length, double low_turns, double high_turns);
+
+/* The 8-bit cache: k_cache, v_cache int8, BHTD [B,Hkv,Tcap,D] or BTHD by
+ * kv_layout; k_scale, v_scale float32 [B, Hkv, ceil(Tcap / tokens_per_scale)].
+ * A cached value n stands for n * scale of its head and block of
+ * tokens_per_scale tokens.
+ *
+ * Append: k_new, v_new float32 BTHD [B,Tn,Hkv,D] become tokens
+ * [positions[b], positions[b] + counts[b]) of sequence b (positions, counts:
+ * int32 [B]; counts NULL = Tn, values are held to [0, Tn]; rows past the count
+ * are padding and not read). A touched block's scale becomes the larger of
+ * max|x| / 127 over its new rows and, if it holds tokens before positions[b],
+ * its old scale (its absolute value, should a caller have stored a negative
+ * one); new values are the whole numbers nearest to the exact quotient
+ * x / scale (ties to even, within [-127, 127]); where the scale grew, the
+ * block's earlier values are rounded anew from n * old / new. Tokens of a
+ * touched block after the new rows are left as they were and are not part of
+ * the sequence any more. A NaN or infinite input makes its block's scale NaN or
+ * infinite and its integers 0. Rows outside [0, Tcap) are dropped and set
+ * ANN_DEVERR_CACHE_RANGE. */
+int ann_kv_cache_append_q8_f32(ann_stream stream, const ann_view* k_new, const ann_view* v_new,
+                               const ann_view* k_cache, const ann_view* v_cache, const ann_view* k_scale,
+                               const ann_view* v_scale, const ann_view* positions, const ann_view* counts,
+                               uint32_t tokens_per_scale, int32_t kv_layout);
+/* Read-back: k_out, v_out float32 in the cache's layout and extents, or with
+ * fewer tokens: out = n * scale for the tokens before lengths[b] (int32 [B],
+ * NULL = all); later rows of the output are left as they were. Feeds
+ * ann_attention_prefill_f32 with a cached prefix. */
+int ann_kv_cache_read_q8_f32(ann_stream stream, const ann_view* k_cache, const ann_view* v_cache,
+                             const ann_view* k_scale, const ann_view* v_scale, const ann_view* k_out,
+                             const ann_view* v_out, const ann_view* lengths, uint32_t tokens_per_scale,
+                             int32_t kv_layout);
+/* Attention of the last Tq tokens of every sequence over the cache: q, out
+ * float32 BTHD [B,Tq,Hq,D]; query head hq reads KV head hq / g. lengths: int32
+ * [B] keys per sequence, held to [0, Tcap] (NULL = Tcap). causal != 0: query i
+ * sees the keys before lengths[b] - Tq + 1 + i (all of them for Tq = 1); else
+ * every query sees lengths[b] keys. A query that sees no key gives a row of
+ * zeros. Scores, softmax and sums are held to fp32 accuracy. ANN_ENOTSUP
+ * unless D is 64, 128 or 256, tokens_per_scale a power of two of 16 or more,
+ * and head vectors unit-stride with 16-byte aligned rows. */
+int ann_attention_decode_q8_f32(ann_stream stream, const ann_view* q, const ann_view* k_cache,
+                                const ann_view* v_cache, const ann_view* k_scale, const ann_view* v_scale,
+                                const ann_view* lengths, const ann_view* out, float scale,
+                                uint32_t queries_per_kv_group, uint32_t tokens_per_scale, int32_t kv_layout,
+                                int32_t causal);
+
+/* 4-bit weights: packed int32 [K/8, N], word (r, n) holding inputs 8r .. 8r+7
+ * of column n in its nibbles, the lowest first; scales float32
+ * [ceil(K / group_size), N]. Nibble u stands for (u - 8) * scale of its group of
+ * group_size consecutive inputs and its column. K is a multiple of 8,
+ * group_size of 32.
+ * pack: weight float32 [K,N] row-major [in, out]; scale = max|w| / 7 of the
+ * group, u - 8 the whole number nearest to the exact quotient w / scale (ties to
+ * even, within [-7, 7]); a group with a NaN or infinite weight gets that scale
+ * and integers 0. */
+int ann_pack_weight_q4_f32(ann_stream stream, const ann_view* weight, const ann_view* packed, const ann_view* scales,
+                           uint32_t group_size);
+/* output [M,N] = act(input [M,K] . W + bias) + residual; bias (rank 1 [N]) and
+ * residual ([M,N], may be output) may be NULL, act is ANN_ACT_*. Meant for the few rows of
+ * a decode step (the weights are read once per 16 rows). */
+int ann_linear_q4_f32(ann_stream stream, const ann_view* input, const ann_view* packed, const ann_view* scales,
+                      const ann_view* bias, const ann_view* residual, const ann_view* output, uint32_t group_size,
+                      int32_t act);
 
 /* ---- flat model artifacts: onHost/core/binary.hpp ------------------------
  * TensorSpec (binary.hpp:33-39): one tensor of a little-endian ".bin" file of
