@@ -65,7 +65,11 @@ def attend(q, kc, vc, ks, vs, lengths, block, scale, g, causal=True):
     a bound on a float32 implementation's error, whatever its order of sums:
     d = scale * max_j sum_d |q k| * (D u 2 + 2^-20) for a score (products of
     operands split into parts of 22 bits or more among them), 2 d + (n + 8) 2 u of
-    sum p |v| for the output."""
+    sum p |v| for the output. A probability in two fp16 parts, scaled so that the
+    row's largest is 2^13 or more, is a multiple of fp16's smallest number 2^-24:
+    off by at most 2^-25 / 2^13 = 2^-38 of the largest, which matters where the
+    keys of large p have v = 0: n 2^-38 max |v| more (p relative to the largest is
+    at least p itself)."""
     B, Tq, Hq, D = q.shape
     T = kc.shape[2]
     blk = np.arange(T) // block
@@ -85,7 +89,7 @@ def attend(q, kc, vc, ks, vs, lengths, block, scale, g, causal=True):
                 p /= p.sum()
                 out[b, i, h] = p @ v
                 d = abs(scale) * (np.abs(k) @ np.abs(qq)).max() * (2 * D * U + 2.0 ** -20)
-                tol[b, i, h] = (2 * d + (n + 8) * 2 * U) * (p @ np.abs(v)) + 1e-30
+                tol[b, i, h] = (2 * d + (n + 8) * 2 * U) * (p @ np.abs(v)) + n * 2.0 ** -38 * np.abs(v).max(0) + 1e-30
     return out, tol
 
 
