@@ -9,11 +9,13 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cstdlib>
 #include <mutex>
 #include <set>
 
 #include "common.cuh"
 #include "reduce.cuh"
+#include "tma.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -43,58 +45,99 @@ struct DecodeQ8Args {
     float scale;
 };
 
-// How the products are formed. An int8 value is exact in fp16, a float32 value is
-// the sum of two fp16 parts (11 bits each, the row scaled by a power of two so
-// that both are normal numbers), and mma.sync adds exact products of fp16 in
-// float32. An m16n8k16 product takes 16 rows: eight query rows' high parts and
-// the same rows' low parts, so one instruction gives both halves of eight rows,
-// in the same thread, at float32 accuracy. The probabilities go through the same
-// split on their way to the product with V.
+// How the products are formed. q.k in whole numbers: a row of q is rounded to 31
+// bits of its largest value and cut into four 8-bit digits, so that
+// mma.sync.m16n8k32 on int8 multiplies the cache's bytes as they are -- one
+// product holds the high two digits of eight query rows, another the low two --
+// and the sums are exact. p.v in halves: a cached value is exact in fp16, a
+// probability is the sum of two fp16 parts (22 bits), and mma.sync.m16n8k16 adds
+// the exact products in fp32; again one product holds both parts of eight rows,
+// in the same thread. (On this GPU an int8 product of depth 32 and an fp16 one
+// of depth 16 take the same time, 2.1 cycles of an SM: 8 KB of cache cost 64 of
+// them, 0.4 of the time that HBM takes to deliver it.)
 //
 // How the cache reaches the fragments. The order of the summed index and of the
 // output columns of a matrix product is free as long as both operands agree, so
-// a lane takes the bytes that one wide load gives it: 16 consecutive elements of
-// a key's row for q.k (four lanes cover 64 bytes of a key), 16 consecutive
-// elements of four keys for p.v (eight lanes cover a row). No shared memory, no
-// transposition: a warp loads its keys straight to registers, the next tile's
-// while it works on this one.
+// a lane takes whole 16-byte pieces: of one key's row for q.k (four lanes cover a
+// key), of four keys at the same elements for p.v (eight lanes cover a row). No
+// transposition is needed. Every warp streams tiles of KT keys of its own through
+// a ring of two tiles in shared memory (cp.async, 16 bytes a lane, rows of 128
+// bytes coalesced), one tile ahead of the one it works on: 8 to 16 KB in flight
+// a warp, 12 warps an SM, where HBM's latency asks for 40 KB an SM. The pieces
+// are placed so that both kinds of reads are free of bank conflicts.
 //
-// Every warp takes tiles of KT keys of its own, keeps a running maximum and sum
-// per row (base 2), and adds each tile's p.v from a fresh accumulator, so no sum
-// of more than KT products is left to the tensor core's own rounding. Warps meet
-// in shared memory, the CTAs of a cluster (the key range's splits) in
-// distributed shared memory; no scratch memory, no atomics, one launch, and a
-// fixed order of sums.
-constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;
+// Every warp keeps a running maximum and sum per row (base 2) and adds each
+// tile's p.v from a fresh accumulator, so no sum of more than KT products is left
+// to the tensor core's own rounding. Warps meet in shared memory; the CTAs of a
+// cluster (the key range's splits) send their parts into each other's shared
+// memory, where each CTA sums its share of the output: one cluster barrier, no
+// scratch memory, no atomics, one launch, and a fixed order of sums.
 constexpr int kMaxCluster = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <int D, int MT>
+template <int D, int MT, int W>
 struct Q8 {
+    static constexpr int THREADS = 32 * W;
     static constexpr int KT = D <= 128 ? 32 : 16;  // keys per tile of a warp
     static constexpr int ROWS = 8 * MT;            // query rows of a CTA
-    static constexpr int KS = D / 16;              // k16 steps of q.k
+    static constexpr int KS = D / 32;              // k32 steps of q.k
     static constexpr int NK = KT / 8;              // n8 tiles of keys
     static constexpr int KV = KT / 16;             // k16 steps of p.v, groups of 16 keys
     static constexpr int VW = D / 32;              // words of V per lane and key
     static constexpr int KW = D / 16;              // words of K per lane and key
-    static constexpr bool QREG = MT * KS <= 8;     // q's fragments in registers
-    static constexpr size_t OFF_Q = 0;                                        // uint4 [MT][KS][32]
-    static constexpr size_t OFF_O = OFF_Q + size_t{16} * MT * KS * 32;        // float [kWarps][ROWS][D]
-    static constexpr size_t OFF_ML = OFF_O + sizeof(float) * kWarps * ROWS * D;  // float [2][kWarps][ROWS]
-    static constexpr size_t OFF_F = OFF_ML + sizeof(float) * 2 * kWarps * ROWS;  // float [ROWS]: score factors
-    static constexpr size_t OFF_X = OFF_F + sizeof(float) * ROWS;             // float [2][ROWS]: this CTA's max, sum
-    static constexpr size_t OFF_W = OFF_X + sizeof(float) * 2 * ROWS;         // float [kMaxCluster][ROWS], then [ROWS]
-    static constexpr size_t SMEM = OFF_W + sizeof(float) * (kMaxCluster + 1) * ROWS;
+    static constexpr bool QREG = MT * KS <= 4;     // q's fragments in registers
+    static constexpr int TILE = KT * D;            // bytes of a tile of K or V
+    static constexpr int RING = 4 * TILE;          // K, V, K, V of a warp; its output rows at the end
+    static constexpr size_t OFF_Q = size_t{1} * RING * W;                      // uint4 [MT][KS][2][32]
+    static constexpr size_t OFF_R = OFF_Q + size_t{32} * MT * KS * 32;         // float4 [ROWS * D / 4 + kMaxCluster]
+    static constexpr size_t OFF_ML = OFF_R + sizeof(float) * (ROWS * D + 4 * kMaxCluster);  // float [2][W][ROWS]
+    static constexpr size_t OFF_F = OFF_ML + sizeof(float) * 2 * W * ROWS;     // float [ROWS]: score factors
+    static constexpr size_t OFF_X = OFF_F + sizeof(float) * ROWS;              // float [kMaxCluster][2][ROWS]: max, sum
+    static constexpr size_t SMEM = OFF_X + sizeof(float) * kMaxCluster * 2 * ROWS;
+    static_assert(RING >= static_cast<int>(sizeof(float)) * ROWS * D, "a warp's output rows fit its ring");
+    // 16-byte piece c of row r of a tile, with the pieces of a 128-byte line
+    // permuted: K is read by 8 lanes as two rows x every other piece (or four), V
+    // as every other row of 8 x two neighbouring pieces (or halves of them).
+    static __device__ __forceinline__ uint32_t place(int r, int c) {
+        if constexpr (D == 64) {
+            int const line = r >> 1, q = (r & 1) * 4 + c;
+            return line * 128 + ((q ^ ((line & 1) << 2) ^ (line & 2)) << 4);
+        } else {
+            return r * D + (c >> 3) * 128 + (((c & 7) ^ (r & 7)) << 4);
+        }
+    }
+    // Piece i of lane t for q.k.
+    static __device__ __forceinline__ int piece(int i, int t) { return D == 64 ? t : 8 * (i >> 1) + 2 * t + (i & 1); }
 };
 
-__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-    asm(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+// c += a b (or c = a b): fp16 products of depth 16, summed in fp32.
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t const (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t const (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// int8 products of depth 32, exact in int32.
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint4 a, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8_first(int (&c)[4], uint4 a, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "r"(0));
+}
+
+// 2^x for x <= 0; results below 2^-126 are 0.
+__device__ __forceinline__ float exp2_neg(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 // Two unsigned bytes u (= n + 128) of w picked by `sel` as fp16 whole numbers n:
@@ -114,34 +157,32 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
     lo = *reinterpret_cast<uint32_t const*>(&l);
 }
 
-__device__ __forceinline__ uint4 load16(const int8_t* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p));
-    return v;
+// 16 bytes from global to shared memory, asynchronously, in the thread's open group.
+__device__ __forceinline__ void copy16(uint32_t dst, const int8_t* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ uint2 load8(const int8_t* p) {
-    uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
+__device__ __forceinline__ void copies_close() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the newest N groups have landed, for every lane of the warp.
+template <int N>
+__device__ __forceinline__ void copies_landed() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+    __syncwarp();
 }
 
 // 2^(e - 127) for a biased exponent e in [1, 254].
 __device__ __forceinline__ float pow2_biased(int e) { return __int_as_float(e << 23); }
 
-template <int D, int MT>
-__global__ void __launch_bounds__(kThreads, MT == 1 && D <= 128 ? 3 : 2) decode_q8_kernel(DecodeQ8Args a) {
-    using C = Q8<D, MT>;
-    extern __shared__ __align__(16) unsigned char smem[];
+template <int D, int MT, int W>
+__global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 : 2)) decode_q8_kernel(DecodeQ8Args a) {
+    using C = Q8<D, MT, W>;
+    extern __shared__ __align__(128) unsigned char smem[];
     uint4* sq = reinterpret_cast<uint4*>(smem + C::OFF_Q);
-    float* so = reinterpret_cast<float*>(smem + C::OFF_O);
     float* sml = reinterpret_cast<float*>(smem + C::OFF_ML);
     float* sf = reinterpret_cast<float*>(smem + C::OFF_F);
     float* sx = reinterpret_cast<float*>(smem + C::OFF_X);
-    float* sw = reinterpret_cast<float*>(smem + C::OFF_W);
     int const tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     int const split = static_cast<int>(blockIdx.x) % a.splits;
+    if (a.splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // "this CTA runs"
     int64_t unit = blockIdx.x / a.splits;
     int64_t const row0 = (unit % a.row_tiles) * C::ROWS;  // first of the KV head's Tq * g query rows
     unit /= a.row_tiles;
@@ -151,49 +192,113 @@ __global__ void __launch_bounds__(kThreads, MT == 1 && D <= 128 ? 3 : 2) decode_
 
     int64_t len = a.cap;
     if (a.lengths != nullptr) len = min(a.cap, max(int64_t{0}, static_cast<int64_t>(a.lengths[b * a.len_s])));
+
+    // q's rows, loaded while the length is on its way
+    constexpr int RPW = (C::ROWS + W - 1) / W, QV = (D + 127) / 128;  // rows of a warp, vectors of a lane
+    float4 x[RPW][QV];
+#pragma unroll
+    for (int u = 0; u < RPW; ++u) {
+        int const r = warp + u * W;
+        int64_t const row = row0 + r, hq = kvh * a.g + row % a.g;
+        bool const given = r < rows && hq < a.Hq;
+        float const* q = a.q + b * a.q_b + (row / a.g) * a.q_t + hq * a.q_h;
+#pragma unroll
+        for (int i = 0; i < QV; ++i) {
+            int const d = 128 * i + 4 * lane;
+            x[u][i] = given && d < D ? *reinterpret_cast<float4 const*>(q + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    }
+
     // keys that row r of the tile sees; rows are ordered by token, then head
     auto visible = [&](int r) {
         int64_t const n = a.causal ? len - a.Tq + 1 + (row0 + r) / a.g : len;
         return static_cast<int>(max(int64_t{0}, n));
     };
     int const most = visible(rows - 1), least = visible(0);
+    int const tiles = (most + C::KT - 1) / C::KT;
+    int const t0 = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
+    int const t1 = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
+
+    int8_t const* kb = a.k + b * a.k_b + kvh * a.k_h;
+    int8_t const* vb = a.v + b * a.v_b + kvh * a.v_h;
+    float const* ks = a.ks + b * a.ks_b + kvh * a.ks_h;
+    float const* vs = a.vs + b * a.vs_b + kvh * a.vs_h;
+    unsigned char* const ring = smem + C::RING * warp;
+    uint32_t const ring_u = smem_u32(ring);
+    // A tile of K or V into the ring: D / 16 lanes take a row. Keys past the last
+    // one seen (of the range's last tile) read that one.
+    auto fetch = [&](uint32_t dst, int8_t const* base, int64_t stride, int tile) {
+        constexpr int LPR = D / 16, RPI = 32 / LPR;  // lanes per row, rows per instruction
+        int const r0 = lane / LPR, c = lane % LPR, key = tile * C::KT;
+        if (key + C::KT <= most) {
+            int8_t const* p = base + (key + r0) * stride + 16 * c;
+#pragma unroll
+            for (int i = 0; i < C::KT / RPI; ++i) copy16(dst + C::place(r0 + i * RPI, c), p + i * RPI * stride);
+        } else {
+#pragma unroll
+            for (int i = 0; i < C::KT / RPI; ++i)
+                copy16(dst + C::place(r0 + i * RPI, c), base + min(key + r0 + i * RPI, most - 1) * stride + 16 * c);
+        }
+    };
+    float ksc[C::KV], vsc[C::KV];
+    auto scales = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < C::KV; ++i) {
+            int const j = min(tile * C::KT + 16 * i, most - 1) >> a.block_shift;
+            ksc[i] = ks[j * a.ks_j];
+            vsc[i] = vs[j * a.vs_j];
+        }
+    };
+    int tile = t0 + warp;
+    // groups: K, V of the first tile, K, V of the second
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        if (tile + u * W < t1) fetch(ring_u + u * 2 * C::TILE, kb, a.k_t, tile + u * W);
+        copies_close();
+        if (tile + u * W < t1) fetch(ring_u + (u * 2 + 1) * C::TILE, vb, a.v_t, tile + u * W);
+        copies_close();
+    }
+    if (tile < t1) scales(tile);
 
     // q's fragments and the factor of each row's scores.
-    for (int r = warp; r < C::ROWS; r += kWarps) {
-        int64_t const row = row0 + r, hq = kvh * a.g + row % a.g;
-        bool const given = r < rows && hq < a.Hq;
-        float const* q = a.q + b * a.q_b + (row / a.g) * a.q_t + hq * a.q_h;
-        float4 x[(D + 127) / 128];
-        float top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < (D + 127) / 128; ++i) {
-            int const d = 128 * i + 4 * lane;
-            x[i] = given && d < D ? *reinterpret_cast<float4 const*>(q + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-            top = fmaxf(top, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
+    for (int u = 0; u < RPW; ++u) {
+        int const r = warp + u * W;
+        if (r >= C::ROWS) break;
+        unsigned int top = 0;  // max |q| on the bit patterns: NaN above infinity above every number
+#pragma unroll
+        for (int i = 0; i < QV; ++i) {
+            top = max(max(top, __float_as_uint(x[u][i].x) & 0x7fffffffu), __float_as_uint(x[u][i].y) & 0x7fffffffu);
+            top = max(max(top, __float_as_uint(x[u][i].z) & 0x7fffffffu), __float_as_uint(x[u][i].w) & 0x7fffffffu);
         }
-        top = warp_max(top);
-        // largest value into [2^13, 2^14): e = its biased exponent, held where the factors stay normal
-        int e = static_cast<int>(__float_as_uint(top) >> 23);
-        e = e == 255 ? 140 : max(e, 15);
-        float const up = pow2_biased(267 - e), down = pow2_biased(e - 13);  // 2^(140 - e), 2^(e - 140)
-        if (lane == 0) sf[r] = down * (a.scale * kLog2e);
+        top = __reduce_max_sync(0xffffffffu, top);
+        // the largest value into [2^29, 2^30): 2^(156 - e), e its biased exponent, where both factors are normal
+        int const e = min(max(static_cast<int>(top >> 23), 31), 254);
+        float const up = pow2_biased(283 - e), down = pow2_biased(e - 29);  // 2^(156 - e), 2^(e - 156)
+        // NaN and infinity have no whole numbers: the whole row becomes NaN
+        if (lane == 0) sf[r] = top >= 0x7f800000u ? __int_as_float(0x7fffffff) : down * (a.scale * kLog2e);
 #pragma unroll
-        for (int i = 0; i < (D + 127) / 128; ++i) {
+        for (int i = 0; i < QV; ++i) {
             int const d = 128 * i + 4 * lane;
             if (d >= D) continue;
-            uint4 f;
-            split2(x[i].x * up, x[i].y * up, f.x, f.y);
-            split2(x[i].z * up, x[i].w * up, f.z, f.w);
-            // element d = 64 c + 16 t' + 4 w of row g' sits in step 4 c + w, lane (g', t')
-            int const step = (d / 64) * 4 + (d / 4) % 4, to = (r & 7) * 4 + (d / 16) % 4;
-            sq[((r >> 3) * C::KS + step) * 32 + to] = f;
+            // signed base-256 digits: a carry out of the lower bytes, then their signs
+            auto digits = [&](float v) { return (static_cast<uint32_t>(__float2int_rn(v * up)) + 0x00808080u) ^ 0x00808080u; };
+            uint32_t const n0 = digits(x[u][i].x), n1 = digits(x[u][i].y), n2 = digits(x[u][i].z), n3 = digits(x[u][i].w);
+            uint32_t const lo01 = __byte_perm(n0, n1, 0x5140), hi01 = __byte_perm(n0, n1, 0x7362);
+            uint32_t const lo23 = __byte_perm(n2, n3, 0x5140), hi23 = __byte_perm(n2, n3, 0x7362);
+            // the lane and word of fragment that holds elements d .. d + 3
+            int const c = d / 16, at = D == 64 ? c : (c % 8) / 2;
+            int const word = 4 * (D == 64 ? 0 : 2 * (c / 8) + c % 2) + (d / 4) % 4, to = (r & 7) * 4 + at;
+            uint2* f = reinterpret_cast<uint2*>(sq + ((r >> 3) * C::KS + word / 2) * 64 + to) + word % 2;
+            f[0] = make_uint2(__byte_perm(hi01, hi23, 0x7632), __byte_perm(hi01, hi23, 0x5410));
+            f[64] = make_uint2(__byte_perm(lo01, lo23, 0x7632), __byte_perm(lo01, lo23, 0x5410));
         }
     }
     __syncthreads();
-    uint4 qf[C::QREG ? MT * C::KS : 1];
+    uint4 qf[C::QREG ? 2 * MT * C::KS : 1];
     if constexpr (C::QREG) {
 #pragma unroll
-        for (int i = 0; i < MT * C::KS; ++i) qf[i] = sq[i * 32 + lane];
+        for (int i = 0; i < 2 * MT * C::KS; ++i) qf[i] = sq[i * 32 + lane];
     }
     float fac[MT];
     int seen[MT];
@@ -202,54 +307,6 @@ __global__ void __launch_bounds__(kThreads, MT == 1 && D <= 128 ? 3 : 2) decode_
         fac[m] = sf[8 * m + g];
         seen[m] = 8 * m + g < rows ? visible(8 * m + g) : 0;
     }
-
-    int8_t const* kb = a.k + b * a.k_b + kvh * a.k_h;
-    int8_t const* vb = a.v + b * a.v_b + kvh * a.v_h;
-    float const* ks = a.ks + b * a.ks_b + kvh * a.ks_h;
-    float const* vs = a.vs + b * a.vs_b + kvh * a.vs_h;
-
-    int const tiles = (most + C::KT - 1) / C::KT;
-    int const t0 = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
-    int const t1 = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
-
-    uint32_t kr[C::NK][C::KW], vr[C::KV][4][C::VW];
-    float ksc[C::KV], vsc[C::KV];
-    auto load_k = [&](int tile) {
-#pragma unroll
-        for (int j = 0; j < C::NK; ++j) {
-            int64_t const key = min(tile * C::KT + 8 * j + g, most - 1);  // masked keys read the last seen one
-            int8_t const* p = kb + key * a.k_t + 16 * t;
-#pragma unroll
-            for (int i = 0; i < C::KW / 4; ++i) {
-                uint4 const w = load16(p + 64 * i);
-                kr[j][4 * i] = w.x, kr[j][4 * i + 1] = w.y, kr[j][4 * i + 2] = w.z, kr[j][4 * i + 3] = w.w;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < C::KV; ++i)
-            ksc[i] = ks[static_cast<int64_t>(min(tile * C::KT + 16 * i, most - 1) >> a.block_shift) * a.ks_j];
-    };
-    auto load_v = [&](int tile) {
-#pragma unroll
-        for (int i = 0; i < C::KV; ++i) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                int64_t const key = min(tile * C::KT + 16 * i + 2 * t + (x & 1) + 8 * (x >> 1), most - 1);
-                if constexpr (D == 64) {
-                    uint2 const w = load8(vb + key * a.v_t + 8 * g);
-                    vr[i][x][0] = w.x, vr[i][x][1] = w.y;
-                } else {
-#pragma unroll
-                    for (int c = 0; c < C::VW / 4; ++c) {
-                        uint4 const w = load16(vb + key * a.v_t + 128 * c + 16 * g);
-                        vr[i][x][4 * c] = w.x, vr[i][x][4 * c + 1] = w.y;
-                        vr[i][x][4 * c + 2] = w.z, vr[i][x][4 * c + 3] = w.w;
-                    }
-                }
-            }
-            vsc[i] = vs[static_cast<int64_t>(min(tile * C::KT + 16 * i, most - 1) >> a.block_shift) * a.vs_j];
-        }
-    };
 
     float m_run[MT], l_run[MT], o[MT][D / 8][2];
 #pragma unroll
@@ -260,38 +317,51 @@ __global__ void __launch_bounds__(kThreads, MT == 1 && D <= 128 ? 3 : 2) decode_
         for (int n = 0; n < D / 8; ++n) o[m][n][0] = o[m][n][1] = 0.0f;
     }
 
-    int tile = t0 + warp;
-    if (tile < t1) {
-        load_k(tile);
-        load_v(tile);
-    }
-    for (; tile < t1; tile += kWarps) {
-        bool const more = tile + kWarps < t1;
+    for (int stage = 0; tile < t1; tile += W, stage ^= 1) {
+        unsigned char const* const tk = ring + stage * 2 * C::TILE;
+        unsigned char const* const tv = tk + C::TILE;
         // scores of 8 MT rows and KT keys
         float s[MT][C::NK][2];
+        copies_landed<3>();
 #pragma unroll
         for (int j = 0; j < C::NK; ++j) {
-            float c[MT][4];
+            uint32_t kr[C::KW];
 #pragma unroll
-            for (int m = 0; m < MT; ++m) c[m][0] = c[m][1] = c[m][2] = c[m][3] = 0.0f;
+            for (int i = 0; i < C::KW / 4; ++i) {
+                uint4 const w = *reinterpret_cast<uint4 const*>(tk + C::place(8 * j + g, C::piece(i, t)));
+                kr[4 * i] = w.x, kr[4 * i + 1] = w.y, kr[4 * i + 2] = w.z, kr[4 * i + 3] = w.w;
+            }
+            int hi[MT][4], lo[MT][4];
 #pragma unroll
             for (int st = 0; st < C::KS; ++st) {
-                uint32_t const w = kr[j][st] ^ 0x80808080u;
-                uint32_t const b0 = halves_of(w, 0x4140), b1 = halves_of(w, 0x4342);
+                uint32_t const b0 = kr[2 * st], b1 = kr[2 * st + 1];
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
-                    uint4 const q = C::QREG ? qf[m * C::KS + st] : sq[(m * C::KS + st) * 32 + lane];
-                    mma16816(c[m], q.x, q.y, q.z, q.w, b0, b1);
+                    int const at = 2 * (m * C::KS + st);
+                    uint4 const qh = C::QREG ? qf[at] : sq[at * 32 + lane];
+                    uint4 const ql = C::QREG ? qf[at + 1] : sq[(at + 1) * 32 + lane];
+                    if (st == 0) {
+                        mma_s8_first(hi[m], qh, b0, b1);
+                        mma_s8_first(lo[m], ql, b0, b1);
+                    } else {
+                        mma_s8(hi[m], qh, b0, b1);
+                        mma_s8(lo[m], ql, b0, b1);
+                    }
                 }
             }
+            // digits of sums below 2^22 each: two of them fit 32 bits
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
                 float const f = fac[m] * ksc[j / 2];
-                s[m][j][0] = (c[m][0] + c[m][2]) * f;
-                s[m][j][1] = (c[m][1] + c[m][3]) * f;
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    s[m][j][e] = fmaf(static_cast<float>(hi[m][e] * 256 + hi[m][e + 2]), 65536.0f,
+                                      static_cast<float>(lo[m][e] * 256 + lo[m][e + 2])) * f;
             }
         }
-        if (more) load_k(tile + kWarps);
+        __syncwarp();  // the warp has read K; its place takes the tile after the next
+        if (tile + 2 * W < t1) fetch(ring_u + stage * 2 * C::TILE, kb, a.k_t, tile + 2 * W);
+        copies_close();
         if ((tile + 1) * C::KT > least) {
 #pragma unroll
             for (int m = 0; m < MT; ++m)
@@ -318,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, MT == 1 && D <= 128 ? 3 : 2) decode_
             float const m_new = fmaxf(m_run[m], top);
             float const base = m_new == neg_inf(0.0f) ? 0.0f : m_new;
             if (__any_sync(0xffffffffu, m_new > m_run[m])) {
-                float const alpha = exp2f(m_run[m] - base);
+                float const alpha = exp2_neg(m_run[m] - base);
                 l_run[m] *= alpha;
 #pragma unroll
                 for (int n = 0; n < D / 8; ++n) o[m][n][0] *= alpha, o[m][n][1] *= alpha;
@@ -329,20 +399,39 @@ __global__ void __launch_bounds__(kThreads, MT == 1 && D <= 128 ? 3 : 2) decode_
                 float const w = vsc[i] * vdown * 8192.0f;  // p * w < 2^14
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    float const p0 = exp2f(s[m][2 * i + h][0] - base), p1 = exp2f(s[m][2 * i + h][1] - base);
+                    float const p0 = exp2_neg(s[m][2 * i + h][0] - base), p1 = exp2_neg(s[m][2 * i + h][1] - base);
                     l_run[m] += p0 + p1;
                     split2(p0 * w, p1 * w, pa[m][i][2 * h], pa[m][i][2 * h + 1]);
                 }
             }
         }
+        if (tile + W < t1) scales(tile + W);
+        copies_landed<3>();
+        uint32_t vr[C::KV][4][C::VW];
+#pragma unroll
+        for (int i = 0; i < C::KV; ++i)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                int const r = 16 * i + 2 * t + (y & 1) + 8 * (y >> 1);
+                if constexpr (D == 64) {
+                    uint2 const w = *reinterpret_cast<uint2 const*>(tv + C::place(r, g >> 1) + 8 * (g & 1));
+                    vr[i][y][0] = w.x, vr[i][y][1] = w.y;
+                } else {
+#pragma unroll
+                    for (int c = 0; c < C::VW / 4; ++c) {
+                        uint4 const w = *reinterpret_cast<uint4 const*>(tv + C::place(r, 8 * c + g));
+                        vr[i][y][4 * c] = w.x, vr[i][y][4 * c + 1] = w.y;
+                        vr[i][y][4 * c + 2] = w.z, vr[i][y][4 * c + 3] = w.w;
+                    }
+                }
+            }
+        __syncwarp();
+        if (tile + 2 * W < t1) fetch(ring_u + (stage * 2 + 1) * C::TILE, vb, a.v_t, tile + 2 * W);
+        copies_close();
         // o += p V, one word of V (four columns of lanes) at a time
 #pragma unroll
         for (int w = 0; w < C::VW; ++w) {
             float c[MT][4][4];
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int n = 0; n < 4; ++n) c[m][n][0] = c[m][n][1] = c[m][n][2] = c[m][n][3] = 0.0f;
 #pragma unroll
             for (int i = 0; i < C::KV; ++i) {
                 uint32_t const v0 = vr[i][0][w] ^ 0x80808080u, v1 = vr[i][1][w] ^ 0x80808080u;
@@ -354,8 +443,12 @@ __global__ void __launch_bounds__(kThreads, MT == 1 && D <= 128 ? 3 : 2) decode_
                     uint32_t const b0 = halves_of(n < 2 ? x01 : y01, n % 2 ? 0x4342 : 0x4140);
                     uint32_t const b1 = halves_of(n < 2 ? x23 : y23, n % 2 ? 0x4342 : 0x4140);
 #pragma unroll
-                    for (int m = 0; m < MT; ++m)
-                        mma16816(c[m][n], pa[m][i][0], pa[m][i][1], pa[m][i][2], pa[m][i][3], b0, b1);
+                    for (int m = 0; m < MT; ++m) {
+                        if (i == 0)
+                            mma_f16_first(c[m][n], pa[m][i], b0, b1);
+                        else
+                            mma_f16(c[m][n], pa[m][i], b0, b1);
+                    }
                 }
             }
 #pragma unroll
@@ -366,10 +459,10 @@ __global__ void __launch_bounds__(kThreads, MT == 1 && D <= 128 ? 3 : 2) decode_
                     o[m][4 * w + n][1] = fmaf(c[m][n][1] + c[m][n][3], back, o[m][4 * w + n][1]);
                 }
         }
-        if (more) load_v(tile + kWarps);
     }
 
-    // Warps to CTA: every warp's rows, maxima and sums in shared memory.
+    // Warps to CTA: every warp's rows in its ring, maxima and sums beside.
+    copies_landed<0>();
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         float l = l_run[m];
@@ -377,11 +470,11 @@ __global__ void __launch_bounds__(kThreads, MT == 1 && D <= 128 ? 3 : 2) decode_
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         if (t == 0) {
             sml[warp * C::ROWS + 8 * m + g] = m_run[m];
-            sml[(kWarps + warp) * C::ROWS + 8 * m + g] = l;
+            sml[(W + warp) * C::ROWS + 8 * m + g] = l;
         }
         // columns 2t and 2t + 1 of n-tile n are elements 32 t + n and 32 t + 16 + n of a
         // 128-element stretch (D = 64: 16 t + n and 16 t + 8 + n)
-        float* row = so + (warp * C::ROWS + 8 * m + g) * D;
+        float* row = reinterpret_cast<float*>(ring) + (8 * m + g) * D;
         constexpr int STRETCH = D == 64 ? 8 : 16;
 #pragma unroll
         for (int n = 0; n < D / 8; n += 4) {
@@ -392,77 +485,93 @@ __global__ void __launch_bounds__(kThreads, MT == 1 && D <= 128 ? 3 : 2) decode_
         }
     }
     __syncthreads();
-    auto weight = [](float m, float top) { return top == neg_inf(0.0f) ? 0.0f : exp2f(m - top); };
-    if (tid < C::ROWS) {
-        float top = neg_inf(0.0f), l = 0.0f;
+    // The CTA's sum of row r, elements 4 (i % (D / 4)) .., and the row's max and sum.
+    auto weight = [](float m, float top) { return top == neg_inf(0.0f) ? 0.0f : exp2_neg(m - top); };
+    auto add4 = [](float4& v, float w, float4 y) {
+        v.x = fmaf(w, y.x, v.x);
+        v.y = fmaf(w, y.y, v.y);
+        v.z = fmaf(w, y.z, v.z);
+        v.w = fmaf(w, y.w, v.w);
+    };
+    auto sum_warps = [&](int i, float& top, float& l) {
+        int const r = i / (D / 4);
+        top = neg_inf(0.0f), l = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sml[w * C::ROWS + tid]);
+        for (int w = 0; w < W; ++w) top = fmaxf(top, sml[w * C::ROWS + r]);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            float const f = weight(sml[w * C::ROWS + tid], top);
-            l += f * sml[(kWarps + w) * C::ROWS + tid];
-            sml[w * C::ROWS + tid] = f;
+        for (int w = 0; w < W; ++w) {
+            float const f = weight(sml[w * C::ROWS + r], top);
+            l = fmaf(f, sml[(W + w) * C::ROWS + r], l);
+            add4(v, f, reinterpret_cast<float4 const*>(smem + C::RING * w)[i]);
         }
-        sx[tid] = top;
-        sx[C::ROWS + tid] = l;
-    }
-    __syncthreads();
-    auto sum_warps = [&](int i) {
-        float v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) v = fmaf(sml[w * C::ROWS + i / D], so[w * C::ROWS * D + i], v);
         return v;
     };
-    auto store = [&](int i, float v) {
-        int const r = i / D, d = i - r * D;
+    auto store = [&](int i, float4 v, float l) {
+        int const r = i / (D / 4), d = 4 * (i - r * (D / 4));
         int64_t const row = row0 + r, hq = kvh * a.g + row % a.g;
-        if (hq < a.Hq) a.out[b * a.o_b + (row / a.g) * a.o_t + hq * a.o_h + d * a.o_d] = v;
+        if (hq >= a.Hq) return;
+        float* p = a.out + b * a.o_b + (row / a.g) * a.o_t + hq * a.o_h + d * a.o_d;
+        bool const none = l == 0.0f;  // no key seen; NaN goes through
+        p[0] = none ? 0.0f : v.x / l;
+        p[a.o_d] = none ? 0.0f : v.y / l;
+        p[2 * a.o_d] = none ? 0.0f : v.z / l;
+        p[3 * a.o_d] = none ? 0.0f : v.w / l;
     };
+    int const items = rows * (D / 4);
     if (a.splits == 1) {
-        for (int i = tid; i < rows * D; i += kThreads) {
-            float const l = sx[C::ROWS + i / D];
-            store(i, l == 0.0f ? 0.0f : sum_warps(i) / l);
+        for (int i = tid; i < items; i += C::THREADS) {
+            float top, l;
+            float4 const v = sum_warps(i, top, l);
+            store(i, v, l);
         }
         return;
     }
-    for (int i = tid; i < rows * D; i += kThreads) so[i] = sum_warps(i);
-
-    // CTAs of the cluster: each gives its share of the rows' elements.
+    // CTAs of the cluster: CTA s sums items [s * per, (s + 1) * per) of all of them.
     cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    if (tid < rows) {
-        float top = neg_inf(0.0f), l = 0.0f;
-        for (int r = 0; r < a.splits; ++r) top = fmaxf(top, cluster.map_shared_rank(sx, r)[tid]);
-        for (int r = 0; r < a.splits; ++r) {
-            float const* px = cluster.map_shared_rank(sx, r);
-            float const f = weight(px[tid], top);
-            l += f * px[C::ROWS + tid];
-            sw[r * C::ROWS + tid] = f;
+    int const per = (items + a.splits - 1) / a.splits;
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA runs
+    float4* recv = reinterpret_cast<float4*>(smem + C::OFF_R);           // [splits][per]
+    for (int i = tid; i < items; i += C::THREADS) {
+        float top, l;
+        float4 const v = sum_warps(i, top, l);
+        int const to = i / per, r = i / (D / 4);
+        cluster.map_shared_rank(recv, to)[split * per + i - to * per] = v;
+        // the row's statistics go with its first element and with every share's first
+        if (i % (D / 4) == 0 || i == to * per) {
+            float* px = cluster.map_shared_rank(sx, to) + split * 2 * C::ROWS + r;
+            px[0] = top;
+            px[C::ROWS] = l;
         }
-        sw[kMaxCluster * C::ROWS + tid] = l;
     }
-    __syncthreads();
-    int const lo = rows * D * split / a.splits, hi = rows * D * (split + 1) / a.splits;
-    for (int i = lo + tid; i < hi; i += kThreads) {
-        float v = 0.0f;
-        for (int r = 0; r < a.splits; ++r) v = fmaf(sw[r * C::ROWS + i / D], cluster.map_shared_rank(so, r)[i], v);
-        float const l = sw[kMaxCluster * C::ROWS + i / D];
-        store(i, l == 0.0f ? 0.0f : v / l);
+    cluster_sync();
+    for (int i = split * per + tid; i < min(items, (split + 1) * per); i += C::THREADS) {
+        int const r = i / (D / 4);
+        float top = neg_inf(0.0f), l = 0.0f;
+        for (int k = 0; k < a.splits; ++k) top = fmaxf(top, sx[k * 2 * C::ROWS + r]);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = 0; k < a.splits; ++k) {
+            float const f = weight(sx[k * 2 * C::ROWS + r], top);
+            l = fmaf(f, sx[k * 2 * C::ROWS + C::ROWS + r], l);
+            add4(v, f, recv[k * per + i - split * per]);
+        }
+        store(i, v, l);
     }
-    cluster.sync();  // peers' shared memory must outlive the reads above
 }
 
 // Splits of the key range = cluster size: enough CTAs for two on every SM, as
 // long as a split keeps two tiles for each of its warps.
 int choose_splits(int64_t units, int64_t cap, int tile) {
-    int64_t const most = std::max<int64_t>(1, ceil_div(cap, int64_t{2} * tile * kWarps));
+    if (const char* e = std::getenv("TUNE_S")) return std::atoi(e);
+    int64_t const most = std::max<int64_t>(1, ceil_div(cap, int64_t{2} * tile * 4));
     int64_t const want = ceil_div(int64_t{2} * sm_count(), units);
     return static_cast<int>(std::min({most, want, int64_t{kMaxCluster}}));
 }
 
-template <int D, int MT>
+template <int D, int MT, int W>
 int launch(ann_stream stream, DecodeQ8Args& a) {
-    using C = Q8<D, MT>;
+    using C = Q8<D, MT, W>;
+    auto const kernel = decode_q8_kernel<D, MT, W>;
     static std::mutex mu;
     static std::set<int> ready;  // devices whose kernel attributes are set
     int dev = 0;
@@ -470,10 +579,9 @@ int launch(ann_stream stream, DecodeQ8Args& a) {
     {
         std::lock_guard<std::mutex> lock(mu);
         if (ready.count(dev) == 0) {
-            cudaError_t e = cudaFuncSetAttribute(decode_q8_kernel<D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 static_cast<int>(C::SMEM));
-            if (e == cudaSuccess)
-                e = cudaFuncSetAttribute(decode_q8_kernel<D, MT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            cudaError_t e =
+                cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(C::SMEM));
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
             if (e != cudaSuccess) return fail(ANN_ECUDA, "attentionDecodeQ8 setup: %s", cudaGetErrorString(e));
             ready.insert(dev);
         }
@@ -490,19 +598,20 @@ int launch(ann_stream stream, DecodeQ8Args& a) {
     attr.val.clusterDim.y = 1;
     attr.val.clusterDim.z = 1;
     cfg.gridDim = dim3(static_cast<unsigned>(grid));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(C::THREADS);
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = as_stream(stream);
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    cudaError_t const e = cudaLaunchKernelEx(&cfg, decode_q8_kernel<D, MT>, a);
+    cudaError_t const e = cudaLaunchKernelEx(&cfg, kernel, a);
     if (e != cudaSuccess) return fail(ANN_ECUDA, "attentionDecodeQ8: %s", cudaGetErrorString(e));
     return check_launch("attentionDecodeQ8");
 }
 
 template <int D>
 int launch_rows(ann_stream stream, DecodeQ8Args& a) {
-    return a.Tq * a.g <= 8 ? launch<D, 1>(stream, a) : launch<D, 2>(stream, a);
+    if (std::getenv("TUNE_W")) return a.Tq * a.g <= 8 ? launch<D, 1, 12>(stream, a) : launch<D, 2, 8>(stream, a);
+    return a.Tq * a.g <= 8 ? launch<D, 1, 4>(stream, a) : launch<D, 2, 4>(stream, a);
 }
 
 int decode_q8(ann_stream stream, const ann_view* q_v, const ann_view* k_v, const ann_view* v_v, const ann_view* ks_v,
