@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <cstdlib>
+#include <map>
 #include <mutex>
 #include <set>
 
@@ -40,7 +41,8 @@ struct DecodeQ8Args {
     int64_t B, Tq, Hq, Hkv, cap;
     uint32_t g;
     int64_t row_tiles;  // CTAs for the Tq * g rows of a KV head
-    int splits;         // of the key range
+    int splits;         // CTAs of a cluster that share a KV head's keys
+    float* parts;       // of the even shares: [2 * gridDim.x][ROWS * D], then [2 * gridDim.x][2][ROWS]
     int block_shift, causal;
     float scale;
 };
@@ -73,6 +75,7 @@ struct DecodeQ8Args {
 // memory, where each CTA sums its share of the output: one cluster barrier, no
 // scratch memory, no atomics, one launch, and a fixed order of sums.
 constexpr int kMaxCluster = 16;
+constexpr int kMaxShares = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D, int MT, int W>
@@ -148,6 +151,34 @@ __device__ __forceinline__ uint32_t halves_of(uint32_t w, uint32_t sel) {
     return *reinterpret_cast<uint32_t const*>(&h);
 }
 
+// Two fp32 values in one 64-bit register: one instruction for both.
+using pair_t = unsigned long long;
+__device__ __forceinline__ pair_t pair(float x, float y) {
+    pair_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    return v;
+}
+__device__ __forceinline__ float2 unpair(pair_t v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+}
+__device__ __forceinline__ pair_t add2(pair_t a, pair_t b) {
+    pair_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ pair_t mul2(pair_t a, pair_t b) {
+    pair_t v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ pair_t fma2(pair_t a, pair_t b, pair_t c) {
+    pair_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+
 // x, y -> their fp16 parts, high and low, each as a pair.
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
     __half2 const h = __floats2half2_rn(x, y);
@@ -172,7 +203,66 @@ __device__ __forceinline__ void copies_landed() {
 // 2^(e - 127) for a biased exponent e in [1, 254].
 __device__ __forceinline__ float pow2_biased(int e) { return __int_as_float(e << 23); }
 
-template <int D, int MT, int W>
+// ---- even shares of all keys ----------------------------------------------------
+// The tiles of every KV head of every sequence in one row, KV heads (and row
+// tiles) of a sequence one after another; CTA c of G takes tiles [cut(c),
+// cut(c + 1)), whole rounds of its W warps. Lengths are known on the device only,
+// so both kernels walk them.
+struct Shares {
+    int total, W, q, rem;  // the first rem CTAs take q + 1 rounds, the others q
+    __device__ Shares(int total, int G, int W) : total(total), W(W) {
+        int const rounds = (total + W - 1) / W;
+        q = rounds / G;
+        rem = rounds - q * G;
+    }
+    __device__ int cut(int c) const { return min(total, W * (c * q + min(c, rem))); }
+    // The CTA whose share tile p < total lies in.
+    __device__ int owner(int p) const {
+        int const r = p / W, wide = rem * (q + 1);
+        return r < wide ? r / (q + 1) : rem + (r - wide) / q;
+    }
+};
+
+// Keys of sequence b.
+__device__ __forceinline__ int64_t keys_of(DecodeQ8Args const& a, int64_t b) {
+    if (a.lengths == nullptr) return a.cap;
+    return min(a.cap, max(int64_t{0}, static_cast<int64_t>(a.lengths[b * a.len_s])));
+}
+
+// Tiles of the first `stop` sequences of one KV head and row tile (each warp by itself).
+template <int KT>
+__device__ __forceinline__ int tiles_before(DecodeQ8Args const& a, int64_t stop) {
+    int sum = 0;
+    for (int64_t b = threadIdx.x & 31; b < stop; b += 32) sum += static_cast<int>((keys_of(a, b) + KT - 1) / KT);
+    return warp_sum(sum);
+}
+// The sequence that holds tile p of one KV head's row, and its first tile.
+template <int KT>
+__device__ __forceinline__ int64_t sequence_of(DecodeQ8Args const& a, int p, int& first) {
+    int const lane = threadIdx.x & 31;
+    int before = 0;
+    for (int64_t b0 = 0;; b0 += 32) {
+        int const n = b0 + lane < a.B ? static_cast<int>((keys_of(a, b0 + lane) + KT - 1) / KT) : 0;
+        int upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            int const y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        unsigned const past = __ballot_sync(0xffffffffu, before + upto > p);
+        if (past != 0 || b0 + 32 >= a.B) {
+            int const at = past != 0 ? __ffs(static_cast<int>(past)) - 1 : 31;
+            first = before + __shfl_sync(0xffffffffu, upto - n, at);
+            return b0 + at;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+}
+
+// SHARES: CTAs take even shares of all keys and leave parts of rows for
+// merge_kernel; else a cluster of a.splits CTAs takes a KV head's keys and merges
+// them itself.
+template <int D, int MT, int W, bool SHARES>
 __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 : 2)) decode_q8_kernel(DecodeQ8Args a) {
     using C = Q8<D, MT, W>;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -181,17 +271,36 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
     float* sf = reinterpret_cast<float*>(smem + C::OFF_F);
     float* sx = reinterpret_cast<float*>(smem + C::OFF_X);
     int const tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    int const split = static_cast<int>(blockIdx.x) % a.splits;
-    if (a.splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // "this CTA runs"
-    int64_t unit = blockIdx.x / a.splits;
-    int64_t const row0 = (unit % a.row_tiles) * C::ROWS;  // first of the KV head's Tq * g query rows
-    unit /= a.row_tiles;
-    int64_t const kvh = unit % a.Hkv, b = unit / a.Hkv;
+    int const split = SHARES ? 0 : static_cast<int>(blockIdx.x) % a.splits;
+    if (!SHARES && a.splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // "this CTA runs"
+
+    int64_t b;            // sequence
+    int unit, units = 0;  // KV head and row tile in it
+    int at = 0, end = 0;  // SHARES: tiles still to do
+    int t0 = 0, t1 = 0;
+    bool first = true;
+    if constexpr (SHARES) {
+        units = static_cast<int>(a.Hkv * a.row_tiles);
+        Shares const sh(tiles_before<C::KT>(a, a.B) * units, gridDim.x, W);
+        at = sh.cut(blockIdx.x), end = sh.cut(blockIdx.x + 1);
+        if (at >= end) return;
+        int before;
+        b = sequence_of<C::KT>(a, at / units, before);
+        // the sequences before fill the first before * units tiles
+        int const n = static_cast<int>((keys_of(a, b) + C::KT - 1) / C::KT), off = at - before * units;
+        unit = off / n;
+        t0 = off - unit * n;
+    } else {
+        int64_t const all = blockIdx.x / a.splits, per = a.Hkv * a.row_tiles;
+        b = all / per;
+        unit = static_cast<int>(all - b * per);
+    }
+  for (;;) {
+    int64_t const kvh = unit / a.row_tiles;
+    int64_t const row0 = (unit - kvh * a.row_tiles) * C::ROWS;  // first of the KV head's Tq * g query rows
     int64_t const left = a.Tq * a.g - row0;
     int const rows = static_cast<int>(min(left, int64_t{C::ROWS}));
-
-    int64_t len = a.cap;
-    if (a.lengths != nullptr) len = min(a.cap, max(int64_t{0}, static_cast<int64_t>(a.lengths[b * a.len_s])));
+    int64_t const len = keys_of(a, b);
 
     // q's rows, loaded while the length is on its way
     constexpr int RPW = (C::ROWS + W - 1) / W, QV = (D + 127) / 128;  // rows of a warp, vectors of a lane
@@ -215,9 +324,14 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
         return static_cast<int>(max(int64_t{0}, n));
     };
     int const most = visible(rows - 1), least = visible(0);
-    int const tiles = (most + C::KT - 1) / C::KT;
-    int const t0 = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
-    int const t1 = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
+    int const tiles = static_cast<int>(((SHARES ? len : most) + C::KT - 1) / C::KT);
+    if constexpr (SHARES) {
+        t1 = min(tiles, t0 + end - at);
+    } else {
+        t0 = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
+        t1 = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
+    }
+    int const t1_seen = min(t1, (most + C::KT - 1) / C::KT);  // a row tile of earlier tokens sees fewer keys
 
     int8_t const* kb = a.k + b * a.k_b + kvh * a.k_h;
     int8_t const* vb = a.v + b * a.v_b + kvh * a.v_h;
@@ -230,7 +344,11 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
     auto fetch = [&](uint32_t dst, int8_t const* base, int64_t stride, int tile) {
         constexpr int LPR = D / 16, RPI = 32 / LPR;  // lanes per row, rows per instruction
         int const r0 = lane / LPR, c = lane % LPR, key = tile * C::KT;
-        if (key + C::KT <= most) {
+        if (key + C::KT <= most && stride == D) {
+            int8_t const* p = base + static_cast<int64_t>(key) * D + 16 * lane;
+#pragma unroll
+            for (int i = 0; i < C::KT / RPI; ++i) copy16(dst + C::place(r0 + i * RPI, c), p + 512 * i);
+        } else if (key + C::KT <= most) {
             int8_t const* p = base + (key + r0) * stride + 16 * c;
 #pragma unroll
             for (int i = 0; i < C::KT / RPI; ++i) copy16(dst + C::place(r0 + i * RPI, c), p + i * RPI * stride);
@@ -253,12 +371,12 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
     // groups: K, V of the first tile, K, V of the second
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-        if (tile + u * W < t1) fetch(ring_u + u * 2 * C::TILE, kb, a.k_t, tile + u * W);
+        if (tile + u * W < t1_seen) fetch(ring_u + u * 2 * C::TILE, kb, a.k_t, tile + u * W);
         copies_close();
-        if (tile + u * W < t1) fetch(ring_u + (u * 2 + 1) * C::TILE, vb, a.v_t, tile + u * W);
+        if (tile + u * W < t1_seen) fetch(ring_u + (u * 2 + 1) * C::TILE, vb, a.v_t, tile + u * W);
         copies_close();
     }
-    if (tile < t1) scales(tile);
+    if (tile < t1_seen) scales(tile);
 
     // q's fragments and the factor of each row's scores.
 #pragma unroll
@@ -308,16 +426,17 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
         seen[m] = 8 * m + g < rows ? visible(8 * m + g) : 0;
     }
 
-    float m_run[MT], l_run[MT], o[MT][D / 8][2];
+    float m_run[MT], l_run[MT];
+    pair_t o[MT][D / 8];  // columns 2t and 2t + 1 of n-tile n
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         m_run[m] = neg_inf(0.0f);
         l_run[m] = 0.0f;
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n) o[m][n][0] = o[m][n][1] = 0.0f;
+        for (int n = 0; n < D / 8; ++n) o[m][n] = pair(0.0f, 0.0f);
     }
 
-    for (int stage = 0; tile < t1; tile += W, stage ^= 1) {
+    for (int stage = 0; tile < t1_seen; tile += W, stage ^= 1) {
         unsigned char const* const tk = ring + stage * 2 * C::TILE;
         unsigned char const* const tv = tk + C::TILE;
         // scores of 8 MT rows and KT keys
@@ -360,7 +479,7 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
             }
         }
         __syncwarp();  // the warp has read K; its place takes the tile after the next
-        if (tile + 2 * W < t1) fetch(ring_u + stage * 2 * C::TILE, kb, a.k_t, tile + 2 * W);
+        if (tile + 2 * W < t1_seen) fetch(ring_u + stage * 2 * C::TILE, kb, a.k_t, tile + 2 * W);
         copies_close();
         if ((tile + 1) * C::KT > least) {
 #pragma unroll
@@ -391,7 +510,7 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
                 float const alpha = exp2_neg(m_run[m] - base);
                 l_run[m] *= alpha;
 #pragma unroll
-                for (int n = 0; n < D / 8; ++n) o[m][n][0] *= alpha, o[m][n][1] *= alpha;
+                for (int n = 0; n < D / 8; ++n) o[m][n] = mul2(o[m][n], pair(alpha, alpha));
                 m_run[m] = m_new;
             }
 #pragma unroll
@@ -401,11 +520,12 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
                 for (int h = 0; h < 2; ++h) {
                     float const p0 = exp2_neg(s[m][2 * i + h][0] - base), p1 = exp2_neg(s[m][2 * i + h][1] - base);
                     l_run[m] += p0 + p1;
-                    split2(p0 * w, p1 * w, pa[m][i][2 * h], pa[m][i][2 * h + 1]);
+                    float2 const pw = unpair(mul2(pair(p0, p1), pair(w, w)));
+                    split2(pw.x, pw.y, pa[m][i][2 * h], pa[m][i][2 * h + 1]);
                 }
             }
         }
-        if (tile + W < t1) scales(tile + W);
+        if (tile + W < t1_seen) scales(tile + W);
         copies_landed<3>();
         uint32_t vr[C::KV][4][C::VW];
 #pragma unroll
@@ -426,7 +546,7 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
                 }
             }
         __syncwarp();
-        if (tile + 2 * W < t1) fetch(ring_u + (stage * 2 + 1) * C::TILE, vb, a.v_t, tile + 2 * W);
+        if (tile + 2 * W < t1_seen) fetch(ring_u + (stage * 2 + 1) * C::TILE, vb, a.v_t, tile + 2 * W);
         copies_close();
         // o += p V, one word of V (four columns of lanes) at a time
 #pragma unroll
@@ -454,10 +574,9 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    o[m][4 * w + n][0] = fmaf(c[m][n][0] + c[m][n][2], back, o[m][4 * w + n][0]);
-                    o[m][4 * w + n][1] = fmaf(c[m][n][1] + c[m][n][3], back, o[m][4 * w + n][1]);
-                }
+                for (int n = 0; n < 4; ++n)
+                    o[m][4 * w + n] = fma2(add2(pair(c[m][n][0], c[m][n][1]), pair(c[m][n][2], c[m][n][3])),
+                                           pair(back, back), o[m][4 * w + n]);
         }
     }
 
@@ -479,9 +598,10 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
 #pragma unroll
         for (int n = 0; n < D / 8; n += 4) {
             float* p = row + (n / STRETCH) * 128 + 2 * STRETCH * t + n % STRETCH;
-            *reinterpret_cast<float4*>(p) = make_float4(o[m][n][0], o[m][n + 1][0], o[m][n + 2][0], o[m][n + 3][0]);
-            *reinterpret_cast<float4*>(p + STRETCH) =
-                make_float4(o[m][n][1], o[m][n + 1][1], o[m][n + 2][1], o[m][n + 3][1]);
+            float2 const v0 = unpair(o[m][n]), v1 = unpair(o[m][n + 1]), v2 = unpair(o[m][n + 2]),
+                         v3 = unpair(o[m][n + 3]);
+            *reinterpret_cast<float4*>(p) = make_float4(v0.x, v1.x, v2.x, v3.x);
+            *reinterpret_cast<float4*>(p + STRETCH) = make_float4(v0.y, v1.y, v2.y, v3.y);
         }
     }
     __syncthreads();
@@ -519,14 +639,41 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
         p[3 * a.o_d] = none ? 0.0f : v.w / l;
     };
     int const items = rows * (D / 4);
-    if (a.splits == 1) {
+    bool const whole = SHARES ? t0 == 0 && t1 == tiles : a.splits == 1;
+    if (whole) {
         for (int i = tid; i < items; i += C::THREADS) {
             float top, l;
             float4 const v = sum_warps(i, top, l);
             store(i, v, l);
         }
-        return;
+    } else if constexpr (SHARES) {
+        // a part of the rows: slot 0 if the share starts with it, else slot 1 (it ends the share)
+        int64_t const slot = 2 * static_cast<int64_t>(blockIdx.x) + (first ? 0 : 1);
+        float4* po = reinterpret_cast<float4*>(a.parts) + slot * (C::ROWS * D / 4);
+        float* ps = a.parts + 2 * static_cast<int64_t>(gridDim.x) * (C::ROWS * D) + slot * (2 * C::ROWS);
+        for (int i = tid; i < items; i += C::THREADS) {
+            float top, l;
+            po[i] = sum_warps(i, top, l);
+            if (i % (D / 4) == 0) {
+                ps[i / (D / 4)] = top;
+                ps[C::ROWS + i / (D / 4)] = l;
+            }
+        }
     }
+    if constexpr (SHARES) {
+        at += t1 - t0;
+        if (at >= end) return;
+        first = false;
+        t0 = 0;
+        if (++unit == units) {
+            unit = 0;
+            do ++b;
+            while (keys_of(a, b) == 0);  // `end` lies past a sequence that has keys
+        }
+        __syncthreads();  // the rings and statistics are read
+        continue;
+    }
+    if (whole) return;
     // CTAs of the cluster: CTA s sums items [s * per, (s + 1) * per) of all of them.
     cg::cluster_group cluster = cg::this_cluster();
     int const per = (items + a.splits - 1) / a.splits;
@@ -557,38 +704,136 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
         }
         store(i, v, l);
     }
+    return;
+  }
 }
 
-// Splits of the key range = cluster size: enough CTAs for two on every SM, as
-// long as a split keeps two tiles for each of its warps.
-int choose_splits(int64_t units, int64_t cap, int tile) {
-    if (const char* e = std::getenv("TUNE_S")) return std::atoi(e);
-    int64_t const most = std::max<int64_t>(1, ceil_div(cap, int64_t{2} * tile * 4));
-    int64_t const want = ceil_div(int64_t{2} * sm_count(), units);
-    return static_cast<int>(std::min({most, want, int64_t{kMaxCluster}}));
+// The parts that the even shares left: a block per query row, KG groups of
+// threads over the parts, then over the groups.
+template <int D, int ROWS, int KT>
+__global__ void __launch_bounds__(256) merge_kernel(DecodeQ8Args a, int G, int W) {
+    constexpr int TPR = D / 4, KG = 256 / TPR;  // threads of a row, groups
+    __shared__ float4 sv[256];
+    __shared__ float wt[kMaxShares];
+    __shared__ float red[8];
+    int const tid = threadIdx.x, item = tid % TPR, grp = tid / TPR;
+    int const units = static_cast<int>(a.Hkv * a.row_tiles), r = blockIdx.y;
+    int64_t const b = blockIdx.x / units;
+    int const u = static_cast<int>(blockIdx.x - b * units);
+    int64_t const kvh = u / a.row_tiles, row = (u - kvh * a.row_tiles) * ROWS + r, hq = kvh * a.g + row % a.g;
+    if (row >= a.Tq * a.g || hq >= a.Hq) return;
+    float* out = a.out + b * a.o_b + (row / a.g) * a.o_t + hq * a.o_h;
+    int const n = static_cast<int>((keys_of(a, b) + KT - 1) / KT);
+    auto write = [&](float4 v) {
+        float* p = out + 4 * item * a.o_d;
+        p[0] = v.x, p[a.o_d] = v.y, p[2 * a.o_d] = v.z, p[3 * a.o_d] = v.w;
+    };
+    Shares const sh(tiles_before<KT>(a, a.B) * units, G, W);
+    int const p0 = tiles_before<KT>(a, b) * units + u * n;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the shares are done and visible
+    if (n == 0) {  // no keys: nobody's share
+        if (grp == 0) write(make_float4(0.f, 0.f, 0.f, 0.f));
+        return;
+    }
+    int const c0 = sh.owner(p0), c1 = sh.owner(p0 + n - 1);
+    if (c0 == c1) return;  // a whole unit: written by its CTA
+    int const parts = c1 - c0 + 1;
+    float const* stats = a.parts + 2 * G * (ROWS * D);
+    // the first CTA may have come from the unit before, the others start with this one
+    auto slot = [&](int k) { return 2 * (c0 + k) + (k == 0 && sh.cut(c0) < p0 ? 1 : 0); };
+    float top = neg_inf(0.0f);
+    for (int k = tid; k < parts; k += 256) top = fmaxf(top, stats[slot(k) * 2 * ROWS + r]);
+    top = block_max<8>(top, red);
+    float l = 0.0f;
+    for (int k = tid; k < parts; k += 256) {
+        float const* ps = stats + slot(k) * 2 * ROWS + r;
+        float const w = top == neg_inf(0.0f) ? 0.0f : exp2_neg(ps[0] - top);
+        l = fmaf(w, ps[ROWS], l);
+        wt[k] = w;
+    }
+    l = block_sum<8>(l, red);  // orders wt too
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 const* po = reinterpret_cast<float4 const*>(a.parts) + r * TPR + item;
+    for (int k = grp; k < parts; k += KG) {
+        float4 const y = po[slot(k) * (ROWS * TPR)];
+        float const w = wt[k];
+        v.x = fmaf(w, y.x, v.x), v.y = fmaf(w, y.y, v.y), v.z = fmaf(w, y.z, v.z), v.w = fmaf(w, y.w, v.w);
+    }
+    sv[tid] = v;
+    __syncthreads();
+    if (grp != 0) return;
+#pragma unroll
+    for (int k = 1; k < KG; ++k) {
+        float4 const y = sv[k * TPR + item];
+        v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
+    }
+    bool const none = l == 0.0f;
+    write(none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v.x / l, v.y / l, v.z / l, v.w / l));
 }
 
-template <int D, int MT, int W>
-int launch(ann_stream stream, DecodeQ8Args& a) {
-    using C = Q8<D, MT, W>;
-    auto const kernel = decode_q8_kernel<D, MT, W>;
+// Scratch for the parts, in stream order, from a pool of the library's own for
+// each device: the default pool would give the memory back to the driver at
+// every synchronisation.
+int scratch_alloc(void** p, size_t bytes, cudaStream_t stream) {
     static std::mutex mu;
-    static std::set<int> ready;  // devices whose kernel attributes are set
+    static std::map<int, cudaMemPool_t> pools;
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return fail(ANN_ECUDA, "attentionDecodeQ8: no CUDA device.");
+    cudaMemPool_t pool = nullptr;
     {
         std::lock_guard<std::mutex> lock(mu);
-        if (ready.count(dev) == 0) {
-            cudaError_t e =
-                cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(C::SMEM));
-            if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-            if (e != cudaSuccess) return fail(ANN_ECUDA, "attentionDecodeQ8 setup: %s", cudaGetErrorString(e));
-            ready.insert(dev);
+        auto const it = pools.find(dev);
+        if (it != pools.end()) {
+            pool = it->second;
+        } else {
+            // the first call of all may be one that is captured: making a pool is no work on its stream
+            cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+            cudaThreadExchangeStreamCaptureMode(&mode);
+            cudaMemPoolProps props{};
+            props.allocType = cudaMemAllocationTypePinned;
+            props.location.type = cudaMemLocationTypeDevice;
+            props.location.id = dev;
+            cudaError_t e = cudaMemPoolCreate(&pool, &props);
+            uint64_t keep = UINT64_MAX;
+            if (e == cudaSuccess) e = cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep);
+            cudaThreadExchangeStreamCaptureMode(&mode);
+            if (e != cudaSuccess) return fail(ANN_ECUDA, "attentionDecodeQ8 scratch: %s", cudaGetErrorString(e));
+            pools[dev] = pool;
         }
     }
-    a.row_tiles = ceil_div(a.Tq * a.g, C::ROWS);
-    int64_t const units = a.B * a.Hkv * a.row_tiles;
-    a.splits = choose_splits(units, a.cap, C::KT);
+    cudaError_t const e = cudaMallocFromPoolAsync(p, bytes, pool, stream);
+    if (e != cudaSuccess) return fail(ANN_ECUDA, "attentionDecodeQ8 scratch: %s", cudaGetErrorString(e));
+    return ANN_OK;
+}
+
+// Kernel attributes, once per device.
+template <typename K>
+int prepare(K kernel, size_t smem, bool wide_cluster, std::set<int>& ready, std::mutex& mu) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return fail(ANN_ECUDA, "attentionDecodeQ8: no CUDA device.");
+    std::lock_guard<std::mutex> lock(mu);
+    if (ready.count(dev) != 0) return ANN_OK;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e == cudaSuccess && wide_cluster)
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return fail(ANN_ECUDA, "attentionDecodeQ8 setup: %s", cudaGetErrorString(e));
+    ready.insert(dev);
+    return ANN_OK;
+}
+
+// One launch, a cluster of CTAs per KV head: for calls of little work.
+template <int D, int MT>
+int launch_cluster(ann_stream stream, DecodeQ8Args& a, int64_t units) {
+    constexpr int W = 4;
+    using C = Q8<D, MT, W>;
+    auto const kernel = decode_q8_kernel<D, MT, W, false>;
+    static std::mutex mu;
+    static std::set<int> ready;
+    ANN_TRY(prepare(kernel, C::SMEM, true, ready, mu));
+    // two CTAs for every SM, as long as a split keeps two tiles for each of its warps
+    int64_t const most = std::max<int64_t>(1, ceil_div(a.cap, int64_t{2} * C::KT * W));
+    int64_t const want = ceil_div(int64_t{2} * sm_count(), units);
+    a.splits = static_cast<int>(std::min({most, want, int64_t{kMaxCluster}}));
     int64_t const grid = units * a.splits;
     if (grid > INT32_MAX) return fail(ANN_ENOTSUP, "attentionDecodeQ8: grid too large.");
     cudaLaunchConfig_t cfg{};
@@ -608,10 +853,58 @@ int launch(ann_stream stream, DecodeQ8Args& a) {
     return check_launch("attentionDecodeQ8");
 }
 
+// Even shares of all keys for as many CTAs as fit the GPU, then the merge of the
+// rows that several CTAs share.
+template <int D, int MT>
+int launch_shares(ann_stream stream, DecodeQ8Args& a, int64_t units, int per_sm) {
+    constexpr int W = 4;
+    using C = Q8<D, MT, W>;
+    auto const kernel = decode_q8_kernel<D, MT, W, true>;
+    static std::mutex mu;
+    static std::set<int> ready;
+    ANN_TRY(prepare(kernel, C::SMEM, false, ready, mu));
+    int64_t const G = std::min<int64_t>(kMaxShares, int64_t{sm_count()} * per_sm);
+    void* parts = nullptr;
+    ANN_TRY(scratch_alloc(&parts, sizeof(float) * 2 * G * (C::ROWS * D + 2 * C::ROWS), as_stream(stream)));
+    a.parts = static_cast<float*>(parts);
+    kernel<<<static_cast<unsigned>(G), C::THREADS, C::SMEM, as_stream(stream)>>>(a);
+    int rc = check_launch("attentionDecodeQ8");
+    if (rc == ANN_OK) {
+        cudaLaunchConfig_t cfg{};
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its launch overlaps the shares' end
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        unsigned const rows = static_cast<unsigned>(std::min<int64_t>(C::ROWS, a.Tq * a.g));
+        cfg.gridDim = dim3(static_cast<unsigned>(units), rows);
+        cfg.blockDim = dim3(256);
+        cfg.stream = as_stream(stream);
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        cudaError_t const e = cudaLaunchKernelEx(&cfg, merge_kernel<D, C::ROWS, C::KT>, a, static_cast<int>(G), W);
+        rc = e != cudaSuccess ? fail(ANN_ECUDA, "attentionDecodeQ8: %s", cudaGetErrorString(e))
+                              : check_launch("attentionDecodeQ8");
+    }
+    cudaFreeAsync(parts, as_stream(stream));
+    return rc;
+}
+
+template <int D, int MT>
+int launch(ann_stream stream, DecodeQ8Args& a) {
+    using C = Q8<D, MT, 4>;
+    a.row_tiles = ceil_div(a.Tq * a.g, C::ROWS);
+    int64_t const units = a.B * a.Hkv * a.row_tiles;
+    if (units * C::ROWS > INT32_MAX) return fail(ANN_ENOTSUP, "attentionDecodeQ8: grid too large.");
+    int const per_sm = MT == 1 && D <= 128 ? 3 : 2;
+    // every share's parts are indexed in 32 bits
+    bool const large = units * ceil_div(a.cap, C::KT) > INT32_MAX / 2;
+    bool const small = large || units * ceil_div(a.cap, C::KT) <= int64_t{2} * 4 * per_sm * sm_count();
+    if (std::getenv("TUNE_P") ? std::atoi(std::getenv("TUNE_P")) : small) return launch_cluster<D, MT>(stream, a, units);
+    return launch_shares<D, MT>(stream, a, units, per_sm);
+}
+
 template <int D>
 int launch_rows(ann_stream stream, DecodeQ8Args& a) {
-    if (std::getenv("TUNE_W")) return a.Tq * a.g <= 8 ? launch<D, 1, 12>(stream, a) : launch<D, 2, 8>(stream, a);
-    return a.Tq * a.g <= 8 ? launch<D, 1, 4>(stream, a) : launch<D, 2, 4>(stream, a);
+    return a.Tq * a.g <= 8 ? launch<D, 1>(stream, a) : launch<D, 2>(stream, a);
 }
 
 int decode_q8(ann_stream stream, const ann_view* q_v, const ann_view* k_v, const ann_view* v_v, const ann_view* ks_v,
