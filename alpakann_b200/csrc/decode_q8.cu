@@ -296,10 +296,9 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
         unit = static_cast<int>(all - b * per);
     }
   for (;;) {
-    int64_t const kvh = unit / a.row_tiles;
-    int64_t const row0 = (unit - kvh * a.row_tiles) * C::ROWS;  // first of the KV head's Tq * g query rows
-    int64_t const left = a.Tq * a.g - row0;
-    int const rows = static_cast<int>(min(left, int64_t{C::ROWS}));
+    int const kvh = unit / static_cast<int>(a.row_tiles);
+    uint32_t const row0 = (unit - kvh * static_cast<int>(a.row_tiles)) * C::ROWS;  // first of the KV head's Tq * g query rows
+    int const rows = static_cast<int>(min(static_cast<uint32_t>(a.Tq) * a.g - row0, uint32_t{C::ROWS}));
     int64_t const len = keys_of(a, b);
 
     // q's rows, loaded while the length is on its way
@@ -308,7 +307,8 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
 #pragma unroll
     for (int u = 0; u < RPW; ++u) {
         int const r = warp + u * W;
-        int64_t const row = row0 + r, hq = kvh * a.g + row % a.g;
+        uint32_t const row = row0 + r;
+        int64_t const hq = static_cast<int64_t>(kvh) * a.g + row % a.g;
         bool const given = r < rows && hq < a.Hq;
         float const* q = a.q + b * a.q_b + (row / a.g) * a.q_t + hq * a.q_h;
 #pragma unroll
@@ -629,7 +629,8 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
     };
     auto store = [&](int i, float4 v, float l) {
         int const r = i / (D / 4), d = 4 * (i - r * (D / 4));
-        int64_t const row = row0 + r, hq = kvh * a.g + row % a.g;
+        uint32_t const row = row0 + r;
+        int64_t const hq = static_cast<int64_t>(kvh) * a.g + row % a.g;
         if (hq >= a.Hq) return;
         float* p = a.out + b * a.o_b + (row / a.g) * a.o_t + hq * a.o_h + d * a.o_d;
         bool const none = l == 0.0f;  // no key seen; NaN goes through
@@ -708,67 +709,82 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
   }
 }
 
-// The parts that the even shares left: a block per query row, KG groups of
-// threads over the parts, then over the groups.
+// The parts that the even shares left. A block takes `per_block` (1 or 8) rows of
+// a KV head's row tile; the 8 / per_block warps of a row share its parts.
 template <int D, int ROWS, int KT>
-__global__ void __launch_bounds__(256) merge_kernel(DecodeQ8Args a, int G, int W) {
-    constexpr int TPR = D / 4, KG = 256 / TPR;  // threads of a row, groups
-    __shared__ float4 sv[256];
-    __shared__ float wt[kMaxShares];
-    __shared__ float red[8];
-    int const tid = threadIdx.x, item = tid % TPR, grp = tid / TPR;
-    int const units = static_cast<int>(a.Hkv * a.row_tiles), r = blockIdx.y;
+__global__ void __launch_bounds__(256) merge_kernel(DecodeQ8Args a, int G, int W, int per_block) {
+    constexpr int LV = (D + 127) / 128;  // float4 of a row per lane
+    __shared__ float4 sv[8][LV * 32];
+    int const lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int const units = static_cast<int>(a.Hkv * a.row_tiles), wpr = 8 / per_block;
+    int const r = blockIdx.y * per_block + warp / wpr, sub = warp % wpr;
     int64_t const b = blockIdx.x / units;
     int const u = static_cast<int>(blockIdx.x - b * units);
-    int64_t const kvh = u / a.row_tiles, row = (u - kvh * a.row_tiles) * ROWS + r, hq = kvh * a.g + row % a.g;
-    if (row >= a.Tq * a.g || hq >= a.Hq) return;
-    float* out = a.out + b * a.o_b + (row / a.g) * a.o_t + hq * a.o_h;
     int const n = static_cast<int>((keys_of(a, b) + KT - 1) / KT);
-    auto write = [&](float4 v) {
-        float* p = out + 4 * item * a.o_d;
-        p[0] = v.x, p[a.o_d] = v.y, p[2 * a.o_d] = v.z, p[3 * a.o_d] = v.w;
-    };
     Shares const sh(tiles_before<KT>(a, a.B) * units, G, W);
     int const p0 = tiles_before<KT>(a, b) * units + u * n;
+    int const c0 = n > 0 ? sh.owner(p0) : 0, c1 = n > 0 ? sh.owner(p0 + n - 1) : 0;
+    if (n > 0 && c0 == c1) return;  // a whole unit: written by its CTA
+    int const rt = static_cast<int>(a.row_tiles), kvh = u / rt;
+    uint32_t const row = static_cast<uint32_t>((u - kvh * rt) * ROWS + r);
+    int64_t const hq = static_cast<int64_t>(kvh) * a.g + row % a.g;
+    bool const given = row < a.Tq * a.g && hq < a.Hq;
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the shares are done and visible
-    if (n == 0) {  // no keys: nobody's share
-        if (grp == 0) write(make_float4(0.f, 0.f, 0.f, 0.f));
-        return;
-    }
-    int const c0 = sh.owner(p0), c1 = sh.owner(p0 + n - 1);
-    if (c0 == c1) return;  // a whole unit: written by its CTA
-    int const parts = c1 - c0 + 1;
+    int const parts = n > 0 ? c1 - c0 + 1 : 0;          // no keys: nobody's share, a row of zeros
     float const* stats = a.parts + 2 * G * (ROWS * D);
     // the first CTA may have come from the unit before, the others start with this one
-    auto slot = [&](int k) { return 2 * (c0 + k) + (k == 0 && sh.cut(c0) < p0 ? 1 : 0); };
-    float top = neg_inf(0.0f);
-    for (int k = tid; k < parts; k += 256) top = fmaxf(top, stats[slot(k) * 2 * ROWS + r]);
-    top = block_max<8>(top, red);
-    float l = 0.0f;
-    for (int k = tid; k < parts; k += 256) {
-        float const* ps = stats + slot(k) * 2 * ROWS + r;
-        float const w = top == neg_inf(0.0f) ? 0.0f : exp2_neg(ps[0] - top);
-        l = fmaf(w, ps[ROWS], l);
-        wt[k] = w;
-    }
-    l = block_sum<8>(l, red);  // orders wt too
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    float4 const* po = reinterpret_cast<float4 const*>(a.parts) + r * TPR + item;
-    for (int k = grp; k < parts; k += KG) {
-        float4 const y = po[slot(k) * (ROWS * TPR)];
-        float const w = wt[k];
-        v.x = fmaf(w, y.x, v.x), v.y = fmaf(w, y.y, v.y), v.z = fmaf(w, y.z, v.z), v.w = fmaf(w, y.w, v.w);
-    }
-    sv[tid] = v;
-    __syncthreads();
-    if (grp != 0) return;
+    auto slot = [&](int k) { return static_cast<int64_t>(2 * (c0 + k) + (k == 0 && sh.cut(c0) < p0 ? 1 : 0)); };
+    float top = neg_inf(0.0f), l = 0.0f;
+    float4 v[LV];
 #pragma unroll
-    for (int k = 1; k < KG; ++k) {
-        float4 const y = sv[k * TPR + item];
-        v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
+    for (int i = 0; i < LV; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (given) {
+        for (int k = lane; k < parts; k += 32) top = fmaxf(top, stats[slot(k) * 2 * ROWS + r]);
+        top = warp_max(top);
+        auto weight = [&](float m) { return top == neg_inf(0.0f) ? 0.0f : exp2_neg(m - top); };
+        for (int k = lane; k < parts; k += 32) {
+            float const* ps = stats + slot(k) * 2 * ROWS + r;
+            l = fmaf(weight(ps[0]), ps[ROWS], l);
+        }
+        l = warp_sum(l);
+#pragma unroll 4
+        for (int k = sub; k < parts; k += wpr) {
+            int64_t const sl = slot(k);
+            float const w = weight(stats[sl * 2 * ROWS + r]);
+            float4 const* po = reinterpret_cast<float4 const*>(a.parts) + (sl * ROWS + r) * (D / 4);
+#pragma unroll
+            for (int i = 0; i < LV; ++i) {
+                if (32 * i + lane >= D / 4) continue;
+                float4 const y = po[32 * i + lane];
+                v[i].x = fmaf(w, y.x, v[i].x), v[i].y = fmaf(w, y.y, v[i].y);
+                v[i].z = fmaf(w, y.z, v[i].z), v[i].w = fmaf(w, y.w, v[i].w);
+            }
+        }
     }
+    if (wpr > 1) {
+#pragma unroll
+        for (int i = 0; i < LV; ++i) sv[warp][32 * i + lane] = v[i];
+        __syncthreads();
+        if (sub != 0) return;
+        for (int k = 1; k < wpr; ++k)
+#pragma unroll
+            for (int i = 0; i < LV; ++i) {
+                float4 const y = sv[warp + k][32 * i + lane];
+                v[i].x += y.x, v[i].y += y.y, v[i].z += y.z, v[i].w += y.w;
+            }
+    }
+    if (!given) return;
+    float* out = a.out + b * a.o_b + (row / a.g) * a.o_t + hq * a.o_h;
     bool const none = l == 0.0f;
-    write(none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v.x / l, v.y / l, v.z / l, v.w / l));
+#pragma unroll
+    for (int i = 0; i < LV; ++i) {
+        if (32 * i + lane >= D / 4) continue;
+        float* p = out + 4 * (32 * i + lane) * a.o_d;
+        p[0] = none ? 0.0f : v[i].x / l;
+        p[a.o_d] = none ? 0.0f : v[i].y / l;
+        p[2 * a.o_d] = none ? 0.0f : v[i].z / l;
+        p[3 * a.o_d] = none ? 0.0f : v[i].w / l;
+    }
 }
 
 // Scratch for the parts, in stream order, from a pool of the library's own for
@@ -874,13 +890,15 @@ int launch_shares(ann_stream stream, DecodeQ8Args& a, int64_t units, int per_sm)
         cudaLaunchAttribute attr{};
         attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its launch overlaps the shares' end
         attr.val.programmaticStreamSerializationAllowed = 1;
-        unsigned const rows = static_cast<unsigned>(std::min<int64_t>(C::ROWS, a.Tq * a.g));
-        cfg.gridDim = dim3(static_cast<unsigned>(units), rows);
+        // few units: many parts each, so all warps of a block to one row
+        int const rows = static_cast<int>(std::min<int64_t>(C::ROWS, a.Tq * a.g)), per_block = units < G / 8 ? 1 : 8;
+        cfg.gridDim = dim3(static_cast<unsigned>(units), static_cast<unsigned>(ceil_div(rows, per_block)));
         cfg.blockDim = dim3(256);
         cfg.stream = as_stream(stream);
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
-        cudaError_t const e = cudaLaunchKernelEx(&cfg, merge_kernel<D, C::ROWS, C::KT>, a, static_cast<int>(G), W);
+        cudaError_t const e = cudaLaunchKernelEx(&cfg, merge_kernel<D, C::ROWS, C::KT>, a, static_cast<int>(G), W,
+                                                 per_block);
         rc = e != cudaSuccess ? fail(ANN_ECUDA, "attentionDecodeQ8: %s", cudaGetErrorString(e))
                               : check_launch("attentionDecodeQ8");
     }
@@ -891,6 +909,7 @@ int launch_shares(ann_stream stream, DecodeQ8Args& a, int64_t units, int per_sm)
 template <int D, int MT>
 int launch(ann_stream stream, DecodeQ8Args& a) {
     using C = Q8<D, MT, 4>;
+    if (a.Tq > INT32_MAX / 2 / static_cast<int64_t>(a.g)) return fail(ANN_ENOTSUP, "attentionDecodeQ8: more than 2^30 rows.");
     a.row_tiles = ceil_div(a.Tq * a.g, C::ROWS);
     int64_t const units = a.B * a.Hkv * a.row_tiles;
     if (units * C::ROWS > INT32_MAX) return fail(ANN_ENOTSUP, "attentionDecodeQ8: grid too large.");
