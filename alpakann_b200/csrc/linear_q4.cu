@@ -7,9 +7,9 @@
 //   packed [K / 8, N] int32, scales [ceil(K / group), N].
 //   y[m, n] = act(sum_k x[m, k] W[k, n] + bias[n]) + residual[m, n]
 #include <cooperative_groups.h>
-#include <cuda_fp16.h>
 
 #include <algorithm>
+#include <climits>
 #include <cstdlib>
 #include <mutex>
 #include <set>
@@ -45,90 +45,132 @@ __device__ __forceinline__ float activate(float v, int act) {
     }
 }
 
-// The product on mma.sync.m16n8k16, transposed: 16 columns of W by 8 slots, the
-// slots being the two fp16 parts (11 bits each) of up to four rows of x, so that
-// one product gives both parts of four rows in the same thread and the weights
-// -- whole numbers -8..7, exact in fp16 -- are converted once for all rows. Sums
-// are fp32; every 32 inputs they leave the tensor core and meet their group's
+// The product in whole numbers. A nibble u is an 8-bit operand as it is: two
+// masks unpack the eight of a word. A row of x is rounded to 31 bits of its
+// largest value (over a warp's inputs) and cut into four 8-bit digits, and
+// mma.sync.m16n8k32 on int8 multiplies, transposed: 16 columns of W by 8 slots,
+// the slots being the digits of two rows. The sums are exact in int32, the offset
+// of 8 included: a product with ones gives the digits' sums, of which eight times
+// are taken off. They become fp32 when their group of inputs ends and meet its
 // scale. The order of the summed index is free, so a lane takes the words as a
-// 16-byte load gives them: eight inputs (its octet of 32) of four neighbouring
-// columns, whose nibbles j and j + 4 sit 16 bits apart and become a fp16 pair with
-// one mask and one addition; x is laid out to match.
+// 16-byte load gives them, eight inputs (its octet of 32) of four neighbouring
+// columns; x's digits are laid out to match.
 //
-// A CTA takes 32 CT columns, its warps (and the CTAs of a cluster) the inputs;
-// partial sums meet in shared memory and, across the cluster, in the CTA that
-// owns a share of the columns, which applies bias, activation and residual. One
-// launch, no scratch memory, no atomics, a fixed order of sums.
+// A CTA stays and takes one tile of 32 CT columns after another. Each of its warps
+// (and each CTA of a cluster, where columns are few) has inputs of its own, whose
+// digits it prepares once; it streams their weights through a ring
+// in shared memory (cp.async, each lane its own 16 bytes, on across tiles), 4 KB
+// in flight a warp. The warps' sums of a tile meet in shared memory, across a
+// cluster in the CTA that owns a share of the columns, which applies bias,
+// activation and residual. One launch, no scratch memory, no atomics, a fixed
+// order of sums.
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxCluster = 16;
-constexpr uint32_t kZeros = 0x88888888u;  // eight weights of 0
+// Bytes of x's digits in a CTA: at most 61 steps a warp, 1952 inputs of |u d| <=
+// 1920, so that 256 times their sum fits 32 bits.
+constexpr int kMaxDigits = 120 << 10;
 
-// d += a b (or d = a b), fp16 products summed in fp32.
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// Shared memory: rings [kWarps][DEPTH][CT][2][32] uint4 (words, scales), two
+// buffers of sums [kWarps][ROWS][COLS] and of the cluster's [per * splits], digits
+// uint2 [steps of the CTA][NT][32].
+template <int CT, int NT>
+struct Q4 {
+    static constexpr int COLS = 32 * CT, ROWS = 2 * NT, ITEMS = ROWS * COLS;
+    static constexpr int DEPTH = 8 / CT;  // steps of 32 inputs in flight a warp
+    static constexpr size_t RING = size_t{16} * DEPTH * CT * 2 * 32;  // of a warp
+    static constexpr size_t OFF_S = RING * kWarps;
+    static constexpr size_t OFF_R = OFF_S + sizeof(float) * 2 * kWarps * ITEMS;
+    static constexpr size_t OFF_D = OFF_R + sizeof(float) * 2 * (ITEMS + kMaxCluster);
+    static constexpr size_t digits(int64_t steps) { return static_cast<size_t>(steps) * NT * 32 * sizeof(uint2); }
+};
+
+// c += a b, int8 products of depth 32, exact in int32.
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y));
 }
-__device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                              uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 
-__device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t const*>(&h); }
-__device__ __forceinline__ __half2 half2_of(uint32_t w) { return *reinterpret_cast<__half2 const*>(&w); }
-
-// A word's weights as fp16 pairs (j, j + 4), j = 0..3. 0x6400 | u is 1024 + u, and
-// 1032 is taken off; with the nibble 4 bits higher it is 1024 + 16 u, of which a
-// sixteenth less 72 is left. All exact.
-__device__ __forceinline__ void weights_of(uint32_t w, uint32_t (&h)[4]) {
-    __half2 const off = half2_of(0x64086408u), sixteenth = half2_of(0x2c002c00u), off16 = half2_of(0xd480d480u);
-    uint32_t const v = w >> 8;
-    h[0] = bits(__hsub2(half2_of((w & 0x000f000fu) | 0x64006400u), off));
-    h[1] = bits(__hfma2(half2_of((w & 0x00f000f0u) | 0x64006400u), sixteenth, off16));
-    h[2] = bits(__hsub2(half2_of((v & 0x000f000fu) | 0x64006400u), off));
-    h[3] = bits(__hfma2(half2_of((v & 0x00f000f0u) | 0x64006400u), sixteenth, off16));
-}
-
-// CT: 16-byte words of columns per lane (32 CT columns a CTA); NT: slots / 8 (4 NT
+// CT: 16-byte words of columns per lane (32 CT columns a tile); NT: slots / 8 (2 NT
 // rows a CTA); VEC: words and scales of four columns are one aligned load.
 template <int CT, int NT, bool VEC>
-__global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) linear_q4_kernel(LinearQ4Args a) {
-    constexpr int COLS = 32 * CT, ROWS = 4 * NT, ITEMS = ROWS * COLS;
-    extern __shared__ __align__(16) float sums[];  // [kWarps][ROWS][COLS], then [splits][per]
+__global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kernel(LinearQ4Args a) {
+    using C = Q4<CT, NT>;
+    extern __shared__ __align__(16) unsigned char smem[];
     int const tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     int const split = static_cast<int>(blockIdx.x) % a.splits;
     if (a.splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // "this CTA runs"
-    int64_t const col0 = static_cast<int64_t>(blockIdx.x / a.splits) * COLS, row0 = static_cast<int64_t>(blockIdx.y) * ROWS;
+    int64_t const row0 = static_cast<int64_t>(blockIdx.y) * C::ROWS;
     // this warp's steps of 32 inputs
     int const steps = static_cast<int>((a.K + 31) / 32), parts = a.splits * kWarps, part = split * kWarps + warp;
+    int const first = static_cast<int>(static_cast<int64_t>(steps) * (split * kWarps) / parts);  // the CTA's first
     int const s0 = static_cast<int>(static_cast<int64_t>(steps) * part / parts);
     int const s1 = static_cast<int>(static_cast<int64_t>(steps) * (part + 1) / parts);
-    int const octets = static_cast<int>(a.K / 8);
+    int const octets = static_cast<int>(a.K / 8), per_group = a.group / 32;
+    int const tiles = static_cast<int>((a.N + C::COLS - 1) / C::COLS);
+    int const tile0 = static_cast<int>(blockIdx.x) / a.splits, stride = static_cast<int>(gridDim.x) / a.splits;
 
-    auto load_w = [&](int step, uint32_t (&w)[CT][4]) {
-        int const r = 4 * step + t;
-        uint32_t const* p = a.w + r * a.w_r;
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-            int64_t const n = col0 + 32 * c + 4 * g;
-            if constexpr (VEC) {
-                uint4 v = make_uint4(kZeros, kZeros, kZeros, kZeros);
-                if (r < octets && n < a.N) v = __ldg(reinterpret_cast<uint4 const*>(p + n));
-                w[c][0] = v.x, w[c][1] = v.y, w[c][2] = v.z, w[c][3] = v.w;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[c][e] = r < octets && n + e < a.N ? __ldg(p + (n + e) * a.w_n) : kZeros;
-            }
-        }
+    uint4* const ring = reinterpret_cast<uint4*>(smem + C::RING * warp);
+    uint32_t const ring_u = smem_u32(ring) + 16 * lane;
+    uint2* const dig = reinterpret_cast<uint2*>(smem + C::OFF_D) + static_cast<size_t>(s0 - first) * NT * 32;
+    // Steps are fetched in the order of their use, tile after tile. Sums meet their
+    // scale after the last step of a group and after the last of the range.
+    int const left0 = per_group - s0 % per_group;  // steps of the first group
+    int64_t const w_step = 4 * a.w_r;
+    uint32_t const* const w0 = a.w + (4 * static_cast<int64_t>(s0) + t) * a.w_r + 4 * g * a.w_n;
+    float const* const sc0 = a.s + s0 / per_group * a.s_g + 4 * g * a.s_n;
+    uint32_t const* f_w = w0;
+    float const* f_s = sc0;
+    int f_tile = tile0, f_step = s0, f_left = left0, f_slot = 0, f_cols = 0;  // f_cols: columns from this lane's first on
+    auto open_tile = [&]() {
+        int64_t const col = static_cast<int64_t>(f_tile) * C::COLS;
+        f_w = w0 + col * a.w_n;
+        f_s = sc0 + col * a.s_n;
+        f_cols = f_tile < tiles && s0 < s1 ? static_cast<int>(min(a.N - col, int64_t{C::COLS})) - 4 * g : INT_MIN;
+        f_step = s0, f_left = left0;
     };
-    // x of slot row g / 2 (+ 4 nt): this lane's octet of a step
-    auto load_x = [&](int step, int nt, float (&x)[8]) {
-        int64_t const m = row0 + 4 * nt + (g >> 1), k = 32 * static_cast<int64_t>(step) + 8 * t;
-        bool const in = m < a.M && k < a.K;
+    auto fetch = [&]() {
+        if (f_cols != INT_MIN) {
+            uint32_t const dst = ring_u + static_cast<uint32_t>(f_slot) * (CT * 2 * 512);
+            bool const in = 4 * f_step + t < octets, last = f_left == 1 || f_step + 1 == s1;
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                if constexpr (VEC) {
+                    if (in && 32 * c < f_cols) copy16(dst + c * 1024, f_w + 32 * c);
+                    if (last && 32 * c < f_cols) copy16(dst + c * 1024 + 512, f_s + 32 * c);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (in && 32 * c + e < f_cols) copy4(dst + c * 1024 + 4 * e, f_w + (32 * c + e) * a.w_n);
+                        if (last && 32 * c + e < f_cols) copy4(dst + c * 1024 + 512 + 4 * e, f_s + (32 * c + e) * a.s_n);
+                    }
+                }
+            }
+            f_w += w_step;
+            if (--f_left == 0) f_left = per_group, f_s += a.s_g;
+            if (++f_step == s1) f_tile += stride, open_tile();
+        }
+        if (++f_slot == C::DEPTH) f_slot = 0;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    open_tile();
+#pragma unroll
+    for (int i = 0; i < C::DEPTH; ++i) fetch();
+
+    // x's digits: a lane takes an octet of a row at a time. First the rows' largest
+    // values, then the digits. Lanes t and t + 1 of a row's four slots hold its high
+    // and low digits, so a lane keeps the factor of row t / 2 of its two.
+    float down[NT];
+    auto load_x = [&](int r, int base, float (&x)[8]) {
+        int64_t const m = row0 + r, k = 32 * static_cast<int64_t>(base) + 8 * lane;
+        bool const in = m < a.M && k < a.K && base + lane / 4 < s1;
         float const* p = a.x + m * a.x_m + k * a.x_k;
         if (a.x_vec) {
             float4 const zero = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -140,141 +182,171 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) linear_q4_kernel(Li
             for (int e = 0; e < 8; ++e) x[e] = in ? p[e * a.x_k] : 0.0f;
         }
     };
-
-    uint32_t w[2][CT][4];
-    if (s0 < s1) load_w(s0, w[0]);
-    // The power of two that brings this warp's largest |x| of each row to [2^13, 2^14).
-    float up[NT], down[NT];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        unsigned int top = 0;
-        for (int s = s0; s < s1; ++s) {
+    for (int r = 0; r < C::ROWS; ++r) {
+        unsigned int top = 0;  // max |x| on the bit patterns: NaN above infinity above every number
+        for (int base = s0; base < s1; base += 8) {
             float x[8];
-            load_x(s, nt, x);
+            load_x(r, base, x);
 #pragma unroll
             for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
         }
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        int e = static_cast<int>(top >> 23);
-        e = e == 255 ? 140 : max(e, 15);  // NaN and infinity pass through as they are
-        up[nt] = __int_as_float((267 - e) << 23);
-        // slot 2t holds row t: its lane's factor
-        down[nt] = __shfl_sync(0xffffffffu, __int_as_float((e - 13) << 23), 8 * t);
+        top = __reduce_max_sync(0xffffffffu, top);
+        // the largest value into [2^29, 2^30): 2^(156 - e), e its biased exponent, where both factors are normal
+        int const e = min(max(static_cast<int>(top >> 23), 31), 254);
+        float const up = __int_as_float((283 - e) << 23);
+        // NaN and infinity have no whole numbers: the row's sums become NaN
+        float const back = top >= 0x7f800000u ? __int_as_float(0x7fffffff) : __int_as_float((e - 29) << 23);
+        if ((t >> 1) == (r & 1)) down[r / 2] = back;
+        for (int base = s0; base < s1; base += 8) {
+            float x[8];
+            load_x(r, base, x);
+            if (base + lane / 4 >= s1) continue;
+            uint32_t n[8];  // signed base-256 digits: a carry out of the lower bytes, then their signs
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                n[i] = (static_cast<uint32_t>(__float2int_rn(x[i] * up)) + 0x00808080u) ^ 0x00808080u;
+            // bytes of elements 0, 2, 4, 6 and 1, 3, 5, 7 (the two masks of a word), digit by digit
+            uint32_t d[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t const lo01 = __byte_perm(n[h], n[2 + h], 0x5140), hi01 = __byte_perm(n[h], n[2 + h], 0x7362);
+                uint32_t const lo23 = __byte_perm(n[4 + h], n[6 + h], 0x5140), hi23 = __byte_perm(n[4 + h], n[6 + h], 0x7362);
+                d[h][0] = __byte_perm(hi01, hi23, 0x7632);
+                d[h][1] = __byte_perm(hi01, hi23, 0x5410);
+                d[h][2] = __byte_perm(lo01, lo23, 0x7632);
+                d[h][3] = __byte_perm(lo01, lo23, 0x5410);
+            }
+            uint2* const to = dig + ((base - s0 + (lane >> 2)) * NT + r / 2) * 32 + (r & 1) * 16 + t;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) to[4 * j] = make_uint2(d[0][j], d[1][j]);
+        }
     }
+    __syncwarp();
 
-    float acc[NT][CT][4];
+    int const rows = static_cast<int>(min(static_cast<int64_t>(C::ROWS), a.M - row0));
+    int const items = rows * C::COLS, per = (items + a.splits - 1) / a.splits;
+    int slot = 0;
+    for (int tile = tile0, round = 0; tile < tiles; tile += stride, round ^= 1) {
+        float acc[NT][CT][4];
+        int c[NT][CT][2][4], ones[NT][4];  // columns 4g + {0, 1} and 4g + {2, 3}: rows g and g + 8 of two products
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
+            for (int e = 0; e < 4; ++e) ones[nt][e] = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[nt][c][e] = 0.0f;
-
-    for (int s = s0; s < s1; s += 2) {
+            for (int k = 0; k < CT; ++k)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            int const step = s + u;
-            if (step >= s1) break;
-            if (step + 1 < s1) load_w(step + 1, w[u ^ 1]);
-            uint32_t b[NT][4];  // pairs (j, j + 4)
+                for (int e = 0; e < 4; ++e) acc[nt][k][e] = 0.0f, c[nt][k][0][e] = c[nt][k][1][e] = 0;
+        }
+        int left = left0;
+        uint2 const* digits = dig + lane;
+        for (int step = s0; step < s1; ++step) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(C::DEPTH - 1) : "memory");
+            uint4 const* const rs = ring + slot * (CT * 64) + lane;
+            if (++slot == C::DEPTH) slot = 0;
+            uint2 b[NT];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                float x[8];
-                load_x(step, nt, x);
+                b[nt] = digits[32 * nt];
+                mma_s8(ones[nt], 0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u, b[nt]);
+            }
+            // the last octets of a K that is no multiple of 32 meet digits of 0
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float const y0 = x[j] * up[nt], y1 = x[j + 4] * up[nt];
-                    __half2 const hi = __floats2half2_rn(y0, y1);
-                    float2 const f = __half22float2(hi);
-                    __half2 const lo = __floats2half2_rn(isinf(f.x) ? 0.0f : y0 - f.x, isinf(f.y) ? 0.0f : y1 - f.y);
-                    b[nt][j] = g & 1 ? bits(lo) : bits(hi);
+            for (int k = 0; k < CT; ++k) {
+                uint4 const w = rs[k * 64];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t const w0 = h ? w.z : w.x, w1 = h ? w.w : w.y;
+                    uint32_t const a0 = w0 & 0x0f0f0f0fu, a2 = (w0 >> 4) & 0x0f0f0f0fu;
+                    uint32_t const a1 = w1 & 0x0f0f0f0fu, a3 = (w1 >> 4) & 0x0f0f0f0fu;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma_s8(c[nt][k][h], a0, a1, a2, a3, b[nt]);
                 }
             }
-            int64_t const group = 32 * static_cast<int64_t>(step) / a.group;
+            digits += 32 * NT;
+            if (--left == 0 || step + 1 == s1) {
+                left = per_group;
 #pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                int64_t const n = col0 + 32 * c + 4 * g;
-                float sc[4] = {0.f, 0.f, 0.f, 0.f};
-                float const* ps = a.s + group * a.s_g;
-                if constexpr (VEC) {
-                    if (n < a.N) {
-                        float4 const v = __ldg(reinterpret_cast<float4 const*>(ps + n));
-                        sc[0] = v.x, sc[1] = v.y, sc[2] = v.z, sc[3] = v.w;
+                for (int k = 0; k < CT; ++k) {
+                    float4 const f = reinterpret_cast<float4 const*>(rs)[k * 64 + 32];
+                    float const sc[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        int const off = 8 * (ones[nt][0] * 256 + ones[nt][1]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            int (&q)[4] = c[nt][k][e / 2];
+                            int const i = 2 * (e & 1);
+                            acc[nt][k][e] = fmaf(static_cast<float>(q[i] * 256 + q[i + 1] - off), sc[e], acc[nt][k][e]);
+                            q[i] = q[i + 1] = 0;
+                        }
                     }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (n + e < a.N) sc[e] = __ldg(ps + (n + e) * a.s_n);
                 }
-                uint32_t h[4][4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) weights_of(w[u][c][e], h[e]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int e = 0; e < 4; e += 2) {  // columns 4g + e, 4g + e + 1 are rows g, g + 8 of the product
-                        float d[4];
-                        mma_f16_first(d, h[e][0], h[e + 1][0], h[e][1], h[e + 1][1], b[nt][0], b[nt][1]);
-                        mma_f16(d, h[e][2], h[e + 1][2], h[e][3], h[e + 1][3], b[nt][2], b[nt][3]);
-                        acc[nt][c][e] = fmaf(d[0] + d[1], sc[e], acc[nt][c][e]);
-                        acc[nt][c][e + 1] = fmaf(d[2] + d[3], sc[e + 1], acc[nt][c][e + 1]);
-                    }
+                    for (int e = 0; e < 4; ++e) ones[nt][e] = 0;
             }
+            fetch();
         }
-    }
-    // Warps to CTA.
+        // Warps to CTA: high and low digits, the row's factor, then the sums.
+        float* const sums = reinterpret_cast<float*>(smem + C::OFF_S) + round * (kWarps * C::ITEMS);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
-            *reinterpret_cast<float4*>(sums + (warp * ROWS + 4 * nt + t) * COLS + 32 * c + 4 * g) =
-                make_float4(acc[nt][c][0] * down[nt], acc[nt][c][1] * down[nt], acc[nt][c][2] * down[nt],
-                            acc[nt][c][3] * down[nt]);
-    __syncthreads();
-    int const rows = static_cast<int>(min(static_cast<int64_t>(ROWS), a.M - row0));
-    int const cols = static_cast<int>(min(static_cast<int64_t>(COLS), a.N - col0));
-    auto sum_warps = [&](int i) {
-        float v = 0.0f;
+            for (int k = 0; k < CT; ++k) {
+                float v[4];
 #pragma unroll
-        for (int k = 0; k < kWarps; ++k) v += sums[k * ITEMS + i];
-        return v;
-    };
-    auto store = [&](int i, float v) {
-        int const r = i / COLS, c = i - r * COLS;
-        if (r >= rows || c >= cols) return;
-        int64_t const m = row0 + r, n = col0 + c;
-        if (a.bias != nullptr) v += a.bias[n * a.b_n];
-        v = activate(v, a.act);
-        if (a.res != nullptr) v += a.res[m * a.r_m + n * a.r_n];
-        a.y[m * a.y_m + n * a.y_n] = v;
-    };
-    int const items = rows * COLS;
-    if (a.splits == 1) {
-        for (int i = tid; i < items; i += kThreads) store(i, sum_warps(i));
-        return;
-    }
-    // CTAs of the cluster: CTA s takes items [s * per, (s + 1) * per) of all of them.
-    cg::cluster_group cluster = cg::this_cluster();
-    int const per = (items + a.splits - 1) / a.splits;
-    float* recv = sums + kWarps * ITEMS;
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA runs
-    for (int i = tid; i < items; i += kThreads) {
-        int const to = i / per;
-        cluster.map_shared_rank(recv, to)[split * per + i - to * per] = sum_warps(i);
-    }
-    cluster_sync();
-    for (int i = split * per + tid; i < min(items, (split + 1) * per); i += kThreads) {
-        float v = 0.0f;
-        for (int k = 0; k < a.splits; ++k) v += recv[k * per + i - split * per];
-        store(i, v);
+                for (int e = 0; e < 4; ++e) {
+                    float const low = __shfl_down_sync(0xffffffffu, acc[nt][k][e], 1);
+                    v[e] = fmaf(acc[nt][k][e], 65536.0f, low) * down[nt];
+                }
+                if ((t & 1) == 0)
+                    *reinterpret_cast<float4*>(sums + (warp * C::ROWS + 2 * nt + t / 2) * C::COLS + 32 * k + 4 * g) =
+                        make_float4(v[0], v[1], v[2], v[3]);
+            }
+        __syncthreads();
+        int64_t const col0 = static_cast<int64_t>(tile) * C::COLS;
+        auto sum_warps = [&](int i) {
+            float v = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kWarps; ++k) v += sums[k * C::ITEMS + i];
+            return v;
+        };
+        auto store = [&](int i, float v) {
+            int const r = i / C::COLS;
+            int64_t const m = row0 + r, n = col0 + i - r * C::COLS;
+            if (n >= a.N) return;
+            if (a.bias != nullptr) v += a.bias[n * a.b_n];
+            v = activate(v, a.act);
+            if (a.res != nullptr) v += a.res[m * a.r_m + n * a.r_n];
+            a.y[m * a.y_m + n * a.y_n] = v;
+        };
+        if (a.splits == 1) {
+            for (int i = tid; i < items; i += kThreads) store(i, sum_warps(i));
+            continue;
+        }
+        // CTAs of the cluster: CTA s takes items [s * per, (s + 1) * per) of all of them.
+        cg::cluster_group cluster = cg::this_cluster();
+        float* const recv = reinterpret_cast<float*>(smem + C::OFF_R) + round * (C::ITEMS + kMaxCluster);
+        if (tile == tile0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA runs
+        for (int i = tid; i < items; i += kThreads) {
+            int const to = i / per;
+            cluster.map_shared_rank(recv, to)[split * per + i - to * per] = sum_warps(i);
+        }
+        cluster_sync();
+        for (int i = split * per + tid; i < min(items, (split + 1) * per); i += kThreads) {
+            float v = 0.0f;
+            for (int k = 0; k < a.splits; ++k) v += recv[k * per + i - split * per];
+            store(i, v);
+        }
     }
 }
 
 template <int CT, int NT, bool VEC>
 int launch(ann_stream stream, LinearQ4Args& a) {
-    constexpr int COLS = 32 * CT, ROWS = 4 * NT;
-    constexpr size_t smem = sizeof(float) * ((kWarps + 1) * ROWS * COLS + kMaxCluster);
+    using C = Q4<CT, NT>;
     auto const kernel = linear_q4_kernel<CT, NT, VEC>;
     static std::mutex mu;
     static std::set<int> ready;  // devices whose kernel attributes are set
@@ -283,25 +355,37 @@ int launch(ann_stream stream, LinearQ4Args& a) {
     {
         std::lock_guard<std::mutex> lock(mu);
         if (ready.count(dev) == 0) {
-            cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+            cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 static_cast<int>(C::OFF_D + kMaxDigits));
             if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
             if (e != cudaSuccess) return fail(ANN_ECUDA, "linearQ4 setup: %s", cudaGetErrorString(e));
             ready.insert(dev);
         }
     }
-    int64_t const tiles = ceil_div(a.N, COLS), row_tiles = ceil_div(a.M, ROWS);
-    int64_t const steps = ceil_div(a.K, 32);
+    int64_t const tiles = ceil_div(a.N, C::COLS), row_tiles = ceil_div(a.M, C::ROWS), steps = ceil_div(a.K, 32);
+    // Splits of the inputs: until every SM has two CTAs, as long as a warp keeps two
+    // steps; and as many as x's digits need to fit a CTA.
     int64_t const want = ceil_div(int64_t{2} * sm_count(), tiles * row_tiles);
-    a.splits = static_cast<int>(std::max<int64_t>(1, std::min({want, ceil_div(steps, 2 * kWarps), int64_t{kMaxCluster}})));
-    if (const char* e = std::getenv("TUNE_S")) a.splits = std::atoi(e);
-    if (tiles * a.splits > INT32_MAX || row_tiles > 65535) return fail(ANN_ENOTSUP, "linearQ4: grid too large.");
+    int64_t splits = std::max<int64_t>(1, std::min(want, steps / (2 * kWarps)));
+    if (const char* e = std::getenv("TUNE_S")) splits = std::atoi(e);
+    int64_t const per_step = static_cast<int64_t>(C::digits(1));
+    splits = std::max(splits, ceil_div((steps + kWarps) * per_step, kMaxDigits));
+    splits = std::min<int64_t>(splits, kMaxCluster);
+    int64_t const mine = ceil_div(steps, splits) + 1;  // steps of a CTA at most
+    if (mine * per_step > kMaxDigits) return fail(ANN_ENOTSUP, "linearQ4: too many inputs (%lld).", static_cast<long long>(a.K));
+    size_t const smem = C::OFF_D + static_cast<size_t>(mine * per_step);
+    a.splits = static_cast<int>(splits);
+    // As many clusters as fit the GPU at once, each with the same number of tiles or one less.
+    int64_t const room = std::max<int64_t>(1, int64_t{sm_count()} * (smem <= (110u << 10) && NT * CT < 4 ? 2 : 1) / (splits * row_tiles));
+    int64_t const rounds = ceil_div(tiles, room), clusters = ceil_div(tiles, rounds);
+    if (tiles > INT32_MAX || row_tiles > 65535) return fail(ANN_ENOTSUP, "linearQ4: grid too large.");
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = static_cast<unsigned>(a.splits);
     attr.val.clusterDim.y = 1;
     attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(tiles * a.splits), static_cast<unsigned>(row_tiles));
+    cfg.gridDim = dim3(static_cast<unsigned>(clusters * splits), static_cast<unsigned>(row_tiles));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = as_stream(stream);
@@ -317,11 +401,10 @@ int launch_vec(ann_stream stream, LinearQ4Args& a, bool vec) {
     return vec ? launch<CT, NT, true>(stream, a) : launch<CT, NT, false>(stream, a);
 }
 
-template <int CT>
-int launch_rows(ann_stream stream, LinearQ4Args& a, bool vec) {
-    if (a.M <= 4) return launch_vec<CT, 1>(stream, a, vec);
-    if (a.M <= 8) return launch_vec<CT, 2>(stream, a, vec);
-    return launch_vec<CT, 4>(stream, a, vec);
+int launch_rows(ann_stream stream, LinearQ4Args& a, bool vec, int cols) {
+    if (a.M <= 2) return cols == 1 ? launch_vec<1, 1>(stream, a, vec) : launch_vec<2, 1>(stream, a, vec);
+    if (a.M <= 4) return cols == 1 ? launch_vec<1, 2>(stream, a, vec) : launch_vec<2, 2>(stream, a, vec);
+    return cols == 1 ? launch_vec<1, 4>(stream, a, vec) : launch_vec<2, 4>(stream, a, vec);
 }
 
 constexpr int kPackThreads = 128;
@@ -417,8 +500,8 @@ int linear_q4(ann_stream stream, const ann_view* x_v, const ann_view* p_v, const
     a.x_vec = a.x_k == 1 && a.x_m % 4 == 0 && aligned(x.data, 16);
     bool const vec = a.w_n == 1 && a.w_r % 4 == 0 && aligned(p.data, 16) && a.s_n == 1 && a.s_g % 4 == 0 &&
                      aligned(s.data, 16) && a.N % 4 == 0;
-    bool const narrow = std::getenv("TUNE_C") ? std::atoi(std::getenv("TUNE_C")) == 1 : a.N * ceil_div(a.M, 16) < 2048;
-    return narrow ? launch_rows<1>(stream, a, vec) : launch_rows<4>(stream, a, vec);
+    int const cols = std::getenv("TUNE_C") ? std::atoi(std::getenv("TUNE_C")) : a.N * ceil_div(a.M, 16) < 2048 ? 1 : 4;
+    return launch_rows(stream, a, vec, cols);
 }
 
 int pack_q4(ann_stream stream, const ann_view* w_v, const ann_view* p_v, const ann_view* s_v, uint32_t group) {
