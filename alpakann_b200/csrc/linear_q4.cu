@@ -58,31 +58,33 @@ __device__ __forceinline__ float activate(float v, int act) {
 //
 // A CTA stays and takes one tile of 32 CT columns after another. Each of its warps
 // (and each CTA of a cluster, where columns are few) has inputs of its own, whose
-// digits it prepares once; it streams their weights through a ring
-// in shared memory (cp.async, each lane its own 16 bytes, on across tiles), 4 KB
-// in flight a warp. The warps' sums of a tile meet in shared memory, across a
-// cluster in the CTA that owns a share of the columns, which applies bias,
-// activation and residual. One launch, no scratch memory, no atomics, a fixed
-// order of sums.
+// digits it prepares once; it streams their weights, 128 inputs at a time (a quad
+// of products' depth), through a ring in shared memory (cp.async, on across tiles),
+// 4 to 8 KB in flight a warp. The warps' sums of a
+// tile meet in shared memory, across a cluster in the CTA that owns a share of the
+// columns, which applies bias, activation and residual. One launch, no scratch
+// memory, no atomics, a fixed order of sums.
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxCluster = 16;
-// Bytes of x's digits in a CTA: at most 61 steps a warp, 1952 inputs of |u d| <=
-// 1920, so that 256 times their sum fits 32 bits.
-constexpr int kMaxDigits = 120 << 10;
+// Bytes of x's digits in a CTA: at most 68 steps of 32 inputs a warp, whose digits'
+// products with nibbles, |u d| <= 1920, sum up to less than 2^23: 256 times that
+// fits 32 bits.
+constexpr size_t kMaxDigits = 136 << 10;
 
-// Shared memory: rings [kWarps][DEPTH][CT][2][32] uint4 (words, scales), two
-// buffers of sums [kWarps][ROWS][COLS] and of the cluster's [per * splits], digits
-// uint2 [steps of the CTA][NT][32].
+// Shared memory: rings [kWarps][DEPTH quads][4][CT][32] uint4, two buffers of sums
+// [kWarps][ROWS][COLS] and of the cluster's [per * splits]; then per quad of the
+// CTA digits uint2 [4][NT][32] and offsets int [4][NT][4].
 template <int CT, int NT>
 struct Q4 {
     static constexpr int COLS = 32 * CT, ROWS = 2 * NT, ITEMS = ROWS * COLS;
-    static constexpr int DEPTH = 8 / CT;  // steps of 32 inputs in flight a warp
-    static constexpr size_t RING = size_t{16} * DEPTH * CT * 2 * 32;  // of a warp
+    static constexpr int DEPTH = 4 / CT;                            // quads in flight a warp
+    static constexpr size_t RING = size_t{16} * DEPTH * 4 * CT * 32;  // of a warp
     static constexpr size_t OFF_S = RING * kWarps;
     static constexpr size_t OFF_R = OFF_S + sizeof(float) * 2 * kWarps * ITEMS;
     static constexpr size_t OFF_D = OFF_R + sizeof(float) * 2 * (ITEMS + kMaxCluster);
-    static constexpr size_t digits(int64_t steps) { return static_cast<size_t>(steps) * NT * 32 * sizeof(uint2); }
+    static constexpr size_t ROOM = kMaxDigits < 227 * 1024 - OFF_D ? kMaxDigits : 227 * 1024 - OFF_D;
+    static constexpr size_t QUAD = size_t{4} * NT * (32 * sizeof(uint2) + 4 * sizeof(int));
 };
 
 // c += a b, int8 products of depth 32, exact in int32.
@@ -108,54 +110,54 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
     int const split = static_cast<int>(blockIdx.x) % a.splits;
     if (a.splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // "this CTA runs"
     int64_t const row0 = static_cast<int64_t>(blockIdx.y) * C::ROWS;
-    // this warp's steps of 32 inputs
-    int const steps = static_cast<int>((a.K + 31) / 32), parts = a.splits * kWarps, part = split * kWarps + warp;
-    int const first = static_cast<int>(static_cast<int64_t>(steps) * (split * kWarps) / parts);  // the CTA's first
-    int const s0 = static_cast<int>(static_cast<int64_t>(steps) * part / parts);
-    int const s1 = static_cast<int>(static_cast<int64_t>(steps) * (part + 1) / parts);
+    // this warp's quads of 128 inputs, in steps of 32
+    int const quads = static_cast<int>((a.K + 127) / 128), parts = a.splits * kWarps, part = split * kWarps + warp;
+    int const first = static_cast<int>(static_cast<int64_t>(quads) * (split * kWarps) / parts);  // the CTA's first
+    int const q0 = static_cast<int>(static_cast<int64_t>(quads) * part / parts);
+    int const q1 = static_cast<int>(static_cast<int64_t>(quads) * (part + 1) / parts);
+    int const s0 = 4 * q0, s1 = min(4 * q1, static_cast<int>((a.K + 31) / 32));
     int const octets = static_cast<int>(a.K / 8), per_group = a.group / 32;
     int const tiles = static_cast<int>((a.N + C::COLS - 1) / C::COLS);
     int const tile0 = static_cast<int>(blockIdx.x) / a.splits, stride = static_cast<int>(gridDim.x) / a.splits;
 
-    uint4* const ring = reinterpret_cast<uint4*>(smem + C::RING * warp);
-    uint32_t const ring_u = smem_u32(ring) + 16 * lane;
-    uint2* const dig = reinterpret_cast<uint2*>(smem + C::OFF_D) + static_cast<size_t>(s0 - first) * NT * 32;
-    // Steps are fetched in the order of their use, tile after tile. Sums meet their
-    // scale after the last step of a group and after the last of the range.
-    int const left0 = per_group - s0 % per_group;  // steps of the first group
+    // A lane copies 16 bytes of word row lane / 8 of four, so that eight lanes take
+    // 128 consecutive bytes; the lane that uses them is (g, t) = (4 columns, row). The
+    // place within a row's 128 bytes is permuted by the row, which keeps both the
+    // writes and the reads off each other's banks.
+    int const fg = lane & 7, ft = lane >> 3;
+    uint4* const ring = reinterpret_cast<uint4*>(smem + C::RING * warp) + 8 * t + (g ^ (2 * t));
+    uint32_t const ring_u = smem_u32(smem + C::RING * warp) + 16 * (8 * ft + (fg ^ (2 * ft)));
+    unsigned char* const mine = smem + C::OFF_D + C::QUAD * (q0 - first);  // digits and offsets, quad by quad
+    // Quads are fetched in the order of their use, tile after tile.
     int64_t const w_step = 4 * a.w_r;
-    uint32_t const* const w0 = a.w + (4 * static_cast<int64_t>(s0) + t) * a.w_r + 4 * g * a.w_n;
-    float const* const sc0 = a.s + s0 / per_group * a.s_g + 4 * g * a.s_n;
+    uint32_t const* const w0 = a.w + (16 * static_cast<int64_t>(q0) + ft) * a.w_r + 4 * fg * a.w_n;
     uint32_t const* f_w = w0;
-    float const* f_s = sc0;
-    int f_tile = tile0, f_step = s0, f_left = left0, f_slot = 0, f_cols = 0;  // f_cols: columns from this lane's first on
+    int f_tile = tile0, f_quad = q0, f_slot = 0, f_cols = 0;  // f_cols: columns from this lane's first on, 0: none
     auto open_tile = [&]() {
         int64_t const col = static_cast<int64_t>(f_tile) * C::COLS;
         f_w = w0 + col * a.w_n;
-        f_s = sc0 + col * a.s_n;
-        f_cols = f_tile < tiles && s0 < s1 ? static_cast<int>(min(a.N - col, int64_t{C::COLS})) - 4 * g : INT_MIN;
-        f_step = s0, f_left = left0;
+        f_cols = f_tile < tiles && q0 < q1 ? max(0, static_cast<int>(min(a.N - col, int64_t{C::COLS})) - 4 * fg) : 0;
+        f_quad = q0;
     };
     auto fetch = [&]() {
-        if (f_cols != INT_MIN) {
-            uint32_t const dst = ring_u + static_cast<uint32_t>(f_slot) * (CT * 2 * 512);
-            bool const in = 4 * f_step + t < octets, last = f_left == 1 || f_step + 1 == s1;
+        if (f_tile < tiles && q0 < q1) {
+            uint32_t const dst = ring_u + static_cast<uint32_t>(f_slot) * (4 * CT * 512);
 #pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                if constexpr (VEC) {
-                    if (in && 32 * c < f_cols) copy16(dst + c * 1024, f_w + 32 * c);
-                    if (last && 32 * c < f_cols) copy16(dst + c * 1024 + 512, f_s + 32 * c);
-                } else {
+            for (int i = 0; i < 4; ++i) {
+                bool const in = 16 * f_quad + 4 * i + ft < octets;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (in && 32 * c + e < f_cols) copy4(dst + c * 1024 + 4 * e, f_w + (32 * c + e) * a.w_n);
-                        if (last && 32 * c + e < f_cols) copy4(dst + c * 1024 + 512 + 4 * e, f_s + (32 * c + e) * a.s_n);
+                for (int c = 0; c < CT; ++c) {
+                    if constexpr (VEC) {
+                        if (in && 32 * c < f_cols) copy16(dst + (i * CT + c) * 512, f_w + 32 * c);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (in && 32 * c + e < f_cols) copy4(dst + (i * CT + c) * 512 + 4 * e, f_w + (32 * c + e) * a.w_n);
                     }
                 }
+                f_w += w_step;
             }
-            f_w += w_step;
-            if (--f_left == 0) f_left = per_group, f_s += a.s_g;
-            if (++f_step == s1) f_tile += stride, open_tile();
+            if (++f_quad == q1) f_tile += stride, open_tile();
         }
         if (++f_slot == C::DEPTH) f_slot = 0;
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -198,10 +200,10 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
         // NaN and infinity have no whole numbers: the row's sums become NaN
         float const back = top >= 0x7f800000u ? __int_as_float(0x7fffffff) : __int_as_float((e - 29) << 23);
         if ((t >> 1) == (r & 1)) down[r / 2] = back;
-        for (int base = s0; base < s1; base += 8) {
+        for (int base = s0; base < 4 * q1; base += 8) {
             float x[8];
             load_x(r, base, x);
-            if (base + lane / 4 >= s1) continue;
+            if (base + lane / 4 >= 4 * q1) continue;
             uint32_t n[8];  // signed base-256 digits: a carry out of the lower bytes, then their signs
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -217,9 +219,49 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
                 d[h][2] = __byte_perm(lo01, lo23, 0x7632);
                 d[h][3] = __byte_perm(lo01, lo23, 0x5410);
             }
-            uint2* const to = dig + ((base - s0 + (lane >> 2)) * NT + r / 2) * 32 + (r & 1) * 16 + t;
+            int const st = base - s0 + (lane >> 2);
+            uint2* const to = reinterpret_cast<uint2*>(mine + C::QUAD * (st / 4)) + ((st % 4) * NT + r / 2) * 32 + (r & 1) * 16 + t;
 #pragma unroll
             for (int j = 0; j < 4; ++j) to[4 * j] = make_uint2(d[0][j], d[1][j]);
+        }
+    }
+    __syncwarp();
+
+    // Sums meet their scale after the last step of a group and after the range's
+    // last. The bits of such steps in a quad, given the steps left in its group.
+    int const left0 = per_group - s0 % per_group;
+    auto ends = [&](int quad, int& left) {
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (--left == 0) m |= 1u << i, left = per_group;
+        if (quad + 1 < q1) return m;
+        unsigned const last = 1u << (s1 - 1 - 4 * quad);  // steps past K have no group
+        return (m & (last - 1u)) | last;
+    };
+    // 256 times the high plus the low of a pair of digits' sums up to each of these
+    // steps: the nibbles' offset of 8, the same for all columns.
+    {
+        int ones[NT][4], left = left0;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) ones[nt][0] = ones[nt][1] = ones[nt][2] = ones[nt][3] = 0;
+        for (int quad = q0; quad < q1; ++quad) {
+            uint2 const* const dig = reinterpret_cast<uint2 const*>(mine + C::QUAD * (quad - q0)) + lane;
+            int* const off = reinterpret_cast<int*>(mine + C::QUAD * (quad - q0) + 4 * NT * 32 * sizeof(uint2));
+            unsigned const m = ends(quad, left);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    mma_s8(ones[nt], 0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u, dig[(i * NT + nt) * 32]);
+                if (m >> i & 1u) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        if (g == 0) off[(i * NT + nt) * 4 + t] = 8 * (ones[nt][0] * 256 + ones[nt][1]);
+                        ones[nt][0] = ones[nt][1] = ones[nt][2] = ones[nt][3] = 0;
+                    }
+                }
+            }
         }
     }
     __syncwarp();
@@ -228,67 +270,103 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
     int const items = rows * C::COLS, per = (items + a.splits - 1) / a.splits;
     int slot = 0;
     for (int tile = tile0, round = 0; tile < tiles; tile += stride, round ^= 1) {
+        int64_t const col0 = static_cast<int64_t>(tile) * C::COLS;
+        int const cols = static_cast<int>(min(a.N - col0, int64_t{C::COLS})) - 4 * g;  // from this lane's first on
+        float const* ps = a.s + static_cast<int64_t>(s0 / per_group) * a.s_g + (col0 + 4 * g) * a.s_n;
         float acc[NT][CT][4];
-        int c[NT][CT][2][4], ones[NT][4];  // columns 4g + {0, 1} and 4g + {2, 3}: rows g and g + 8 of two products
+        int c[NT][CT][2][4];  // columns 4g + {0, 1} and 4g + {2, 3}: rows g and g + 8 of two products
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) ones[nt][e] = 0;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int k = 0; k < CT; ++k)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[nt][k][e] = 0.0f, c[nt][k][0][e] = c[nt][k][1][e] = 0;
-        }
-        int left = left0;
-        uint2 const* digits = dig + lane;
-        for (int step = s0; step < s1; ++step) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(C::DEPTH - 1) : "memory");
-            uint4 const* const rs = ring + slot * (CT * 64) + lane;
-            if (++slot == C::DEPTH) slot = 0;
-            uint2 b[NT];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                b[nt] = digits[32 * nt];
-                mma_s8(ones[nt], 0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u, b[nt]);
-            }
-            // the last octets of a K that is no multiple of 32 meet digits of 0
+        // The scales of a step's group, this lane's columns.
+        auto scales = [&](float const* p, float4 (&sc)[CT]) {
 #pragma unroll
             for (int k = 0; k < CT; ++k) {
-                uint4 const w = rs[k * 64];
+                sc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                float const* pk = p + 32 * k * a.s_n;
+                if constexpr (VEC) {
+                    if (32 * k < cols) sc[k] = __ldg(reinterpret_cast<float4 const*>(pk));
+                } else {
+                    if (32 * k < cols) sc[k].x = __ldg(pk);
+                    if (32 * k + 1 < cols) sc[k].y = __ldg(pk + a.s_n);
+                    if (32 * k + 2 < cols) sc[k].z = __ldg(pk + 2 * a.s_n);
+                    if (32 * k + 3 < cols) sc[k].w = __ldg(pk + 3 * a.s_n);
+                }
+            }
+        };
+        // Octets past K and columns past N: whatever lies in the ring meets digits of
+        // 0, or is not stored.
+        auto multiply = [&](uint4 const (&w)[CT], uint2 const (&b)[NT]) {
+#pragma unroll
+            for (int k = 0; k < CT; ++k)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    uint32_t const w0 = h ? w.z : w.x, w1 = h ? w.w : w.y;
+                    uint32_t const w0 = h ? w[k].z : w[k].x, w1 = h ? w[k].w : w[k].y;
                     uint32_t const a0 = w0 & 0x0f0f0f0fu, a2 = (w0 >> 4) & 0x0f0f0f0fu;
                     uint32_t const a1 = w1 & 0x0f0f0f0fu, a3 = (w1 >> 4) & 0x0f0f0f0fu;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) mma_s8(c[nt][k][h], a0, a1, a2, a3, b[nt]);
                 }
-            }
-            digits += 32 * NT;
-            if (--left == 0 || step + 1 == s1) {
-                left = per_group;
+        };
+        auto flush = [&](int const* off, float4 const (&sc)[CT]) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                int const o = off[4 * nt];
 #pragma unroll
                 for (int k = 0; k < CT; ++k) {
-                    float4 const f = reinterpret_cast<float4 const*>(rs)[k * 64 + 32];
-                    float const sc[4] = {f.x, f.y, f.z, f.w};
+                    float const f[4] = {sc[k].x, sc[k].y, sc[k].z, sc[k].w};
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        int const off = 8 * (ones[nt][0] * 256 + ones[nt][1]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            int (&q)[4] = c[nt][k][e / 2];
-                            int const i = 2 * (e & 1);
-                            acc[nt][k][e] = fmaf(static_cast<float>(q[i] * 256 + q[i + 1] - off), sc[e], acc[nt][k][e]);
-                            q[i] = q[i + 1] = 0;
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        int (&q)[4] = c[nt][k][e / 2];
+                        int const j = 2 * (e & 1);
+                        acc[nt][k][e] = fmaf(static_cast<float>(q[j] * 256 + q[j + 1] - o), f[e], acc[nt][k][e]);
+                        q[j] = q[j + 1] = 0;
                     }
                 }
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) ones[nt][e] = 0;
             }
+        };
+        int left = left0;
+        for (int quad = q0; quad < q1; ++quad) {
+            unsigned const m = ends(quad, left);
+            float4 sc[CT];
+            if (m != 0u) scales(ps, sc);  // of the first step that needs them; used when the weights have come
+            uint2 const* const dig = reinterpret_cast<uint2 const*>(mine + C::QUAD * (quad - q0)) + lane;
+            int const* const off = reinterpret_cast<int const*>(mine + C::QUAD * (quad - q0) + 4 * NT * 32 * sizeof(uint2)) + t;
+            asm volatile("cp.async.wait_group %0;" ::"n"(C::DEPTH - 1) : "memory");
+            __syncwarp();
+            uint4 const* const rs = ring + slot * (4 * CT * 32);
+            if (++slot == C::DEPTH) slot = 0;
+            uint4 w[4][CT];
+            uint2 b[4][NT];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                for (int k = 0; k < CT; ++k) w[i][k] = rs[(i * CT + k) * 32];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) b[i][nt] = dig[(i * NT + nt) * 32];
+            }
+            __syncwarp();  // the warp has read the quad; its place takes another
             fetch();
+            if ((m & 7u) == 0u) {  // groups of 128 inputs or more: no sum ends within the quad
+#pragma unroll
+                for (int i = 0; i < 4; ++i) multiply(w[i], b[i]);
+                if (m != 0u) {
+                    flush(off + 12 * NT, sc);
+                    ps += a.s_g;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    multiply(w[i], b[i]);
+                    if ((m >> i & 1u) == 0u) continue;
+                    flush(off + 4 * NT * i, sc);
+                    ps += a.s_g;
+                    if (m >> (i + 1) != 0u) scales(ps, sc);
+                }
+            }
         }
         // Warps to CTA: high and low digits, the row's factor, then the sums.
         float* const sums = reinterpret_cast<float*>(smem + C::OFF_S) + round * (kWarps * C::ITEMS);
@@ -307,7 +385,6 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
                         make_float4(v[0], v[1], v[2], v[3]);
             }
         __syncthreads();
-        int64_t const col0 = static_cast<int64_t>(tile) * C::COLS;
         auto sum_warps = [&](int i) {
             float v = 0.0f;
 #pragma unroll
@@ -356,24 +433,24 @@ int launch(ann_stream stream, LinearQ4Args& a) {
         std::lock_guard<std::mutex> lock(mu);
         if (ready.count(dev) == 0) {
             cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 static_cast<int>(C::OFF_D + kMaxDigits));
+                                                 static_cast<int>(C::OFF_D + C::ROOM));
             if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
             if (e != cudaSuccess) return fail(ANN_ECUDA, "linearQ4 setup: %s", cudaGetErrorString(e));
             ready.insert(dev);
         }
     }
-    int64_t const tiles = ceil_div(a.N, C::COLS), row_tiles = ceil_div(a.M, C::ROWS), steps = ceil_div(a.K, 32);
-    // Splits of the inputs: until every SM has two CTAs, as long as a warp keeps two
-    // steps; and as many as x's digits need to fit a CTA.
+    int64_t const tiles = ceil_div(a.N, C::COLS), row_tiles = ceil_div(a.M, C::ROWS), quads = ceil_div(a.K, 128);
+    // Splits of the inputs: until every SM has two CTAs, as long as a warp keeps a
+    // quad; and as many as x's digits need to fit a CTA.
     int64_t const want = ceil_div(int64_t{2} * sm_count(), tiles * row_tiles);
-    int64_t splits = std::max<int64_t>(1, std::min(want, steps / (2 * kWarps)));
+    int64_t splits = std::max<int64_t>(1, std::min(want, quads / kWarps));
     if (const char* e = std::getenv("TUNE_S")) splits = std::atoi(e);
-    int64_t const per_step = static_cast<int64_t>(C::digits(1));
-    splits = std::max(splits, ceil_div((steps + kWarps) * per_step, kMaxDigits));
+    int64_t const per_quad = static_cast<int64_t>(C::QUAD);
+    splits = std::max(splits, ceil_div((quads + kWarps) * per_quad, static_cast<int64_t>(C::ROOM)));
     splits = std::min<int64_t>(splits, kMaxCluster);
-    int64_t const mine = ceil_div(steps, splits) + 1;  // steps of a CTA at most
-    if (mine * per_step > kMaxDigits) return fail(ANN_ENOTSUP, "linearQ4: too many inputs (%lld).", static_cast<long long>(a.K));
-    size_t const smem = C::OFF_D + static_cast<size_t>(mine * per_step);
+    int64_t const mine = ceil_div(quads, splits) + 1;  // quads of a CTA at most
+    if (mine * per_quad > static_cast<int64_t>(C::ROOM)) return fail(ANN_ENOTSUP, "linearQ4: too many inputs (%lld).", static_cast<long long>(a.K));
+    size_t const smem = C::OFF_D + static_cast<size_t>(mine * per_quad);
     a.splits = static_cast<int>(splits);
     // As many clusters as fit the GPU at once, each with the same number of tiles or one less.
     int64_t const room = std::max<int64_t>(1, int64_t{sm_count()} * (smem <= (110u << 10) && NT * CT < 4 ? 2 : 1) / (splits * row_tiles));
