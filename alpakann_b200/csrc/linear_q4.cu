@@ -163,13 +163,13 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     open_tile();
-#pragma unroll
-    for (int i = 0; i < C::DEPTH; ++i) fetch();
 
-    // x's digits: a lane takes an octet of a row at a time. First the rows' largest
-    // values, then the digits. Lanes t and t + 1 of a row's four slots hold its high
-    // and low digits, so a lane keeps the factor of row t / 2 of its two.
-    float down[NT];
+    // x's digits: a lane takes an octet of a row at a time, eight steps a warp. First
+    // the rows' largest values (the first eight steps' inputs stay in registers, and
+    // their loads go out before the weights'), then the digits. Lanes t and t + 1 of
+    // a row's four slots hold its high and low digits, so a lane keeps the factor of
+    // row t / 2 of its two.
+    float down[NT], up[C::ROWS];
     auto load_x = [&](int r, int base, float (&x)[8]) {
         int64_t const m = row0 + r, k = 32 * static_cast<int64_t>(base) + 8 * lane;
         bool const in = m < a.M && k < a.K && base + lane / 4 < s1;
@@ -184,30 +184,50 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
             for (int e = 0; e < 8; ++e) x[e] = in ? p[e * a.x_k] : 0.0f;
         }
     };
+    float x[C::ROWS][8];
 #pragma unroll
-    for (int r = 0; r < C::ROWS; ++r) {
-        unsigned int top = 0;  // max |x| on the bit patterns: NaN above infinity above every number
-        for (int base = s0; base < s1; base += 8) {
-            float x[8];
-            load_x(r, base, x);
+    for (int r = 0; r < C::ROWS; ++r) load_x(r, s0, x[r]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+    for (int i = 0; i < C::DEPTH; ++i) fetch();
+    {
+        unsigned int top[C::ROWS];  // max |x| on the bit patterns: NaN above infinity above every number
+        auto raise = [&](float (&y)[8], unsigned int& m) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(y[e]) & 0x7fffffffu);
+        };
+#pragma unroll
+        for (int r = 0; r < C::ROWS; ++r) raise(x[r], top[r] = 0);
+        for (int base = s0 + 8; base < s1; base += 8) {
+            float y[C::ROWS][8];
+#pragma unroll
+            for (int r = 0; r < C::ROWS; ++r) load_x(r, base, y[r]);
+#pragma unroll
+            for (int r = 0; r < C::ROWS; ++r) raise(y[r], top[r]);
         }
-        top = __reduce_max_sync(0xffffffffu, top);
-        // the largest value into [2^29, 2^30): 2^(156 - e), e its biased exponent, where both factors are normal
-        int const e = min(max(static_cast<int>(top >> 23), 31), 254);
-        float const up = __int_as_float((283 - e) << 23);
-        // NaN and infinity have no whole numbers: the row's sums become NaN
-        float const back = top >= 0x7f800000u ? __int_as_float(0x7fffffff) : __int_as_float((e - 29) << 23);
-        if ((t >> 1) == (r & 1)) down[r / 2] = back;
-        for (int base = s0; base < 4 * q1; base += 8) {
-            float x[8];
-            load_x(r, base, x);
-            if (base + lane / 4 >= 4 * q1) continue;
+#pragma unroll
+        for (int r = 0; r < C::ROWS; ++r) {
+            unsigned int const m = __reduce_max_sync(0xffffffffu, top[r]);
+            // the largest value into [2^29, 2^30): 2^(156 - e), e its biased exponent, where both factors are normal
+            int const e = min(max(static_cast<int>(m >> 23), 31), 254);
+            up[r] = __int_as_float((283 - e) << 23);
+            // NaN and infinity have no whole numbers: the row's sums become NaN
+            float const back = m >= 0x7f800000u ? __int_as_float(0x7fffffff) : __int_as_float((e - 29) << 23);
+            if ((t >> 1) == (r & 1)) down[r / 2] = back;
+        }
+    }
+    for (int base = s0; base < 4 * q1; base += 8) {
+        if (base != s0) {
+#pragma unroll
+            for (int r = 0; r < C::ROWS; ++r) load_x(r, base, x[r]);
+        }
+        int const st = base - s0 + (lane >> 2);
+        if (st >= 4 * (q1 - q0)) continue;
+#pragma unroll
+        for (int r = 0; r < C::ROWS; ++r) {
             uint32_t n[8];  // signed base-256 digits: a carry out of the lower bytes, then their signs
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                n[i] = (static_cast<uint32_t>(__float2int_rn(x[i] * up)) + 0x00808080u) ^ 0x00808080u;
+                n[i] = (static_cast<uint32_t>(__float2int_rn(x[r][i] * up[r])) + 0x00808080u) ^ 0x00808080u;
             // bytes of elements 0, 2, 4, 6 and 1, 3, 5, 7 (the two masks of a word), digit by digit
             uint32_t d[2][4];
 #pragma unroll
@@ -219,7 +239,6 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
                 d[h][2] = __byte_perm(lo01, lo23, 0x7632);
                 d[h][3] = __byte_perm(lo01, lo23, 0x5410);
             }
-            int const st = base - s0 + (lane >> 2);
             uint2* const to = reinterpret_cast<uint2*>(mine + C::QUAD * (st / 4)) + ((st % 4) * NT + r / 2) * 32 + (r & 1) * 16 + t;
 #pragma unroll
             for (int j = 0; j < 4; ++j) to[4 * j] = make_uint2(d[0][j], d[1][j]);
@@ -360,11 +379,17 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
+                    float4 next[CT];
+                    bool const ends_here = m >> i & 1u, another = ends_here && m >> (i + 1) != 0u;
+                    if (another) scales(ps + a.s_g, next);
                     multiply(w[i], b[i]);
-                    if ((m >> i & 1u) == 0u) continue;
+                    if (!ends_here) continue;
                     flush(off + 4 * NT * i, sc);
                     ps += a.s_g;
-                    if (m >> (i + 1) != 0u) scales(ps, sc);
+                    if (another) {
+#pragma unroll
+                        for (int k = 0; k < CT; ++k) sc[k] = next[k];
+                    }
                 }
             }
         }
