@@ -2,6 +2,7 @@
 
 alpakann_b200/csrc/*.cu -> alpakann_b200/_build/obj/*.o -> alpakann_b200/_build/libann_b200.so
 alpakann_b200/csrc/*.cpp (host-only code: file loading, hashing) -> g++ -> same library
+alpakann_b200/binding/binding.c -> gcc -> alpakann_b200/_build/_ann_binding.so (CPython module)
 
 nvcc -gencode arch=compute_100a,code=sm_100a -lineinfo -O3, C++20, static
 cudart inside the shared library (no dependency on the runtime version a
@@ -76,6 +77,24 @@ def _compile(src, extra):
     return obj
 
 
+BINDING_SRC = os.path.join(HERE, "binding", "binding.c")
+BINDING = os.path.join(OUT_DIR, "_ann_binding.so")
+
+
+def build_binding() -> str:
+    """The CPython module of the short calls (binding/binding.c), next to the
+    library it links, for the interpreter that runs this build."""
+    import sysconfig
+    if _stale(BINDING, [BINDING_SRC, __file__, os.path.join(INCLUDE, "ann_b200.h")]):
+        cmd = [cxx().replace("g++", "gcc"), "-O2", "-Wall", "-fPIC", "-shared", "-I", INCLUDE, "-I",
+               sysconfig.get_paths()["include"], BINDING_SRC, "-o", BINDING, "-L", OUT_DIR, "-lann_b200",
+               "-Wl,-rpath,$ORIGIN"]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"binding failed:\n{r.stdout}\n{r.stderr}")
+    return BINDING
+
+
 def build(force: bool = False, verbose_ptxas: bool = False) -> str:
     os.makedirs(OBJ_DIR, exist_ok=True)
     if force:
@@ -90,6 +109,7 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    build_binding()
     return LIB
 
 

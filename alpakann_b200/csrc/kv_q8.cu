@@ -4,8 +4,8 @@
 // one fp32 scale s per KV head and block of `block` tokens:
 //   k_cache, v_cache int8 [B, Hkv, Tcap, D] (or BTHD), scales [B, Hkv, ceil(Tcap / block)].
 //
-// append: s' = max(s of the block's earlier rows, max|x| / 127 over the new
-// rows in the block); a new value becomes the whole number nearest to the exact
+// append: s' = max(s of the block's earlier rows, max|x| times fp32's 1/127 over
+// the new rows in the block); a new value becomes the whole number nearest to the exact
 // quotient x / s' (ties to even); where s' grew, the block's earlier values are
 // rounded anew from n * s / s'. The rounding is exact, not that of a 32-bit
 // quotient, so any implementation of this definition gives the same integers.
@@ -45,7 +45,7 @@ struct AppendArgs {
 };
 
 // The whole number nearest to x / s, exactly, ties to even; |x| <= 127 s up to
-// the rounding of s. t is within 2^-16 of the quotient, so rint(t) is off by one
+// the roundings of s. t is within 2^-16 of the quotient, so rint(t) is off by one
 // at most; r = x - n s is exact in 32 bits (a multiple of half an ulp of s, at
 // most 2^24 of them), and comparing it with s / 2 puts n right.
 __device__ __forceinline__ int nearest(float x, float s, float inv) {
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) top = max(top, red[w]);
-    unsigned int const want = __float_as_uint(__fdiv_rn(__uint_as_float(top), 127.0f));
+    unsigned int const want = __float_as_uint(__uint_as_float(top) * (1.0f / 127.0f));
     float const s = __uint_as_float(max(want, __float_as_uint(old)));
     if (threadIdx.x == 0) *scale = s;  // every thread has read the old one before the barrier above
 

@@ -13,7 +13,7 @@ from dataclasses import dataclass
 
 import torch
 
-from .._capi import AnnView, check, lib, ref, view
+from .._capi import AnnView, binding, check, lib, ref, view
 from ._common import ext, fn, gemm, handle, suffix, trace
 
 BTHD, BHTD = 0, 1
@@ -297,13 +297,17 @@ class RotaryPairs(enum.IntEnum):
     halves = 1       # (p, p + P), P = number of frequencies
 
 
-def _typed(name, dtypes, **tensors):
-    """Element types of a call, and one CUDA device for all of it."""
+binding.types(torch.float32, torch.float64, torch.int8, torch.int32, torch.uint32)
+
+
+def _refuse(name, dtypes, tensors):
+    """Words why the binding found the call's tensors unfit (their element types,
+    or not all on one CUDA device)."""
+    dev = None
     for what, t in tensors.items():
         want = dtypes.get(what, torch.float32)
         if t is not None and t.dtype != want and not (want == torch.int32 and t.dtype == torch.uint32):
             raise TypeError(f"{name}: {what} must be {want}, got {t.dtype}")
-    dev = None
     for what, t in tensors.items():
         if t is None or t.device == dev:
             continue
@@ -312,24 +316,28 @@ def _typed(name, dtypes, **tensors):
         dev = t.device
         if dev.type != "cuda":
             raise ValueError(f"{name} needs CUDA tensors, got {what} on {dev}")
-    return dev
+    raise TypeError(f"{name}: a tensor of more than 8 dimensions, or an argument that is no tensor")
 
 
-def _call(name, queue, dev, *args):
-    """The C call on `queue`, or on the current stream of the tensors' device."""
-    f = getattr(lib, name)
-    if isinstance(queue, torch.cuda.Stream) and queue.device != dev:
-        raise ValueError(f"{name}: the stream is on {queue.device}, the tensors on {dev}")
-    stream = torch.cuda.current_stream(dev).cuda_stream if queue is None else handle(queue)
-    if torch.cuda.current_device() == dev.index:
-        check(f(stream, *args))
+def _run(name, entry, dtypes, queue, tensors, *scalars):
+    """One call of the binding on `queue`, or on the current stream of the tensors'
+    device (the first tensor's; the binding refuses others)."""
+    values = tensors.values()
+    dev = next(iter(values)).get_device()
+    if queue is None:
+        stream = torch._C._cuda_getCurrentRawStream(dev) if dev >= 0 else 0
+    else:
+        stream = handle(queue)
+        if isinstance(queue, torch.cuda.Stream) and queue.device.index != dev and dev >= 0:
+            raise ValueError(f"{name}: the stream is on {queue.device}, the tensors on cuda:{dev}")
+    if dev < 0 or torch._C._cuda_getDevice() == dev:
+        rc = entry(stream, *values, *scalars)
     else:
         with torch.cuda.device(dev):
-            check(f(stream, *args))
-
-
-def _ref(t):
-    return None if t is None else ref(t)
+            rc = entry(stream, *values, *scalars)
+    if rc == -1:
+        _refuse(name, dtypes, tensors)
+    check(rc)
 
 
 def rotaryFrequencies(queue, exec, frequencies, base=10000.0, factor=1.0, trainedLength=0, lowTurns=1.0,
@@ -339,9 +347,15 @@ def rotaryFrequencies(queue, exec, frequencies, base=10000.0, factor=1.0, traine
     (trainedLength 0), or by parts: those that turn more than highTurns times
     over trainedLength tokens are kept, those below lowTurns divided, the ones
     between blended linearly."""
-    dev = _typed("rotaryFrequencies", {"frequencies": torch.float64}, frequencies=frequencies)
-    _call("ann_rotary_frequencies", queue, dev, ref(frequencies), float(base), float(factor), float(trainedLength),
-          float(lowTurns), float(highTurns))
+    if frequencies.dtype != torch.float64 or frequencies.device.type != "cuda":
+        _refuse("rotaryFrequencies", {"frequencies": torch.float64}, {"frequencies": frequencies})
+    with torch.cuda.device(frequencies.device):
+        check(lib.ann_rotary_frequencies(handle(queue), ref(frequencies), float(base), float(factor),
+                                         float(trainedLength), float(lowTurns), float(highTurns)))
+
+
+_ROTARY_TYPES = {t: {"q": t, "k": t, "outQ": t, "outK": t, "positions": torch.int32, "frequencies": torch.float64}
+                 for t in (torch.float32, torch.float64)}
 
 
 def rotary(queue, exec, q, k, positions, frequencies, outQ, outK, pairs=RotaryPairs.interleaved, layout=BTHD,
@@ -351,12 +365,11 @@ def rotary(queue, exec, q, k, positions, frequencies, outQ, outK, pairs=RotaryPa
     int32 [B,T] or [T]; frequencies: float64, P <= D/2 pairs; elements from 2P
     on are copied. inverse applies the transposed rotation: the gradients of q
     and k from those of outQ and outK."""
-    sfx = suffix(q, k, outQ, outK)
-    dev = _typed("rotary", {"q": q.dtype, "k": q.dtype, "outQ": q.dtype, "outK": q.dtype, "positions": torch.int32,
-                            "frequencies": torch.float64},
-                 q=q, k=k, positions=positions, frequencies=frequencies, outQ=outQ, outK=outK)
-    _call(f"ann_rotary_{sfx}", queue, dev, ref(q), _ref(k), ref(positions), ref(frequencies), ref(outQ), _ref(outK),
-          int(pairs), int(layout), float(magnitude), 1 if inverse else 0)
+    if q.dtype not in _ROTARY_TYPES:
+        suffix(q)
+    _run("rotary", binding.rotary_f32 if q.dtype == torch.float32 else binding.rotary_f64, _ROTARY_TYPES[q.dtype],
+         queue, {"q": q, "k": k, "positions": positions, "frequencies": frequencies, "outQ": outQ, "outK": outK},
+         int(pairs), int(layout), float(magnitude), 1 if inverse else 0)
 
 
 _CACHE_TYPES = {"kCache": torch.int8, "vCache": torch.int8, "positions": torch.int32, "counts": torch.int32,
@@ -370,10 +383,9 @@ def kvCacheAppendQ8(queue, exec, kNew, vNew, kCache, vCache, kScale, vScale, pos
     defaults to Tn). kScale, vScale: float32 [B, Hkv, ceil(Tcap /
     tokensPerScale)], one scale per head and block of tokens; a block whose
     scale grows has its earlier tokens rounded anew."""
-    dev = _typed("kvCacheAppendQ8", _CACHE_TYPES, kNew=kNew, vNew=vNew, kCache=kCache, vCache=vCache, kScale=kScale,
-                 vScale=vScale, positions=positions, counts=counts)
-    _call("ann_kv_cache_append_q8_f32", queue, dev, ref(kNew), ref(vNew), ref(kCache), ref(vCache), ref(kScale),
-          ref(vScale), ref(positions), _ref(counts), int(tokensPerScale), int(kvLayout))
+    _run("kvCacheAppendQ8", binding.kv_cache_append_q8, _CACHE_TYPES, queue,
+         {"kNew": kNew, "vNew": vNew, "kCache": kCache, "vCache": vCache, "kScale": kScale, "vScale": vScale,
+          "positions": positions, "counts": counts}, int(tokensPerScale), int(kvLayout))
 
 
 def kvCacheReadQ8(queue, exec, kCache, vCache, kScale, vScale, kOut, vOut, tokensPerScale, lengths=None,
@@ -381,10 +393,9 @@ def kvCacheReadQ8(queue, exec, kCache, vCache, kScale, vScale, kOut, vOut, token
     """The float32 rows that an 8-bit cache stands for, for the tokens before
     lengths[b] (int32 [B], default all of kOut); rows behind are left as they
     were. Feeds attentionPrefill with a cached prefix."""
-    dev = _typed("kvCacheReadQ8", _CACHE_TYPES, kCache=kCache, vCache=vCache, kScale=kScale, vScale=vScale, kOut=kOut,
-                 vOut=vOut, lengths=lengths)
-    _call("ann_kv_cache_read_q8_f32", queue, dev, ref(kCache), ref(vCache), ref(kScale), ref(vScale), ref(kOut),
-          ref(vOut), _ref(lengths), int(tokensPerScale), int(kvLayout))
+    _run("kvCacheReadQ8", binding.kv_cache_read_q8, _CACHE_TYPES, queue,
+         {"kCache": kCache, "vCache": vCache, "kScale": kScale, "vScale": vScale, "kOut": kOut, "vOut": vOut,
+          "lengths": lengths}, int(tokensPerScale), int(kvLayout))
 
 
 def attentionDecodeQ8(queue, exec, Q, kCache, vCache, kScale, vScale, out, tokensPerScale, lengths=None, scale=None,
@@ -394,21 +405,27 @@ def attentionDecodeQ8(queue, exec, Q, kCache, vCache, kScale, vScale, out, token
     default the whole cache). causal: query i sees the keys before
     lengths[b] - Tq + 1 + i; a query that sees none gives zeros. scale defaults
     to 1/sqrt(D)."""
-    dev = _typed("attentionDecodeQ8", _CACHE_TYPES, Q=Q, kCache=kCache, vCache=vCache, kScale=kScale, vScale=vScale,
-                 out=out, lengths=lengths)
     if scale is None:
         scale = 1.0 / math.sqrt(Q.shape[3])
-    _call("ann_attention_decode_q8_f32", queue, dev, ref(Q), ref(kCache), ref(vCache), ref(kScale), ref(vScale),
-          _ref(lengths), ref(out), float(scale), int(queriesPerKvGroup), int(tokensPerScale), int(kvLayout),
-          1 if causal else 0)
+    _run("attentionDecodeQ8", binding.attention_decode_q8, _CACHE_TYPES, queue,
+         {"Q": Q, "kCache": kCache, "vCache": vCache, "kScale": kScale, "vScale": vScale, "lengths": lengths,
+          "out": out}, float(scale), int(queriesPerKvGroup), int(tokensPerScale), int(kvLayout), 1 if causal else 0)
 
 
 def packWeightQ4(queue, exec, weight, packed, scales, groupSize):
     """A float32 weight [K,N] (row-major [in, out]) in 4 bits: packed int32
     [K/8,N], eight inputs a word, scales float32 [ceil(K/groupSize),N]. Once,
     when the weights are loaded."""
-    dev = _typed("packWeightQ4", {"packed": torch.int32}, weight=weight, packed=packed, scales=scales)
-    _call("ann_pack_weight_q4_f32", queue, dev, ref(weight), ref(packed), ref(scales), int(groupSize))
+    tensors = {"weight": weight, "packed": packed, "scales": scales}
+    if (weight.dtype != torch.float32 or packed.dtype not in (torch.int32, torch.uint32) or
+            scales.dtype != torch.float32 or weight.device.type != "cuda" or
+            not (weight.device == packed.device == scales.device)):
+        _refuse("packWeightQ4", {"packed": torch.int32}, tensors)
+    with torch.cuda.device(weight.device):
+        check(lib.ann_pack_weight_q4_f32(handle(queue), ref(weight), ref(packed), ref(scales), int(groupSize)))
+
+
+_LINEAR_TYPES = {"packed": torch.int32}
 
 
 def linearQ4(queue, exec, input, packed, scales, output, groupSize, bias=None, activation=Activation.none,
@@ -416,10 +433,9 @@ def linearQ4(queue, exec, input, packed, scales, output, groupSize, bias=None, a
     """output = activation(input . W + bias) + residual with W in 4 bits
     (packWeightQ4): linear, linearBias and outputProjectionResidual for the few
     rows of a decode step. residual may be output."""
-    dev = _typed("linearQ4", {"packed": torch.int32}, input=input, packed=packed, scales=scales, output=output,
-                 bias=bias, residual=residual)
-    _call("ann_linear_q4_f32", queue, dev, ref(input), ref(packed), ref(scales), _ref(bias), _ref(residual),
-          ref(output), int(groupSize), int(activation))
+    _run("linearQ4", binding.linear_q4, _LINEAR_TYPES, queue,
+         {"input": input, "packed": packed, "scales": scales, "bias": bias, "residual": residual, "output": output},
+         int(groupSize), int(activation))
 
 
 def raise_shape(msg):

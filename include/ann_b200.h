@@ -509,7 +509,7 @@ int ann_rotary_frequencies(ann_stream stream, const ann_view* frequencies, doubl
  * [positions[b], positions[b] + counts[b]) of sequence b (positions, counts:
  * int32 [B]; counts NULL = Tn, values are held to [0, Tn]; rows past the count
  * are padding and not read). A touched block's scale becomes the larger of
- * max|x| / 127 over its new rows and, if it holds tokens before positions[b],
+ * max|x| * (1/127), both in float32, over its new rows and, if it holds tokens before positions[b],
  * its old scale (its absolute value, should a caller have stored a negative
  * one); new values are the whole numbers nearest to the exact quotient
  * x / scale (ties to even, within [-127, 127]); where the scale grew, the

@@ -41,7 +41,7 @@ def append(x, cache, scale, start, count, block):
         rows = x[a - start:b - start]
         with np.errstate(all="ignore"):
             top = np.float32(np.nan) if np.isnan(rows).any() else np.abs(rows).max()
-            s = np.float32(top / np.float32(127))
+            s = np.float32(top * (np.float32(1) / np.float32(127)))
             if j * block < lo:
                 old = np.abs(scale[j])
                 s = old if np.isnan(old) or (not np.isnan(s) and old > s) else s

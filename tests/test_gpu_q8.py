@@ -98,7 +98,7 @@ def test_append_ties_zeros_and_tiny_values(nn):
     block, D = 16, 128
     for amp in (127.0, 12.7, 3e38, 1e-25, 1e-33, 1e-38, 1e-43, 0.0):
         with np.errstate(all="ignore"):
-            s = np.float32(np.float32(amp) / np.float32(127))
+            s = np.float32(np.float32(amp) * (np.float32(1) / np.float32(127)))
             n = np.arange(-64, 64) + 0.5
             x = np.tile((n * np.float64(s)).astype(np.float32), (block, 1))
             x[1] = np.nextafter(x[0], np.float32(np.inf))
