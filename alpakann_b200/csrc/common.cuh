@@ -123,6 +123,23 @@ struct Vec16<double> {
     static constexpr int n = 2;
 };
 
+// Division of n < 2^31 by an invariant d >= 1 as a multiply and a shift
+// (Granlund and Montgomery, "Division by invariant integers using
+// multiplication", 1994): with l = ceil(log2 d) and m = ceil(2^(31+l) / d),
+// which fits in 32 bits, n / d = (n * m) >> (31 + l) for every n < 2^31.
+struct FastDiv {
+    uint32_t d, m, shift;
+    static FastDiv make(uint32_t d) {
+        uint32_t l = 0;
+        while ((uint64_t{1} << l) < d) ++l;
+        uint64_t const num = uint64_t{1} << (31 + l);
+        return FastDiv{d, static_cast<uint32_t>((num + d - 1) / d), 31 + l};
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t n) const {
+        return static_cast<uint32_t>((static_cast<uint64_t>(n) * m) >> shift);
+    }
+};
+
 __host__ __device__ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // (batch, head) pairs per dispatch chunk of a prefill grid: as many as keep one

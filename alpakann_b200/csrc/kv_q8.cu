@@ -25,6 +25,7 @@ namespace {
 __device__ unsigned int g_kv_q8_error;
 
 constexpr int kThreads = 256;
+constexpr int kHeld = 8;  // 16-byte vectors of a thread kept between append's two passes
 
 struct CacheTensor {
     int8_t* q;
@@ -41,7 +42,8 @@ struct AppendArgs {
     const int32_t* counts;  // may be null: every row
     int64_t pos_s, counts_s;
     int64_t Tn, H, D, cap, block, touched;  // touched: blocks a sequence's rows can reach
-    int vec;                                // rows of 4 aligned values
+    FastDiv row;                            // by the items of a row: 4 aligned values (vec) or one
+    int vec;
 };
 
 // The whole number nearest to x / s, exactly, ties to even; |x| <= 127 s up to
@@ -56,12 +58,38 @@ __device__ __forceinline__ int nearest(float x, float s, float inv) {
     if (r < -half || (r == -half && odd)) n -= 1.0f;
     return max(-127, min(127, static_cast<int>(n)));
 }
+// Four of them as bytes. Adding 1.5 * 2^23 rounds x / s to a whole number whose low
+// byte is the sum's; where it may be off, the remainder says so, and the value
+// (one in thousands) is rounded as above.
+__device__ __forceinline__ uint32_t nearest4(float4 x, float s, float inv) {
+    float const magic = 12582912.0f;
+    float const y0 = fmaf(x.x, inv, magic), y1 = fmaf(x.y, inv, magic), y2 = fmaf(x.z, inv, magic),
+                y3 = fmaf(x.w, inv, magic);
+    float const r0 = fmaf(magic - y0, s, x.x), r1 = fmaf(magic - y1, s, x.y), r2 = fmaf(magic - y2, s, x.z),
+                r3 = fmaf(magic - y3, s, x.w);
+    uint32_t const lo = __byte_perm(__float_as_uint(y0), __float_as_uint(y1), 0x0040),
+                   hi = __byte_perm(__float_as_uint(y2), __float_as_uint(y3), 0x0040);
+    uint32_t bytes = __byte_perm(lo, hi, 0x5410);
+    if (fmaxf(fmaxf(fabsf(r0), fabsf(r1)), fmaxf(fabsf(r2), fabsf(r3))) >= 0.5f * s) {
+        char4 const n = make_char4(nearest(x.x, s, inv), nearest(x.y, s, inv), nearest(x.z, s, inv), nearest(x.w, s, inv));
+        bytes = *reinterpret_cast<uint32_t const*>(&n);
+    }
+    return bytes;
+}
+// The larger of |x| and m, NaN if either is.
+__device__ __forceinline__ float max_abs(float x, float m) {
+    float v;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(fabsf(x)), "f"(m));
+    return v;
+}
 // The same in 64 bits, for scales so small that the 32-bit remainder is not
 // exact, and for requantised values n_old * s_old / s.
 __device__ __forceinline__ int nearest64(double x, double s) {
     return static_cast<int>(fmin(fmax(rint(x / s), -127.0), 127.0));
 }
 
+// STEP: a row's items divide the block's threads, which then step over rows.
+template <bool STEP>
 __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
     __shared__ unsigned int red[kThreads / 32];
     int64_t unit = blockIdx.x;
@@ -89,23 +117,45 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
     float* scale = c.scale + b * c.s_b + h * c.s_h + j * c.s_j;
     int const rows = static_cast<int>(hi - lo), D = static_cast<int>(a.D);
 
-    // max |x| on the bit patterns: ordered like the values, infinity above every
-    // number and NaN above infinity.
-    unsigned int top = 0;
-    if (a.vec) {
-        int const dv = D / 4;
-        for (int i = threadIdx.x; i < rows * dv; i += kThreads) {
-            int const r = i / dv, d = i - r * dv;
-            uint4 const v = *reinterpret_cast<uint4 const*>(x + r * x_t + 4 * d);
-            top = max(max(max(top, v.x & 0x7fffffffu), v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
+    // The first kHeld items of a thread stay in registers between the two passes (a
+    // block of 64 tokens of 128 values whole), loaded at once; later ones are read
+    // again.
+    int const per = static_cast<int>(a.row.d), items = rows * per;  // of a row, of the new rows
+    int const r0 = static_cast<int>(a.row.div(threadIdx.x)), c0 = static_cast<int>(threadIdx.x) - r0 * per;
+    auto place = [&](int u, int& r, int& col) {  // item threadIdx.x + u * kThreads
+        if constexpr (STEP) {
+            r = r0 + u * (kThreads / per);
+            col = c0;
+        } else {
+            int const i = static_cast<int>(threadIdx.x) + u * kThreads;
+            r = static_cast<int>(a.row.div(i));
+            col = i - r * per;
         }
+    };
+    int const mine = (items - static_cast<int>(threadIdx.x) + kThreads - 1) / kThreads;  // items of this thread
+    auto vector = [&](int u) {
+        int r, col;
+        place(u, r, col);
+        return *reinterpret_cast<float4 const*>(x + r * x_t + 4 * col);
+    };
+    float most = 0.0f;
+    auto raise = [&](float4 v) { most = max_abs(v.x, max_abs(v.y, max_abs(v.z, max_abs(v.w, most)))); };
+    float4 held[kHeld];
+    if (a.vec) {
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) held[u] = u < mine ? vector(u) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) raise(held[u]);
+        for (int u = kHeld; u < mine; ++u) raise(vector(u));
     } else {
-        for (int i = threadIdx.x; i < rows * D; i += kThreads) {
-            int const r = i / D, d = i - r * D;
-            top = max(top, __float_as_uint(x[r * x_t + d * x_d]) & 0x7fffffffu);
+        for (int u = 0; u < mine; ++u) {
+            int r, col;
+            place(u, r, col);
+            most = max_abs(x[r * x_t + col * x_d], most);
         }
     }
-    top = __reduce_max_sync(0xffffffffu, top);
+    // on the bit patterns: ordered like the values, infinity above every number and NaN above infinity
+    unsigned int top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
     bool const begun = j * a.block < lo;  // the block holds earlier rows
     float const old = begun ? fabsf(*scale) : 0.0f;
@@ -126,24 +176,32 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
             *p = static_cast<int8_t>(finite ? nearest64(static_cast<double>(*p) * old, s) : 0);
         }
     }
-    bool const tiny = s < 1e-30f;  // 64-bit rounding below: the remainder's ulp argument needs normal numbers
+    // 64-bit rounding for tiny scales: the remainder's ulp argument needs normal numbers
+    bool const usual = finite && s >= 1e-30f;
     float const inv = 1.0f / s;
-    auto round1 = [&](float v) {
-        if (!finite) return 0;
-        return tiny ? nearest64(v, s) : nearest(v, s, inv);
+    auto round1 = [&](float v) { return usual ? nearest(v, s, inv) : finite ? nearest64(v, s) : 0; };
+    auto write4 = [&](int u, float4 v) {
+        int r, col;
+        place(u, r, col);
+        uint32_t bytes;
+        if (usual) {
+            bytes = nearest4(v, s, inv);
+        } else {
+            char4 const n = make_char4(round1(v.x), round1(v.y), round1(v.z), round1(v.w));
+            bytes = *reinterpret_cast<uint32_t const*>(&n);
+        }
+        *reinterpret_cast<uint32_t*>(q + (lo + r) * c.q_t + 4 * col) = bytes;
     };
     if (a.vec) {
-        int const dv = D / 4;
-        for (int i = threadIdx.x; i < rows * dv; i += kThreads) {
-            int const r = i / dv, d = i - r * dv;
-            float4 const v = *reinterpret_cast<float4 const*>(x + r * x_t + 4 * d);
-            char4 const n = make_char4(round1(v.x), round1(v.y), round1(v.z), round1(v.w));
-            *reinterpret_cast<char4*>(q + (lo + r) * c.q_t + 4 * d) = n;
-        }
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u)
+            if (u < mine) write4(u, held[u]);
+        for (int u = kHeld; u < mine; ++u) write4(u, vector(u));
     } else {
-        for (int i = threadIdx.x; i < rows * D; i += kThreads) {
-            int const r = i / D, d = i - r * D;
-            q[(lo + r) * c.q_t + d * c.q_d] = static_cast<int8_t>(round1(x[r * x_t + d * x_d]));
+        for (int u = 0; u < mine; ++u) {
+            int r, col;
+            place(u, r, col);
+            q[(lo + r) * c.q_t + col * c.q_d] = static_cast<int8_t>(round1(x[r * x_t + col * x_d]));
         }
     }
 }
@@ -154,13 +212,15 @@ struct ReadArgs {
     int64_t o_b[2], o_h[2], o_t[2], o_d[2];
     const int32_t* lengths;  // may be null: every row
     int64_t len_s;
-    int64_t H, D, Tout, block, chunks;  // chunks of kReadItems items per (batch, head)
+    int64_t H, D, Tout, chunks;  // chunks of kReadItems items per (batch, head)
+    FastDiv row, block;          // by the items of a row (4 aligned values, or one), by a block's tokens
     int vec;
 };
 
-constexpr int kReadItems = kThreads * 8;
+constexpr int kReadEach = 4;  // items of a thread
+constexpr int kReadItems = kThreads * kReadEach;
 
-template <bool VEC>
+template <bool VEC, bool STEP>
 __global__ void __launch_bounds__(kThreads) read_kernel(ReadArgs a) {
     int64_t unit = blockIdx.x;
     int64_t const chunk = unit % a.chunks;
@@ -168,27 +228,44 @@ __global__ void __launch_bounds__(kThreads) read_kernel(ReadArgs a) {
     int const kv = static_cast<int>(unit & 1);
     unit >>= 1;
     int64_t const h = unit % a.H, b = unit / a.H;
-    int64_t rows = a.Tout;
-    if (a.lengths != nullptr) rows = min(rows, max(int64_t{0}, static_cast<int64_t>(a.lengths[b * a.len_s])));
     CacheTensor const& c = kv ? a.c[1] : a.c[0];
     int8_t const* q = c.q + b * c.q_b + h * c.q_h;
     float const* scale = c.scale + b * c.s_b + h * c.s_h;
     float* out = (kv ? a.out[1] : a.out[0]) + b * (kv ? a.o_b[1] : a.o_b[0]) + h * (kv ? a.o_h[1] : a.o_h[0]);
     int64_t const o_t = kv ? a.o_t[1] : a.o_t[0], o_d = kv ? a.o_d[1] : a.o_d[0];
-    int64_t const per = VEC ? a.D / 4 : a.D;  // items per row
-    int64_t const total = rows * per, base = chunk * kReadItems + threadIdx.x;
-#pragma unroll 4
-    for (int u = 0; u < 8; ++u) {
-        int64_t const i = base + u * kThreads;
-        if (i >= total) break;
-        int64_t const t = i / per, d = i - t * per;
-        float const s = scale[t / a.block * c.s_j];
-        if constexpr (VEC) {
-            char4 const n = *reinterpret_cast<char4 const*>(q + t * c.q_t + 4 * d);
-            *reinterpret_cast<float4*>(out + t * o_t + 4 * d) = make_float4(n.x * s, n.y * s, n.z * s, n.w * s);
-        } else {
-            out[t * o_t + d * o_d] = static_cast<float>(q[t * c.q_t + d * c.q_d]) * s;
-        }
+    uint32_t const per = a.row.d, base = static_cast<uint32_t>(chunk) * kReadItems + threadIdx.x;
+    uint32_t const t0 = a.row.div(base), c0 = base - t0 * per, all = static_cast<uint32_t>(a.Tout);
+    auto place = [&](int u, uint32_t& t, uint32_t& col) {
+        t = STEP ? t0 + u * (kThreads / per) : a.row.div(base + u * kThreads);
+        col = STEP ? c0 : base + u * kThreads - t * per;
+    };
+    // All loads of a thread at once, the length among them: rows past it are read
+    // (they are part of the cache) and not written.
+    float s[kReadEach];
+    char4 n[kReadEach];
+#pragma unroll
+    for (int u = 0; u < kReadEach; ++u) {
+        uint32_t t, col;
+        place(u, t, col);
+        if (t >= all) continue;
+        s[u] = scale[a.block.div(t) * c.s_j];
+        if constexpr (VEC)
+            n[u] = *reinterpret_cast<char4 const*>(q + t * c.q_t + 4 * col);
+        else
+            n[u].x = q[t * c.q_t + col * c.q_d];
+    }
+    int64_t rows = a.Tout;
+    if (a.lengths != nullptr) rows = min(rows, max(int64_t{0}, static_cast<int64_t>(a.lengths[b * a.len_s])));
+#pragma unroll
+    for (int u = 0; u < kReadEach; ++u) {
+        uint32_t t, col;
+        place(u, t, col);
+        if (t >= rows) continue;
+        if constexpr (VEC)
+            *reinterpret_cast<float4*>(out + t * o_t + 4 * col) =
+                make_float4(n[u].x * s[u], n[u].y * s[u], n[u].z * s[u], n[u].w * s[u]);
+        else
+            out[t * o_t + col * o_d] = n[u].x * s[u];
     }
 }
 
@@ -273,11 +350,13 @@ int append(ann_stream stream, const ann_view* kn, const ann_view* vn, const ann_
         a.x_d[k] = x[k].str[3];
         if (!rows4(x[k], sizeof(float)) || !rows4(q[k], 1)) a.vec = 0;
     }
+    a.row = FastDiv::make(static_cast<uint32_t>(a.vec ? a.D / 4 : a.D));
     // Rows start anywhere in a block: at most this many blocks hold some of them.
     a.touched = std::min(ceil_div(a.cap, block), ceil_div(a.Tn - 1, block) + 1);
     int64_t const grid = B * a.H * 2 * a.touched;
     if (grid > INT32_MAX) return fail(ANN_ENOTSUP, "kvCacheAppendQ8: grid too large.");
-    append_kernel<<<static_cast<unsigned>(grid), kThreads, 0, as_stream(stream)>>>(a);
+    auto const kernel = kThreads % a.row.d == 0 ? append_kernel<true> : append_kernel<false>;
+    kernel<<<static_cast<unsigned>(grid), kThreads, 0, as_stream(stream)>>>(a);
     return check_launch(what);
 }
 
@@ -304,8 +383,8 @@ int read_back(ann_stream stream, const ann_view* kc, const ann_view* vc, const a
     a.H = q[0].ext[head];
     a.D = q[0].ext[3];
     a.Tout = o[0].ext[tok];
-    a.block = block;
     if (o[0].numel() == 0) return ANN_OK;
+    if (a.Tout * a.D > INT32_MAX) return fail(ANN_ENOTSUP, "kvCacheReadQ8: a head of more than 2^31 values.");
     a.vec = 1;
     for (int k = 0; k < 2; ++k) {
         a.c[k] = tensor_of(q[k], s[k], layout);
@@ -316,13 +395,15 @@ int read_back(ann_stream stream, const ann_view* kc, const ann_view* vc, const a
         a.o_d[k] = o[k].str[3];
         if (!rows4(o[k], sizeof(float)) || !rows4(q[k], 1)) a.vec = 0;
     }
-    a.chunks = ceil_div(a.Tout * (a.vec ? a.D / 4 : a.D), kReadItems);
+    a.row = FastDiv::make(static_cast<uint32_t>(a.vec ? a.D / 4 : a.D));
+    a.block = FastDiv::make(block);
+    a.chunks = ceil_div(a.Tout * a.row.d, kReadItems);
     int64_t const grid = q[0].ext[0] * a.H * 2 * a.chunks;
     if (grid > INT32_MAX) return fail(ANN_ENOTSUP, "kvCacheReadQ8: grid too large.");
-    if (a.vec)
-        read_kernel<true><<<static_cast<unsigned>(grid), kThreads, 0, as_stream(stream)>>>(a);
-    else
-        read_kernel<false><<<static_cast<unsigned>(grid), kThreads, 0, as_stream(stream)>>>(a);
+    bool const step = kThreads % a.row.d == 0;
+    auto const kernel = a.vec ? (step ? read_kernel<true, true> : read_kernel<true, false>)
+                              : (step ? read_kernel<false, true> : read_kernel<false, false>);
+    kernel<<<static_cast<unsigned>(grid), kThreads, 0, as_stream(stream)>>>(a);
     return check_launch(what);
 }
 

@@ -100,23 +100,6 @@ __device__ __forceinline__ void rope_item(RopeArgs const& a, RopeJob const& j, i
     }
 }
 
-// Division of n < 2^31 by an invariant d >= 1 as a multiply and a shift
-// (Granlund and Montgomery, "Division by invariant integers using
-// multiplication", 1994): with l = ceil(log2 d) and m = ceil(2^(31+l) / d),
-// which fits in 32 bits, n / d = (n * m) >> (31 + l) for every n < 2^31.
-struct FastDiv {
-    uint32_t d, m, shift;
-    static FastDiv make(uint32_t d) {
-        uint32_t l = 0;
-        while ((uint64_t{1} << l) < d) ++l;
-        uint64_t const num = uint64_t{1} << (31 + l);
-        return FastDiv{d, static_cast<uint32_t>((num + d - 1) / d), 31 + l};
-    }
-    __device__ __forceinline__ uint32_t div(uint32_t n) const {
-        return static_cast<uint32_t>((static_cast<uint64_t>(n) * m) >> shift);
-    }
-};
-
 // The aligned path when every index fits in 31 bits (the normal case): the
 // flat item index splits into (a0, a1, a2, pair-vector) with three FastDiv
 // steps instead of three 64-bit divisions (which made the kernel
