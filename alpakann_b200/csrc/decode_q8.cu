@@ -291,9 +291,9 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
         unit = off / n;
         t0 = off - unit * n;
     } else {
-        int64_t const all = blockIdx.x / a.splits, per = a.Hkv * a.row_tiles;
+        uint32_t const all = blockIdx.x / a.splits, per = static_cast<uint32_t>(a.Hkv * a.row_tiles);
         b = all / per;
-        unit = static_cast<int>(all - b * per);
+        unit = static_cast<int>(all % per);
     }
   for (;;) {
     int const kvh = unit / static_cast<int>(a.row_tiles);
@@ -718,8 +718,8 @@ __global__ void __launch_bounds__(256) merge_kernel(DecodeQ8Args a, int G, int W
     int const lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int const units = static_cast<int>(a.Hkv * a.row_tiles), wpr = 8 / per_block;
     int const r = blockIdx.y * per_block + warp / wpr, sub = warp % wpr;
-    int64_t const b = blockIdx.x / units;
-    int const u = static_cast<int>(blockIdx.x - b * units);
+    int64_t const b = blockIdx.x / static_cast<uint32_t>(units);
+    int const u = static_cast<int>(blockIdx.x % static_cast<uint32_t>(units));
     int const n = static_cast<int>((keys_of(a, b) + KT - 1) / KT);
     Shares const sh(tiles_before<KT>(a, a.B) * units, G, W);
     int const p0 = tiles_before<KT>(a, b) * units + u * n;

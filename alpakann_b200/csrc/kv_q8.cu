@@ -41,8 +41,10 @@ struct AppendArgs {
     const int32_t* pos;
     const int32_t* counts;  // may be null: every row
     int64_t pos_s, counts_s;
-    int64_t Tn, H, D, cap, block, touched;  // touched: blocks a sequence's rows can reach
-    FastDiv row;                            // by the items of a row: 4 aligned values (vec) or one
+    int64_t Tn, D, cap, block;
+    FastDiv touched, heads;  // blocks a sequence's rows can reach, KV heads
+    FastDiv blocks;          // by a block's tokens
+    FastDiv row;             // by the items of a row: 4 aligned values (vec) or one
     int vec;
 };
 
@@ -92,12 +94,10 @@ __device__ __forceinline__ int nearest64(double x, double s) {
 template <bool STEP>
 __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
     __shared__ unsigned int red[kThreads / 32];
-    int64_t unit = blockIdx.x;
-    int64_t const jb = unit % a.touched;
-    unit /= a.touched;
-    int const kv = static_cast<int>(unit & 1);
-    unit >>= 1;
-    int64_t const h = unit % a.H, b = unit / a.H;
+    uint32_t const bhk = a.touched.div(blockIdx.x), jb = blockIdx.x - bhk * a.touched.d;
+    int const kv = static_cast<int>(bhk & 1u);
+    uint32_t const ub = a.heads.div(bhk >> 1);
+    int64_t const b = ub, h = (bhk >> 1) - ub * a.heads.d;
 
     int64_t const start = a.pos[b * a.pos_s];
     int64_t count = a.Tn;
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
     int64_t const first = max(start, int64_t{0}), end = min(start + count, a.cap);
     if (threadIdx.x == 0 && count > 0 && (start < 0 || start + count > a.cap))
         atomicOr(&g_kv_q8_error, ANN_DEVERR_CACHE_RANGE);
-    int64_t const j = first / a.block + jb;
+    int64_t const j = a.blocks.div(static_cast<uint32_t>(min(first, a.cap))) + jb;
     int64_t const lo = max(first, j * a.block), hi = min(end, (j + 1) * a.block);
     if (lo >= hi) return;
 
@@ -212,8 +212,9 @@ struct ReadArgs {
     int64_t o_b[2], o_h[2], o_t[2], o_d[2];
     const int32_t* lengths;  // may be null: every row
     int64_t len_s;
-    int64_t H, D, Tout, chunks;  // chunks of kReadItems items per (batch, head)
-    FastDiv row, block;          // by the items of a row (4 aligned values, or one), by a block's tokens
+    int64_t D, Tout;
+    FastDiv chunks, heads;  // chunks of kReadItems items per (batch, head), KV heads
+    FastDiv row, block;     // by the items of a row (4 aligned values, or one), by a block's tokens
     int vec;
 };
 
@@ -222,18 +223,16 @@ constexpr int kReadItems = kThreads * kReadEach;
 
 template <bool VEC, bool STEP>
 __global__ void __launch_bounds__(kThreads) read_kernel(ReadArgs a) {
-    int64_t unit = blockIdx.x;
-    int64_t const chunk = unit % a.chunks;
-    unit /= a.chunks;
-    int const kv = static_cast<int>(unit & 1);
-    unit >>= 1;
-    int64_t const h = unit % a.H, b = unit / a.H;
+    uint32_t const bhk = a.chunks.div(blockIdx.x), chunk = blockIdx.x - bhk * a.chunks.d;
+    int const kv = static_cast<int>(bhk & 1u);
+    uint32_t const ub = a.heads.div(bhk >> 1);
+    int64_t const b = ub, h = (bhk >> 1) - ub * a.heads.d;
     CacheTensor const& c = kv ? a.c[1] : a.c[0];
     int8_t const* q = c.q + b * c.q_b + h * c.q_h;
     float const* scale = c.scale + b * c.s_b + h * c.s_h;
     float* out = (kv ? a.out[1] : a.out[0]) + b * (kv ? a.o_b[1] : a.o_b[0]) + h * (kv ? a.o_h[1] : a.o_h[0]);
     int64_t const o_t = kv ? a.o_t[1] : a.o_t[0], o_d = kv ? a.o_d[1] : a.o_d[0];
-    uint32_t const per = a.row.d, base = static_cast<uint32_t>(chunk) * kReadItems + threadIdx.x;
+    uint32_t const per = a.row.d, base = chunk * kReadItems + threadIdx.x;
     uint32_t const t0 = a.row.div(base), c0 = base - t0 * per, all = static_cast<uint32_t>(a.Tout);
     auto place = [&](int u, uint32_t& t, uint32_t& col) {
         t = STEP ? t0 + u * (kThreads / per) : a.row.div(base + u * kThreads);
@@ -333,7 +332,7 @@ int append(ann_stream stream, const ann_view* kn, const ann_view* vn, const ann_
     ANN_TRY(per_sequence(pos_v, "kvCacheAppendQ8 positions", B, a.pos, a.pos_s));
     if (counts_v != nullptr) ANN_TRY(per_sequence(counts_v, "kvCacheAppendQ8 counts", B, a.counts, a.counts_s));
     a.Tn = x[0].ext[1];
-    a.H = x[0].ext[2];
+    int64_t const H = x[0].ext[2];
     a.D = x[0].ext[3];
     a.cap = q[0].ext[tok];
     a.block = block;
@@ -352,8 +351,11 @@ int append(ann_stream stream, const ann_view* kn, const ann_view* vn, const ann_
     }
     a.row = FastDiv::make(static_cast<uint32_t>(a.vec ? a.D / 4 : a.D));
     // Rows start anywhere in a block: at most this many blocks hold some of them.
-    a.touched = std::min(ceil_div(a.cap, block), ceil_div(a.Tn - 1, block) + 1);
-    int64_t const grid = B * a.H * 2 * a.touched;
+    int64_t const touched = std::min(ceil_div(a.cap, block), ceil_div(a.Tn - 1, block) + 1), grid = B * H * 2 * touched;
+    if (a.cap > INT32_MAX) return fail(ANN_ENOTSUP, "kvCacheAppendQ8: more than 2^31 tokens.");
+    a.touched = FastDiv::make(static_cast<uint32_t>(touched));
+    a.heads = FastDiv::make(static_cast<uint32_t>(H));
+    a.blocks = FastDiv::make(block);
     if (grid > INT32_MAX) return fail(ANN_ENOTSUP, "kvCacheAppendQ8: grid too large.");
     auto const kernel = kThreads % a.row.d == 0 ? append_kernel<true> : append_kernel<false>;
     kernel<<<static_cast<unsigned>(grid), kThreads, 0, as_stream(stream)>>>(a);
@@ -380,7 +382,7 @@ int read_back(ann_stream stream, const ann_view* kc, const ann_view* vc, const a
     if (!same_extents(o[0], o[1])) return fail(ANN_EINVAL, "kvCacheReadQ8: K and V output extents differ.");
     ReadArgs a{};
     if (len_v != nullptr) ANN_TRY(per_sequence(len_v, "kvCacheReadQ8 lengths", q[0].ext[0], a.lengths, a.len_s));
-    a.H = q[0].ext[head];
+    int64_t const H = q[0].ext[head];
     a.D = q[0].ext[3];
     a.Tout = o[0].ext[tok];
     if (o[0].numel() == 0) return ANN_OK;
@@ -397,8 +399,9 @@ int read_back(ann_stream stream, const ann_view* kc, const ann_view* vc, const a
     }
     a.row = FastDiv::make(static_cast<uint32_t>(a.vec ? a.D / 4 : a.D));
     a.block = FastDiv::make(block);
-    a.chunks = ceil_div(a.Tout * a.row.d, kReadItems);
-    int64_t const grid = q[0].ext[0] * a.H * 2 * a.chunks;
+    int64_t const chunks = ceil_div(a.Tout * a.row.d, kReadItems), grid = q[0].ext[0] * H * 2 * chunks;
+    a.chunks = FastDiv::make(static_cast<uint32_t>(chunks));
+    a.heads = FastDiv::make(static_cast<uint32_t>(H));
     if (grid > INT32_MAX) return fail(ANN_ENOTSUP, "kvCacheReadQ8: grid too large.");
     bool const step = kThreads % a.row.d == 0;
     auto const kernel = a.vec ? (step ? read_kernel<true, true> : read_kernel<true, false>)
