@@ -25,7 +25,7 @@ namespace {
 __device__ unsigned int g_kv_q8_error;
 
 constexpr int kThreads = 256;
-constexpr int kHeld = 8;  // 16-byte vectors of a thread kept between append's two passes
+constexpr int kHeld = 4;  // 16-byte vectors of a thread kept between append's two passes
 
 struct CacheTensor {
     int8_t* q;
@@ -92,7 +92,7 @@ __device__ __forceinline__ int nearest64(double x, double s) {
 
 // STEP: a row's items divide the block's threads, which then step over rows.
 template <bool STEP>
-__global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(kThreads, 5) append_kernel(AppendArgs a) {
     __shared__ unsigned int red[kThreads / 32];
     uint32_t const bhk = a.touched.div(blockIdx.x), jb = blockIdx.x - bhk * a.touched.d;
     int const kv = static_cast<int>(bhk & 1u);
@@ -117,9 +117,9 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
     float* scale = c.scale + b * c.s_b + h * c.s_h + j * c.s_j;
     int const rows = static_cast<int>(hi - lo), D = static_cast<int>(a.D);
 
-    // The first kHeld items of a thread stay in registers between the two passes (a
-    // block of 64 tokens of 128 values whole), loaded at once; later ones are read
-    // again.
+    // The first kHeld items of a thread stay in registers between the two passes,
+    // loaded at once; later ones are read again, from L2. (More registers for items
+    // mean fewer CTAs an SM: 8 held 29 us, 4 held 26 us at 4 x 2048 tokens.)
     int const per = static_cast<int>(a.row.d), items = rows * per;  // of a row, of the new rows
     int const r0 = static_cast<int>(a.row.div(threadIdx.x)), c0 = static_cast<int>(threadIdx.x) - r0 * per;
     auto place = [&](int u, int& r, int& col) {  // item threadIdx.x + u * kThreads
@@ -133,7 +133,11 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
         }
     };
     int const mine = (items - static_cast<int>(threadIdx.x) + kThreads - 1) / kThreads;  // items of this thread
+    int64_t const x_u = STEP ? kThreads / per * x_t : 0, q_u = STEP ? kThreads / per * c.q_t : 0;
+    float const* const x0 = x + r0 * x_t + 4 * c0;
+    int8_t* const q0 = q + (lo + r0) * c.q_t + 4 * c0;
     auto vector = [&](int u) {
+        if constexpr (STEP) return *reinterpret_cast<float4 const*>(x0 + u * x_u);
         int r, col;
         place(u, r, col);
         return *reinterpret_cast<float4 const*>(x + r * x_t + 4 * col);
@@ -190,7 +194,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
             char4 const n = make_char4(round1(v.x), round1(v.y), round1(v.z), round1(v.w));
             bytes = *reinterpret_cast<uint32_t const*>(&n);
         }
-        *reinterpret_cast<uint32_t*>(q + (lo + r) * c.q_t + 4 * col) = bytes;
+        *reinterpret_cast<uint32_t*>(STEP ? q0 + u * q_u : q + (lo + r) * c.q_t + 4 * col) = bytes;
     };
     if (a.vec) {
 #pragma unroll
@@ -240,31 +244,35 @@ __global__ void __launch_bounds__(kThreads) read_kernel(ReadArgs a) {
     };
     // All loads of a thread at once, the length among them: rows past it are read
     // (they are part of the cache) and not written.
+    int64_t const q_u = STEP ? kThreads / per * c.q_t : 0, o_u = STEP ? kThreads / per * o_t : 0;
+    int8_t const* q0 = q + t0 * c.q_t + (VEC ? 4 * c0 : c0 * c.q_d);
+    float* o0 = out + t0 * o_t + (VEC ? 4 * c0 : c0 * o_d);
     float s[kReadEach];
     char4 n[kReadEach];
 #pragma unroll
     for (int u = 0; u < kReadEach; ++u) {
         uint32_t t, col;
         place(u, t, col);
-        if (t >= all) continue;
-        s[u] = scale[a.block.div(t) * c.s_j];
+        bool const in = t < all;
+        int8_t const* p = STEP ? q0 + u * q_u : q + t * c.q_t + (VEC ? 4 * col : col * c.q_d);
+        s[u] = in ? scale[a.block.div(t) * c.s_j] : 0.0f;
         if constexpr (VEC)
-            n[u] = *reinterpret_cast<char4 const*>(q + t * c.q_t + 4 * col);
+            n[u] = in ? *reinterpret_cast<char4 const*>(p) : make_char4(0, 0, 0, 0);
         else
-            n[u].x = q[t * c.q_t + col * c.q_d];
+            n[u].x = in ? *p : 0;
     }
-    int64_t rows = a.Tout;
-    if (a.lengths != nullptr) rows = min(rows, max(int64_t{0}, static_cast<int64_t>(a.lengths[b * a.len_s])));
+    uint32_t rows = all;
+    if (a.lengths != nullptr) rows = min(rows, static_cast<uint32_t>(max(0, a.lengths[b * a.len_s])));
 #pragma unroll
     for (int u = 0; u < kReadEach; ++u) {
         uint32_t t, col;
         place(u, t, col);
+        float* p = STEP ? o0 + u * o_u : out + t * o_t + (VEC ? 4 * col : col * o_d);
         if (t >= rows) continue;
         if constexpr (VEC)
-            *reinterpret_cast<float4*>(out + t * o_t + 4 * col) =
-                make_float4(n[u].x * s[u], n[u].y * s[u], n[u].z * s[u], n[u].w * s[u]);
+            *reinterpret_cast<float4*>(p) = make_float4(n[u].x * s[u], n[u].y * s[u], n[u].z * s[u], n[u].w * s[u]);
         else
-            out[t * o_t + col * o_d] = n[u].x * s[u];
+            *p = n[u].x * s[u];
     }
 }
 
