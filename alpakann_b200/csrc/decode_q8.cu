@@ -9,6 +9,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdlib>
 #include <map>
 #include <mutex>
@@ -846,10 +847,6 @@ int launch_cluster(ann_stream stream, DecodeQ8Args& a, int64_t units) {
     static std::mutex mu;
     static std::set<int> ready;
     ANN_TRY(prepare(kernel, C::SMEM, true, ready, mu));
-    // two CTAs for every SM, as long as a split keeps two tiles for each of its warps
-    int64_t const most = std::max<int64_t>(1, ceil_div(a.cap, int64_t{2} * C::KT * W));
-    int64_t const want = ceil_div(int64_t{2} * sm_count(), units);
-    a.splits = static_cast<int>(std::min({most, want, int64_t{kMaxCluster}}));
     int64_t const grid = units * a.splits;
     if (grid > INT32_MAX) return fail(ANN_ENOTSUP, "attentionDecodeQ8: grid too large.");
     cudaLaunchConfig_t cfg{};
@@ -906,18 +903,34 @@ int launch_shares(ann_stream stream, DecodeQ8Args& a, int64_t units, int per_sm)
     return rc;
 }
 
+// Which way, and how many splits: the least of these costs, in tiles' times of a
+// warp on a full SM (2.2 us for 8 KB: 12 warps share an SM's part of HBM).
+//  * Clusters of S: rounds of CTAs, each ceil(tiles / 4 S) tiles a warp and about
+//    one tile's time to start and to merge. A tile takes less where the grid
+//    does not fill the GPU, though not in proportion, and no less than 0.45.
+//  * Even shares: their tiles a warp, and about 1.5 tiles' times for the second
+//    launch and for each part of a KV head that a CTA meets.
+// Measured (us, clusters at their best S / shares): 8 x 2048 keys, 32 KV heads 32 /
+// 36; 12 x 4096 keys of 64, 4 heads, four tokens 15 / 21; 31 x 7345 keys of 64, 6
+// heads 41 / 46; 16 x 32768 keys, 8 heads 183 / 173; 1 x 131072 keys, 4 heads 76 / 39.
 template <int D, int MT>
 int launch(ann_stream stream, DecodeQ8Args& a) {
     using C = Q8<D, MT, 4>;
     if (a.Tq > INT32_MAX / 2 / static_cast<int64_t>(a.g)) return fail(ANN_ENOTSUP, "attentionDecodeQ8: more than 2^30 rows.");
     a.row_tiles = ceil_div(a.Tq * a.g, C::ROWS);
-    int64_t const units = a.B * a.Hkv * a.row_tiles;
-    if (units * C::ROWS > INT32_MAX) return fail(ANN_ENOTSUP, "attentionDecodeQ8: grid too large.");
+    int64_t const units = a.B * a.Hkv * a.row_tiles, tiles = ceil_div(a.cap, C::KT);
+    if (units > INT32_MAX) return fail(ANN_ENOTSUP, "attentionDecodeQ8: grid too large.");
     int const per_sm = MT == 1 && D <= 128 ? 3 : 2;
-    // every share's parts are indexed in 32 bits
-    bool const large = units * ceil_div(a.cap, C::KT) > INT32_MAX / 2;
-    bool const small = large || units * ceil_div(a.cap, C::KT) <= int64_t{2} * 4 * per_sm * sm_count();
-    if (std::getenv("TUNE_P") ? std::atoi(std::getenv("TUNE_P")) : small) return launch_cluster<D, MT>(stream, a, units);
+    double const slots = static_cast<double>(sm_count()) * per_sm, all = static_cast<double>(units) * tiles;
+    double best = 1e300;
+    for (int s = 1; s <= kMaxCluster && (s == 1 || (s - 1) * 4 < tiles); ++s) {
+        double const ctas = static_cast<double>(units) * s, full = std::min(1.0, ctas / slots);
+        double const cost = std::ceil(ctas / slots) * (std::ceil(tiles / (4.0 * s)) * std::max(0.45, 0.3 + 0.7 * full) + 1.0);
+        if (cost < best) best = cost, a.splits = s;
+    }
+    // the shares' tiles are counted in 32 bits
+    double const shares = all > INT32_MAX / 2 ? 1e300 : all / (4.0 * slots) + 1.5 * (2.0 + static_cast<double>(units) / slots);
+    if (best <= shares) return launch_cluster<D, MT>(stream, a, units);
     return launch_shares<D, MT>(stream, a, units, per_sm);
 }
 
