@@ -9,8 +9,6 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
-#include <climits>
-#include <cstdlib>
 #include <mutex>
 #include <set>
 
@@ -359,19 +357,25 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
             uint4 const* const rs = ring + slot * (4 * CT * 32);
             if (++slot == C::DEPTH) slot = 0;
             uint4 w[4][CT];
-            uint2 b[4][NT];
+            uint2 b[4][NT];  // all at once, or with four n-tiles a step's at a time
+            auto load_b = [&](int i) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) b[i][nt] = dig[(i * NT + nt) * 32];
+            };
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
 #pragma unroll
                 for (int k = 0; k < CT; ++k) w[i][k] = rs[(i * CT + k) * 32];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) b[i][nt] = dig[(i * NT + nt) * 32];
+                if constexpr (NT <= 2) load_b(i);
             }
             __syncwarp();  // the warp has read the quad; its place takes another
             fetch();
             if ((m & 7u) == 0u) {  // groups of 128 inputs or more: no sum ends within the quad
 #pragma unroll
-                for (int i = 0; i < 4; ++i) multiply(w[i], b[i]);
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (NT > 2) load_b(i);
+                    multiply(w[i], b[i]);
+                }
                 if (m != 0u) {
                     flush(off + 12 * NT, sc);
                     ps += a.s_g;
@@ -382,6 +386,7 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
                     float4 next[CT];
                     bool const ends_here = m >> i & 1u, another = ends_here && m >> (i + 1) != 0u;
                     if (another) scales(ps + a.s_g, next);
+                    if constexpr (NT > 2) load_b(i);
                     multiply(w[i], b[i]);
                     if (!ends_here) continue;
                     flush(off + 4 * NT * i, sc);
@@ -469,7 +474,6 @@ int launch(ann_stream stream, LinearQ4Args& a) {
     // quad; and as many as x's digits need to fit a CTA.
     int64_t const want = ceil_div(int64_t{2} * sm_count(), tiles * row_tiles);
     int64_t splits = std::max<int64_t>(1, std::min(want, quads / kWarps));
-    if (const char* e = std::getenv("TUNE_S")) splits = std::atoi(e);
     int64_t const per_quad = static_cast<int64_t>(C::QUAD);
     splits = std::max(splits, ceil_div((quads + kWarps) * per_quad, static_cast<int64_t>(C::ROOM)));
     splits = std::min<int64_t>(splits, kMaxCluster);
@@ -503,10 +507,11 @@ int launch_vec(ann_stream stream, LinearQ4Args& a, bool vec) {
     return vec ? launch<CT, NT, true>(stream, a) : launch<CT, NT, false>(stream, a);
 }
 
-int launch_rows(ann_stream stream, LinearQ4Args& a, bool vec, int cols) {
-    if (a.M <= 2) return cols == 1 ? launch_vec<1, 1>(stream, a, vec) : launch_vec<2, 1>(stream, a, vec);
-    if (a.M <= 4) return cols == 1 ? launch_vec<1, 2>(stream, a, vec) : launch_vec<2, 2>(stream, a, vec);
-    return cols == 1 ? launch_vec<1, 4>(stream, a, vec) : launch_vec<2, 4>(stream, a, vec);
+template <int CT>
+int launch_rows(ann_stream stream, LinearQ4Args& a, bool vec) {
+    if (a.M <= 2) return launch_vec<CT, 1>(stream, a, vec);
+    if (a.M <= 4) return launch_vec<CT, 2>(stream, a, vec);
+    return launch_vec<CT, 4>(stream, a, vec);
 }
 
 constexpr int kPackThreads = 128;
@@ -602,8 +607,10 @@ int linear_q4(ann_stream stream, const ann_view* x_v, const ann_view* p_v, const
     a.x_vec = a.x_k == 1 && a.x_m % 4 == 0 && aligned(x.data, 16);
     bool const vec = a.w_n == 1 && a.w_r % 4 == 0 && aligned(p.data, 16) && a.s_n == 1 && a.s_g % 4 == 0 &&
                      aligned(s.data, 16) && a.N % 4 == 0;
-    int const cols = std::getenv("TUNE_C") ? std::atoi(std::getenv("TUNE_C")) : a.N * ceil_div(a.M, 16) < 2048 ? 1 : 4;
-    return launch_rows(stream, a, vec, cols);
+    // Few columns: tiles of 32 give twice the CTAs (1024 x 1024, one row: 3.9 us
+    // against 4.2); else 64, whose copies, digits and loops serve twice the weights
+    // (4096 x 65536: 30 us against 34).
+    return a.N < 2048 ? launch_rows<1>(stream, a, vec) : launch_rows<2>(stream, a, vec);
 }
 
 int pack_q4(ann_stream stream, const ann_view* w_v, const ann_view* p_v, const ann_view* s_v, uint32_t group) {
