@@ -48,16 +48,28 @@ struct DecodeQ8Args {
     float scale;
 };
 
-// How the products are formed. q.k in whole numbers: a row of q is rounded to 31
-// bits of its largest value and cut into four 8-bit digits, so that
-// mma.sync.m16n8k32 on int8 multiplies the cache's bytes as they are -- one
-// product holds the high two digits of eight query rows, another the low two --
-// and the sums are exact. p.v in halves: a cached value is exact in fp16, a
-// probability is the sum of two fp16 parts (22 bits), and mma.sync.m16n8k16 adds
-// the exact products in fp32; again one product holds both parts of eight rows,
-// in the same thread. (On this GPU an int8 product of depth 32 and an fp16 one
-// of depth 16 take the same time, 2.1 cycles of an SM: 8 KB of cache cost 64 of
-// them, 0.4 of the time that HBM takes to deliver it.)
+// How the products are formed. In whole numbers: a row of q is rounded to 31 bits
+// of its largest value and cut into four 8-bit digits, so that mma.sync.m16n8k32 on
+// int8 multiplies the cache's bytes as they are, and the sums are exact. With up to
+// four query rows of a KV head (R = 4) one product holds all their digits; with up to
+// eight one holds the high two, another the low two.
+// p.v with R = 4 goes the same way: a probability, relative to a reference that the
+// running maximum passes by at most 2^4, times V's scale, relative to a power of
+// two, is rounded to 2^-25 and cut into digits; the sums over keys stay in int32 for
+// up to 2^16 keys and until the maximum (or V's scale) outgrows its reference. Only
+// then, a few times a call, are they converted: a converted sum per tile would cost
+// more instructions than the tile's products. (8 x 2048 keys, 32 heads: 29.6 us in
+// halves, 24.8 in digits. With eight rows the int32 sums take 128 registers a thread
+// and leave 8 warps an SM: 16 x 32768 keys, 64/8 heads 169 us in halves, 176 in
+// digits.)
+// With more rows, and with heads of 256, p.v runs in halves: a cached value is exact
+// in fp16, a probability is the sum of two fp16 parts (22 bits), and
+// mma.sync.m16n8k16 adds the exact products in fp32, both parts of eight rows in one
+// product, from a fresh accumulator for each tile, so that no sum of more than KT
+// products is left to the tensor core's own rounding.
+// (On this GPU an int8 product of depth 32 and an fp16 one of depth 16 take the same
+// time, 2.1 cycles of an SM: 8 KB of cache cost 64 of them, 0.4 of the time that HBM
+// takes to deliver it; 32 with R = 4.)
 //
 // How the cache reaches the fragments. The order of the summed index and of the
 // output columns of a matrix product is free as long as both operands agree, so
@@ -69,9 +81,8 @@ struct DecodeQ8Args {
 // a warp, 12 warps an SM, where HBM's latency asks for 40 KB an SM. The pieces
 // are placed so that both kinds of reads are free of bank conflicts.
 //
-// Every warp keeps a running maximum and sum per row (base 2) and adds each
-// tile's p.v from a fresh accumulator, so no sum of more than KT products is left
-// to the tensor core's own rounding. Warps meet in shared memory; the CTAs of a
+// Every warp keeps a running maximum and sum per row (base 2). Warps meet in
+// shared memory; the CTAs of a
 // cluster (the key range's splits) send their parts into each other's shared
 // memory, where each CTA sums its share of the output: one cluster barrier, no
 // scratch memory, no atomics, one launch, and a fixed order of sums.
@@ -79,12 +90,15 @@ constexpr int kMaxCluster = 16;
 constexpr int kMaxShares = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <int D, int MT, int W>
+template <int D, int R, int W>
 struct Q8 {
     static constexpr int THREADS = 32 * W;
+    static constexpr bool INTV = R == 4;           // p.v in whole numbers (D <= 128)
+    static constexpr int MT = R == 16 ? 2 : 1;     // groups of eight rows
     static constexpr int KT = D <= 128 ? 32 : 16;  // keys per tile of a warp
-    static constexpr int ROWS = 8 * MT;            // query rows of a CTA
+    static constexpr int ROWS = R;                 // query rows of a CTA
     static constexpr int KS = D / 32;              // k32 steps of q.k
+    static constexpr int QT = R == 4 ? 1 : 2;      // products that hold a row's digits
     static constexpr int NK = KT / 8;              // n8 tiles of keys
     static constexpr int KV = KT / 16;             // k16 steps of p.v, groups of 16 keys
     static constexpr int VW = D / 32;              // words of V per lane and key
@@ -92,13 +106,15 @@ struct Q8 {
     static constexpr bool QREG = MT * KS <= 4;     // q's fragments in registers
     static constexpr int TILE = KT * D;            // bytes of a tile of K or V
     static constexpr int RING = 4 * TILE;          // K, V, K, V of a warp; its output rows at the end
-    static constexpr size_t OFF_Q = size_t{1} * RING * W;                      // uint4 [MT][KS][2][32]
-    static constexpr size_t OFF_R = OFF_Q + size_t{32} * MT * KS * 32;         // float4 [ROWS * D / 4 + kMaxCluster]
+    static constexpr int PER_SM = R <= 8 && D <= 128 ? 3 : 2;  // CTAs, by registers
+    static constexpr size_t OFF_Q = size_t{1} * RING * W;                      // uint4 [MT][KS][QT][32]
+    static constexpr size_t OFF_R = OFF_Q + size_t{16} * MT * KS * QT * 32;    // float4 [ROWS * D / 4 + kMaxCluster]
     static constexpr size_t OFF_ML = OFF_R + sizeof(float) * (ROWS * D + 4 * kMaxCluster);  // float [2][W][ROWS]
     static constexpr size_t OFF_F = OFF_ML + sizeof(float) * 2 * W * ROWS;     // float [ROWS]: score factors
     static constexpr size_t OFF_X = OFF_F + sizeof(float) * ROWS;              // float [kMaxCluster][2][ROWS]: max, sum
     static constexpr size_t SMEM = OFF_X + sizeof(float) * kMaxCluster * 2 * ROWS;
     static_assert(RING >= static_cast<int>(sizeof(float)) * ROWS * D, "a warp's output rows fit its ring");
+    static_assert(!INTV || D <= 128, "int32 sums of whole rows fit the registers");
     // 16-byte piece c of row r of a tile, with the pieces of a 128-byte line
     // permuted: K is read by 8 lanes as two rows x every other piece (or four), V
     // as every other row of 8 x two neighbouring pieces (or halves of them).
@@ -263,9 +279,10 @@ __device__ __forceinline__ int64_t sequence_of(DecodeQ8Args const& a, int p, int
 // SHARES: CTAs take even shares of all keys and leave parts of rows for
 // merge_kernel; else a cluster of a.splits CTAs takes a KV head's keys and merges
 // them itself.
-template <int D, int MT, int W, bool SHARES>
-__global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 : 2)) decode_q8_kernel(DecodeQ8Args a) {
-    using C = Q8<D, MT, W>;
+template <int D, int R, int W, bool SHARES>
+__global__ void __launch_bounds__(32 * W, Q8<D, R, W>::PER_SM) decode_q8_kernel(DecodeQ8Args a) {
+    using C = Q8<D, R, W>;
+    constexpr int MT = C::MT;
     extern __shared__ __align__(128) unsigned char smem[];
     uint4* sq = reinterpret_cast<uint4*>(smem + C::OFF_Q);
     float* sml = reinterpret_cast<float*>(smem + C::OFF_ML);
@@ -408,34 +425,70 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
             // the lane and word of fragment that holds elements d .. d + 3
             int const c = d / 16, at = D == 64 ? c : (c % 8) / 2;
             int const word = 4 * (D == 64 ? 0 : 2 * (c / 8) + c % 2) + (d / 4) % 4, to = (r & 7) * 4 + at;
-            uint2* f = reinterpret_cast<uint2*>(sq + ((r >> 3) * C::KS + word / 2) * 64 + to) + word % 2;
-            f[0] = make_uint2(__byte_perm(hi01, hi23, 0x7632), __byte_perm(hi01, hi23, 0x5410));
-            f[64] = make_uint2(__byte_perm(lo01, lo23, 0x7632), __byte_perm(lo01, lo23, 0x5410));
+            uint2* f = reinterpret_cast<uint2*>(sq + ((r >> 3) * C::KS + word / 2) * (32 * C::QT) + to) + word % 2;
+            uint32_t const d3 = __byte_perm(hi01, hi23, 0x7632), d2 = __byte_perm(hi01, hi23, 0x5410);
+            uint32_t const d1 = __byte_perm(lo01, lo23, 0x7632), d0 = __byte_perm(lo01, lo23, 0x5410);
+            if constexpr (R == 4) {  // rows g and g + 8 of the product: digits 3 and 1 for g < 4, 2 and 0 for g = 4 + row
+                f[0] = make_uint2(d3, d1);
+                f[32] = make_uint2(d2, d0);
+            } else {  // digits 3 and 2 in one product, 1 and 0 in the next
+                f[0] = make_uint2(d3, d2);
+                f[64] = make_uint2(d1, d0);
+            }
         }
     }
     __syncthreads();
-    uint4 qf[C::QREG ? 2 * MT * C::KS : 1];
+    uint4 qf[C::QREG ? C::QT * MT * C::KS : 1];
     if constexpr (C::QREG) {
 #pragma unroll
-        for (int i = 0; i < 2 * MT * C::KS; ++i) qf[i] = sq[i * 32 + lane];
+        for (int i = 0; i < C::QT * MT * C::KS; ++i) qf[i] = sq[i * 32 + lane];
     }
     float fac[MT];
     int seen[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-        fac[m] = sf[8 * m + g];
-        seen[m] = 8 * m + g < rows ? visible(8 * m + g) : 0;
+        int const r = R == 4 ? g & 3 : 8 * m + g;
+        fac[m] = sf[r];
+        seen[m] = r < rows ? visible(r) : 0;
     }
 
-    float m_run[MT], l_run[MT];
-    pair_t o[MT][D / 8];  // columns 2t and 2t + 1 of n-tile n
+    float m_run[MT], l_run[MT];  // INTV: the reference of the row's probabilities, and their sum
+    pair_t o[C::INTV ? 1 : MT][D / 8];  // !INTV: columns 2t and 2t + 1 of n-tile n
+    int acc[D / 8][4];                  // INTV: digits' sums
+    float oh[C::INTV ? D / 8 : 1];      // INTV: fp32 sums of row g % 4, column 2t + g / 4 of n-tile n
+    int ref = 26, since = 0;  // INTV: biased exponent of V's scales' reference, tiles since the last conversion
+    constexpr int STRETCH = D == 64 ? 8 : 16;  // n-tiles of a lane's consecutive elements
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        m_run[m] = neg_inf(0.0f);
-        l_run[m] = 0.0f;
+    for (int m = 0; m < MT; ++m) m_run[m] = neg_inf(0.0f), l_run[m] = 0.0f;
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n) o[m][n] = pair(0.0f, 0.0f);
+    for (int n = 0; n < D / 8; ++n) {
+        if constexpr (C::INTV) {
+            acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0;
+            oh[n] = 0.0f;
+        } else {
+#pragma unroll
+            for (int m = 0; m < MT; ++m) o[m][n] = pair(0.0f, 0.0f);
+        }
     }
+    // INTV: the digits' sums join the fp32 ones, which are scaled by `by` for the
+    // rows' new reference; V's scales go over to the exponent `to` from here on.
+    auto convert = [&](float by, int to) {
+        if constexpr (C::INTV) {
+            float const unit = pow2_biased(ref - 25);  // 2^(ref - 127) 2^-25
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) {
+                float const x0 = fmaf(static_cast<float>(acc[n][0]), 65536.0f, static_cast<float>(acc[n][2]));
+                float const x1 = fmaf(static_cast<float>(acc[n][1]), 65536.0f, static_cast<float>(acc[n][3]));
+                // lanes g < 4 hold digits 3 and 1 and keep column 2t, the others 2 and 0 and column 2t + 1
+                float const mine = g < 4 ? x0 : x1, theirs = __shfl_xor_sync(0xffffffffu, g < 4 ? x1 : x0, 16);
+                float const v = g < 4 ? fmaf(mine, 256.0f, theirs) : fmaf(theirs, 256.0f, mine);
+                oh[n] = fmaf(v, unit, oh[n]) * by;
+                acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0;
+            }
+            ref = max(ref, to);
+            since = 0;
+        }
+    };
 
     for (int stage = 0; tile < t1_seen; tile += W, stage ^= 1) {
         unsigned char const* const tk = ring + stage * 2 * C::TILE;
@@ -457,26 +510,33 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
                 uint32_t const b0 = kr[2 * st], b1 = kr[2 * st + 1];
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
-                    int const at = 2 * (m * C::KS + st);
+                    int const at = C::QT * (m * C::KS + st);
                     uint4 const qh = C::QREG ? qf[at] : sq[at * 32 + lane];
-                    uint4 const ql = C::QREG ? qf[at + 1] : sq[(at + 1) * 32 + lane];
+                    uint4 const ql = C::QREG ? qf[at + C::QT - 1] : sq[(at + C::QT - 1) * 32 + lane];
                     if (st == 0) {
                         mma_s8_first(hi[m], qh, b0, b1);
-                        mma_s8_first(lo[m], ql, b0, b1);
+                        if constexpr (R > 4) mma_s8_first(lo[m], ql, b0, b1);
                     } else {
                         mma_s8(hi[m], qh, b0, b1);
-                        mma_s8(lo[m], ql, b0, b1);
+                        if constexpr (R > 4) mma_s8(lo[m], ql, b0, b1);
                     }
                 }
             }
-            // digits of sums below 2^22 each: two of them fit 32 bits
+            // digits' sums are below 2^22 each
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
                 float const f = fac[m] * ksc[j / 2];
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    s[m][j][e] = fmaf(static_cast<float>(hi[m][e] * 256 + hi[m][e + 2]), 65536.0f,
-                                      static_cast<float>(lo[m][e] * 256 + lo[m][e + 2])) * f;
+                for (int e = 0; e < 2; ++e) {
+                    if constexpr (R == 4) {
+                        float const x = fmaf(static_cast<float>(hi[m][e]), 65536.0f, static_cast<float>(hi[m][e + 2]));
+                        float const y = __shfl_xor_sync(0xffffffffu, x, 16);
+                        s[m][j][e] = (g < 4 ? fmaf(x, 256.0f, y) : fmaf(y, 256.0f, x)) * f;
+                    } else {
+                        s[m][j][e] = fmaf(static_cast<float>(hi[m][e] * 256 + hi[m][e + 2]), 65536.0f,
+                                          static_cast<float>(lo[m][e] * 256 + lo[m][e + 2])) * f;
+                    }
+                }
             }
         }
         __syncwarp();  // the warp has read K; its place takes the tile after the next
@@ -491,13 +551,63 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
                     for (int e = 0; e < 2; ++e)
                         if (tile * C::KT + 8 * j + 2 * t + e >= seen[m]) s[m][j][e] = neg_inf(0.0f);
         }
-        // V's scales relative to a power of two, so that p * scale fits fp16
-        float vtop = 0.0f;
+        unsigned vtop = 0, vbad = 0;  // the largest finite |scale| of V's groups and the largest, on the bit patterns
 #pragma unroll
-        for (int i = 0; i < C::KV; ++i) vtop = fmaxf(vtop, fabsf(vsc[i]));
-        int const ve = min(max(static_cast<int>(__float_as_uint(vtop) >> 23), 15), 253);
+        for (int i = 0; i < C::KV; ++i) {
+            unsigned const v = __float_as_uint(vsc[i]) & 0x7fffffffu;
+            vbad = max(vbad, v);
+            vtop = max(vtop, v < 0x7f800000u ? v : 0u);
+        }
+        uint32_t pa[MT][C::KV][4];   // !INTV: k16 steps' fragments
+        uint32_t pd[4];              // INTV: the k32 step's
+        if constexpr (C::INTV) {
+            float top = neg_inf(0.0f);
+#pragma unroll
+            for (int j = 0; j < C::NK; ++j) top = fmaxf(top, fmaxf(s[0][j][0], s[0][j][1]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            int const ve = min(static_cast<int>(vtop >> 23), 253);
+            bool const grown = top > m_run[0] + 4.0f;  // -infinity: the first key seen
+            if (__any_sync(0xffffffffu, grown) || ve > ref || since == 2048) {
+                float const by = grown ? exp2_neg(m_run[0] - top) : 1.0f;  // nothing before the first key: 0
+                convert(by, max(ve, 26));
+                l_run[0] *= by;
+                if (grown) m_run[0] = top;
+            }
+            ++since;
+            if (vbad >= 0x7f800000u) {  // NaN or infinity makes NaN of the rows that see its keys
+#pragma unroll
+                for (int j = 0; j < C::NK; ++j)
+                    if (fmaxf(s[0][j][0], s[0][j][1]) > neg_inf(0.0f)) l_run[0] += vsc[j / 2] * 0.0f;
+            }
+            float const base = m_run[0] == neg_inf(0.0f) ? 0.0f : m_run[0], vdown = pow2_biased(254 - ref) * 33554432.0f;
+            uint32_t n[C::NK][2];  // p in whole numbers as signed base-256 digits; p * scale < 2^5, below 2^30
+#pragma unroll
+            for (int j = 0; j < C::NK; ++j) {
+                float const w = vsc[j / 2] * vdown;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float const p = exp2_neg(s[0][j][e] - base);
+                    l_run[0] += p;
+                    n[j][e] = (static_cast<uint32_t>(__float2int_rn(p * w)) + 0x00808080u) ^ 0x00808080u;
+                }
+            }
+            // a lane's four keys of each group of 16 are four bytes of a fragment
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                uint32_t const* const k0 = n[2 * i];
+                uint32_t const* const k1 = n[2 * i + 1];
+                uint32_t const lo01 = __byte_perm(k0[0], k0[1], 0x5140), hi01 = __byte_perm(k0[0], k0[1], 0x7362);
+                uint32_t const lo23 = __byte_perm(k1[0], k1[1], 0x5140), hi23 = __byte_perm(k1[0], k1[1], 0x7362);
+                uint32_t const pick = g < 4 ? 0x7632 : 0x5410;  // as q's rows: digits 3 and 1, or 2 and 0
+                pd[2 * i] = __byte_perm(hi01, hi23, pick);
+                pd[2 * i + 1] = __byte_perm(lo01, lo23, pick);
+            }
+        }
+        // !INTV: V's scales relative to a power of two, so that p * scale fits fp16
+        int const ve = min(max(static_cast<int>(vtop >> 23), 15), 253);
         float const vdown = pow2_biased(254 - ve), back = pow2_biased(ve - 13);
-        uint32_t pa[MT][C::KV][4];
+        if constexpr (!C::INTV) {
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             float top = neg_inf(0.0f);
@@ -526,6 +636,7 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
                 }
             }
         }
+        }
         if (tile + W < t1_seen) scales(tile + W);
         copies_landed<3>();
         uint32_t vr[C::KV][4][C::VW];
@@ -550,6 +661,25 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
         if (tile + 2 * W < t1_seen) fetch(ring_u + (stage * 2 + 1) * C::TILE, vb, a.v_t, tile + 2 * W);
         copies_close();
         // o += p V, one word of V (four columns of lanes) at a time
+        if constexpr (C::INTV) {
+            // four keys' words to four columns' bytes
+#pragma unroll
+            for (int w = 0; w < C::VW; ++w) {
+                uint32_t b[2][4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t const x01 = __byte_perm(vr[i][0][w], vr[i][1][w], 0x5140), y01 = __byte_perm(vr[i][0][w], vr[i][1][w], 0x7362);
+                    uint32_t const x23 = __byte_perm(vr[i][2][w], vr[i][3][w], 0x5140), y23 = __byte_perm(vr[i][2][w], vr[i][3][w], 0x7362);
+                    b[i][0] = __byte_perm(x01, x23, 0x5410);
+                    b[i][1] = __byte_perm(x01, x23, 0x7632);
+                    b[i][2] = __byte_perm(y01, y23, 0x5410);
+                    b[i][3] = __byte_perm(y01, y23, 0x7632);
+                }
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+                    mma_s8(acc[4 * w + n], make_uint4(pd[0], pd[1], pd[2], pd[3]), b[0][n], b[1][n]);
+            }
+        } else {
 #pragma unroll
         for (int w = 0; w < C::VW; ++w) {
             float c[MT][4][4];
@@ -579,30 +709,39 @@ __global__ void __launch_bounds__(32 * W, W > 4 ? 1 : (MT == 1 && D <= 128 ? 3 :
                     o[m][4 * w + n] = fma2(add2(pair(c[m][n][0], c[m][n][1]), pair(c[m][n][2], c[m][n][3])),
                                            pair(back, back), o[m][4 * w + n]);
         }
+        }
     }
 
-    // Warps to CTA: every warp's rows in its ring, maxima and sums beside.
+    // Warps to CTA: every warp's rows, maxima and sums. Columns 2t and 2t + 1 of
+    // n-tile n are elements 32 t + n and 32 t + 16 + n of a 128-element stretch (D =
+    // 64: 16 t + n and 16 t + 8 + n).
     copies_landed<0>();
+    if constexpr (C::INTV) {
+        convert(1.0f, ref);
+        float* const p = reinterpret_cast<float*>(ring) + (g & 3) * D + 2 * STRETCH * t + (g >> 2) * STRETCH;
+#pragma unroll
+        for (int n = 0; n < D / 8; n += 4)
+            *reinterpret_cast<float4*>(p + n) = make_float4(oh[n], oh[n + 1], oh[n + 2], oh[n + 3]);
+    }
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         float l = l_run[m];
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (t == 0) {
+        if (t == 0 && (R > 4 || g < 4)) {
             sml[warp * C::ROWS + 8 * m + g] = m_run[m];
             sml[(W + warp) * C::ROWS + 8 * m + g] = l;
         }
-        // columns 2t and 2t + 1 of n-tile n are elements 32 t + n and 32 t + 16 + n of a
-        // 128-element stretch (D = 64: 16 t + n and 16 t + 8 + n)
-        float* row = reinterpret_cast<float*>(ring) + (8 * m + g) * D;
-        constexpr int STRETCH = D == 64 ? 8 : 16;
+        if constexpr (!C::INTV) {
+            float* row = reinterpret_cast<float*>(ring) + (8 * m + g) * D;
 #pragma unroll
-        for (int n = 0; n < D / 8; n += 4) {
-            float* p = row + (n / STRETCH) * 128 + 2 * STRETCH * t + n % STRETCH;
-            float2 const v0 = unpair(o[m][n]), v1 = unpair(o[m][n + 1]), v2 = unpair(o[m][n + 2]),
-                         v3 = unpair(o[m][n + 3]);
-            *reinterpret_cast<float4*>(p) = make_float4(v0.x, v1.x, v2.x, v3.x);
-            *reinterpret_cast<float4*>(p + STRETCH) = make_float4(v0.y, v1.y, v2.y, v3.y);
+            for (int n = 0; n < D / 8; n += 4) {
+                float* p = row + (n / STRETCH) * 128 + 2 * STRETCH * t + n % STRETCH;
+                float2 const v0 = unpair(o[m][n]), v1 = unpair(o[m][n + 1]), v2 = unpair(o[m][n + 2]),
+                             v3 = unpair(o[m][n + 3]);
+                *reinterpret_cast<float4*>(p) = make_float4(v0.x, v1.x, v2.x, v3.x);
+                *reinterpret_cast<float4*>(p + STRETCH) = make_float4(v0.y, v1.y, v2.y, v3.y);
+            }
         }
     }
     __syncthreads();
@@ -839,11 +978,11 @@ int prepare(K kernel, size_t smem, bool wide_cluster, std::set<int>& ready, std:
 }
 
 // One launch, a cluster of CTAs per KV head: for calls of little work.
-template <int D, int MT>
+template <int D, int R>
 int launch_cluster(ann_stream stream, DecodeQ8Args& a, int64_t units) {
     constexpr int W = 4;
-    using C = Q8<D, MT, W>;
-    auto const kernel = decode_q8_kernel<D, MT, W, false>;
+    using C = Q8<D, R, W>;
+    auto const kernel = decode_q8_kernel<D, R, W, false>;
     static std::mutex mu;
     static std::set<int> ready;
     ANN_TRY(prepare(kernel, C::SMEM, true, ready, mu));
@@ -868,15 +1007,15 @@ int launch_cluster(ann_stream stream, DecodeQ8Args& a, int64_t units) {
 
 // Even shares of all keys for as many CTAs as fit the GPU, then the merge of the
 // rows that several CTAs share.
-template <int D, int MT>
-int launch_shares(ann_stream stream, DecodeQ8Args& a, int64_t units, int per_sm) {
+template <int D, int R>
+int launch_shares(ann_stream stream, DecodeQ8Args& a, int64_t units) {
     constexpr int W = 4;
-    using C = Q8<D, MT, W>;
-    auto const kernel = decode_q8_kernel<D, MT, W, true>;
+    using C = Q8<D, R, W>;
+    auto const kernel = decode_q8_kernel<D, R, W, true>;
     static std::mutex mu;
     static std::set<int> ready;
     ANN_TRY(prepare(kernel, C::SMEM, false, ready, mu));
-    int64_t const G = std::min<int64_t>(kMaxShares, int64_t{sm_count()} * per_sm);
+    int64_t const G = std::min<int64_t>(kMaxShares, int64_t{sm_count()} * C::PER_SM);
     void* parts = nullptr;
     ANN_TRY(scratch_alloc(&parts, sizeof(float) * 2 * G * (C::ROWS * D + 2 * C::ROWS), as_stream(stream)));
     a.parts = static_cast<float*>(parts);
@@ -913,15 +1052,14 @@ int launch_shares(ann_stream stream, DecodeQ8Args& a, int64_t units, int per_sm)
 // Measured (us, clusters at their best S / shares): 8 x 2048 keys, 32 KV heads 32 /
 // 36; 12 x 4096 keys of 64, 4 heads, four tokens 15 / 21; 31 x 7345 keys of 64, 6
 // heads 41 / 46; 16 x 32768 keys, 8 heads 183 / 173; 1 x 131072 keys, 4 heads 76 / 39.
-template <int D, int MT>
+template <int D, int R>
 int launch(ann_stream stream, DecodeQ8Args& a) {
-    using C = Q8<D, MT, 4>;
+    using C = Q8<D, R, 4>;
     if (a.Tq > INT32_MAX / 2 / static_cast<int64_t>(a.g)) return fail(ANN_ENOTSUP, "attentionDecodeQ8: more than 2^30 rows.");
     a.row_tiles = ceil_div(a.Tq * a.g, C::ROWS);
     int64_t const units = a.B * a.Hkv * a.row_tiles, tiles = ceil_div(a.cap, C::KT);
     if (units > INT32_MAX) return fail(ANN_ENOTSUP, "attentionDecodeQ8: grid too large.");
-    int const per_sm = MT == 1 && D <= 128 ? 3 : 2;
-    double const slots = static_cast<double>(sm_count()) * per_sm, all = static_cast<double>(units) * tiles;
+    double const slots = static_cast<double>(sm_count()) * C::PER_SM, all = static_cast<double>(units) * tiles;
     double best = 1e300;
     for (int s = 1; s <= kMaxCluster && (s == 1 || (s - 1) * 4 < tiles); ++s) {
         double const ctas = static_cast<double>(units) * s, full = std::min(1.0, ctas / slots);
@@ -930,13 +1068,15 @@ int launch(ann_stream stream, DecodeQ8Args& a) {
     }
     // the shares' tiles are counted in 32 bits
     double const shares = all > INT32_MAX / 2 ? 1e300 : all / (4.0 * slots) + 1.5 * (2.0 + static_cast<double>(units) / slots);
-    if (best <= shares) return launch_cluster<D, MT>(stream, a, units);
-    return launch_shares<D, MT>(stream, a, units, per_sm);
+    if (best <= shares) return launch_cluster<D, R>(stream, a, units);
+    return launch_shares<D, R>(stream, a, units);
 }
 
 template <int D>
 int launch_rows(ann_stream stream, DecodeQ8Args& a) {
-    return a.Tq * a.g <= 8 ? launch<D, 1>(stream, a) : launch<D, 2>(stream, a);
+    if constexpr (D <= 128)
+        if (a.Tq * a.g <= 4) return launch<D, 4>(stream, a);
+    return a.Tq * a.g <= 8 ? launch<D, 8>(stream, a) : launch<D, 16>(stream, a);
 }
 
 int decode_q8(ann_stream stream, const ann_view* q_v, const ann_view* k_v, const ann_view* v_v, const ann_view* ks_v,
