@@ -10,7 +10,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 #include <map>
 #include <mutex>
 #include <set>
@@ -849,14 +848,15 @@ __global__ void __launch_bounds__(32 * W, Q8<D, R, W>::PER_SM) decode_q8_kernel(
   }
 }
 
-// The parts that the even shares left. A block takes `per_block` (1 or 8) rows of
-// a KV head's row tile; the 8 / per_block warps of a row share its parts.
+// The parts that the even shares left. A block takes `per_block` (1, 4 or 8) rows of
+// a KV head's row tile; the kMergeWarps / per_block warps of a row share its parts.
+constexpr int kMergeWarps = 16;
 template <int D, int ROWS, int KT>
-__global__ void __launch_bounds__(256) merge_kernel(DecodeQ8Args a, int G, int W, int per_block) {
+__global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(DecodeQ8Args a, int G, int W, int per_block) {
     constexpr int LV = (D + 127) / 128;  // float4 of a row per lane
-    __shared__ float4 sv[8][LV * 32];
+    __shared__ float4 sv[kMergeWarps][LV * 32];
     int const lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int const units = static_cast<int>(a.Hkv * a.row_tiles), wpr = 8 / per_block;
+    int const units = static_cast<int>(a.Hkv * a.row_tiles), wpr = kMergeWarps / per_block;
     int const r = blockIdx.y * per_block + warp / wpr, sub = warp % wpr;
     int64_t const b = blockIdx.x / static_cast<uint32_t>(units);
     int const u = static_cast<int>(blockIdx.x % static_cast<uint32_t>(units));
@@ -864,12 +864,14 @@ __global__ void __launch_bounds__(256) merge_kernel(DecodeQ8Args a, int G, int W
     Shares const sh(tiles_before<KT>(a, a.B) * units, G, W);
     int const p0 = tiles_before<KT>(a, b) * units + u * n;
     int const c0 = n > 0 ? sh.owner(p0) : 0, c1 = n > 0 ? sh.owner(p0 + n - 1) : 0;
+    // The shares are done and visible. Every block waits for that, those without work
+    // too: this grid's end has to mean that the shares have ended.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (n > 0 && c0 == c1) return;  // a whole unit: written by its CTA
     int const rt = static_cast<int>(a.row_tiles), kvh = u / rt;
     uint32_t const row = static_cast<uint32_t>((u - kvh * rt) * ROWS + r);
     int64_t const hq = static_cast<int64_t>(kvh) * a.g + row % a.g;
     bool const given = row < a.Tq * a.g && hq < a.Hq;
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // the shares are done and visible
     int const parts = n > 0 ? c1 - c0 + 1 : 0;          // no keys: nobody's share, a row of zeros
     float const* stats = a.parts + 2 * G * (ROWS * D);
     // the first CTA may have come from the unit before, the others start with this one
@@ -887,17 +889,28 @@ __global__ void __launch_bounds__(256) merge_kernel(DecodeQ8Args a, int G, int W
             l = fmaf(weight(ps[0]), ps[ROWS], l);
         }
         l = warp_sum(l);
-#pragma unroll 4
-        for (int k = sub; k < parts; k += wpr) {
-            int64_t const sl = slot(k);
-            float const w = weight(stats[sl * 2 * ROWS + r]);
-            float4 const* po = reinterpret_cast<float4 const*>(a.parts) + (sl * ROWS + r) * (D / 4);
+        constexpr int AT_ONCE = 4;  // parts whose loads go out together
+        for (int k0 = sub; k0 < parts; k0 += AT_ONCE * wpr) {
+            float m[AT_ONCE];
+            float4 y[AT_ONCE][LV];
 #pragma unroll
-            for (int i = 0; i < LV; ++i) {
-                if (32 * i + lane >= D / 4) continue;
-                float4 const y = po[32 * i + lane];
-                v[i].x = fmaf(w, y.x, v[i].x), v[i].y = fmaf(w, y.y, v[i].y);
-                v[i].z = fmaf(w, y.z, v[i].z), v[i].w = fmaf(w, y.w, v[i].w);
+            for (int u = 0; u < AT_ONCE; ++u) {
+                int const k = min(k0 + u * wpr, parts - 1);
+                int64_t const sl = slot(k);
+                m[u] = k0 + u * wpr < parts ? stats[sl * 2 * ROWS + r] : neg_inf(0.0f);
+                float4 const* po = reinterpret_cast<float4 const*>(a.parts) + (sl * ROWS + r) * (D / 4);
+#pragma unroll
+                for (int i = 0; i < LV; ++i) y[u][i] = po[min(32 * i + lane, D / 4 - 1)];
+            }
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                if (k0 + u * wpr >= parts) break;
+                float const w = weight(m[u]);
+#pragma unroll
+                for (int i = 0; i < LV; ++i) {
+                    v[i].x = fmaf(w, y[u][i].x, v[i].x), v[i].y = fmaf(w, y[u][i].y, v[i].y);
+                    v[i].z = fmaf(w, y[u][i].z, v[i].z), v[i].w = fmaf(w, y[u][i].w, v[i].w);
+                }
             }
         }
     }
@@ -1027,9 +1040,9 @@ int launch_shares(ann_stream stream, DecodeQ8Args& a, int64_t units) {
         attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its launch overlaps the shares' end
         attr.val.programmaticStreamSerializationAllowed = 1;
         // few units: many parts each, so all warps of a block to one row
-        int const rows = static_cast<int>(std::min<int64_t>(C::ROWS, a.Tq * a.g)), per_block = units < G / 8 ? 1 : 8;
+        int const rows = static_cast<int>(std::min<int64_t>(C::ROWS, a.Tq * a.g)), per_block = units < G / 8 ? 1 : std::min(8, C::ROWS);
         cfg.gridDim = dim3(static_cast<unsigned>(units), static_cast<unsigned>(ceil_div(rows, per_block)));
-        cfg.blockDim = dim3(256);
+        cfg.blockDim = dim3(32 * kMergeWarps);
         cfg.stream = as_stream(stream);
         cfg.attrs = &attr;
         cfg.numAttrs = 1;

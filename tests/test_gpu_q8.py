@@ -251,6 +251,82 @@ def test_attention_long_cache_and_far_offsets(nn):
     assert torch.equal(view, v2) and torch.equal(s1, s2)
 
 
+@pytest.mark.parametrize("D,g_,Tq", [(64, 1, 1), (64, 8, 1), (128, 4, 1), (128, 3, 2), (128, 5, 3), (256, 2, 1),
+                                     (256, 4, 5)])
+@pytest.mark.parametrize("block", [16, 128])
+def test_attention_few_long_sequences(nn, D, g_, Tq, block):
+    """Few KV heads over long caches: shares of keys that cut sequences anywhere, empty and
+    single-key sequences between them, and parts merged."""
+    run_attend(nn, 4, Tq, g_, 2, D, 20011, block, [20011, 0, 1, 7777])
+
+
+@pytest.mark.parametrize("g_", [4, 8])
+def test_attention_many_ragged_sequences(nn, g_):
+    """More sequences than lanes, most of them short, in caches of 20000 tokens."""
+    g = np.random.default_rng(g_)
+    lengths = g.integers(0, 300, 130)
+    lengths[[0, 3, 31, 32, 64, 129]] = [0, 20000, 0, 4096, 12001, 0]
+    run_attend(nn, 130, 1, g_, 1, 64, 20000, 64, lengths)
+
+
+def test_attention_shares_replayed_and_side_by_side(nn):
+    """Calls whose parts are merged: captured with their scratch and replayed with new lengths, two graphs at once."""
+    args, out = run_attend(nn, 2, 1, 8, 1, 128, 30000, 64, [30000, 12345])
+    streams, graphs, outs = [torch.cuda.Stream() for _ in range(2)], [], [torch.empty_like(out) for _ in range(2)]
+    torch.cuda.synchronize()
+    for st, o in zip(streams, outs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            nn.attentionDecodeQ8(None, None, *args[:5], o, *args[6:])
+            nn.attentionDecodeQ8(None, None, *args[:5], o, *args[6:])
+        graphs.append(graph)
+    for n in ([30000, 12345], [1, 29999], [0, 0], [16384, 64]):
+        args[7].copy_(torch.tensor(n, dtype=torch.int32))
+        want = torch.empty_like(out)
+        nn.attentionDecodeQ8(None, None, *args[:5], want, *args[6:])
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for st, graph in zip(streams, graphs):
+                with torch.cuda.stream(st):
+                    graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in outs)
+
+
+def test_attention_scales_of_every_size_and_sign(nn):
+    """V's and K's scales over 2^40 and of both signs: sums whose reference moves along the sequence."""
+    g = np.random.default_rng(12)
+    for g_, T in ((2, 2000), (8, 2000), (4, 40000)):
+        B, Hkv, D, block = 1, 2, 128, 16
+        kc, ks = make_cache(g, B, Hkv, T, D, block)
+        vc, vs = make_cache(g, B, Hkv, T, D, block)
+        vs *= (2.0 ** g.integers(-20, 20, vs.shape)).astype(np.float32) * g.choice([-1, 1], vs.shape)
+        vs[0, 0, :3], vs[0, 1, 5] = 0, np.float32(1e-42)
+        ks *= g.choice([-1, 1], ks.shape)
+        q = g.standard_normal((B, 1, Hkv * g_, D)).astype(np.float32)
+        out = torch.empty(q.shape, device="cuda")
+        nn.attentionDecodeQ8(None, None, dev(q), dev(kc), dev(vc), dev(ks), dev(vs), out, block, None, 0.05, g_)
+        want, tol = ref.attend(q, kc, vc, ks, vs, None, block, 0.05, g_)
+        ref.assert_within(out.cpu().numpy(), want, tol, f"scales {g_} {T}")
+
+
+def test_attention_growing_scores(nn):
+    """Keys in rising and in falling order of score: the running maximum moves at every tile, or never."""
+    D, T, block = 128, 3000, 64
+    g = np.random.default_rng(3)
+    q = np.ones((1, 1, 4, D), np.float32)
+    for order in (1, -1):
+        level = np.linspace(-127, 127, T)[::order]
+        kc = np.clip(np.rint(level[:, None] + g.uniform(-1, 1, (T, D))), -127, 127).astype(np.int8)[None, None]
+        ks = np.full((1, 1, -(-T // block)), 0.01, np.float32)
+        vc, vs = make_cache(g, 1, 1, T, D, block)
+        for scale in (0.01, 0.3):
+            out = torch.empty(q.shape, device="cuda")
+            nn.attentionDecodeQ8(None, None, dev(q), dev(kc), dev(vc), dev(ks), dev(vs), out, block, None, scale, 4)
+            want, tol = ref.attend(q, kc, vc, ks, vs, None, block, scale, 4)
+            ref.assert_within(out.cpu().numpy(), want, tol, f"order {order} scale {scale}")
+
+
 def test_attention_ignores_what_lies_behind_the_last_key(nn):
     """Stale integers and NaN / infinite scales past the length change nothing."""
     args, out = run_attend(nn, 2, 1, 4, 2, 128, 200, 16, [100, 33])
