@@ -77,6 +77,13 @@ static int take_all(PyObject* const* args, int n, const signed char* types, ann_
     return 0;
 }
 
+/* An integer argument; OverflowError outside [low, high]. */
+static long long in_range(PyObject* o, long long low, long long high) {
+    long long const v = PyLong_AsLongLong(o);
+    if (!PyErr_Occurred() && (v < low || v > high)) PyErr_SetString(PyExc_OverflowError, "integer argument out of range");
+    return v;
+}
+
 #define BEGIN(count, ...)                                                              \
     static const signed char types[] = {__VA_ARGS__};                                  \
     enum { N = sizeof types };                                                         \
@@ -93,8 +100,8 @@ static int take_all(PyObject* const* args, int n, const signed char* types, ann_
     if (rc == -2) return NULL;                                                         \
     if (rc == MISMATCH) return PyLong_FromLong(MISMATCH);                              \
     PyObject* const* const s = args + 1 + N
-#define INT(i) ((int32_t)PyLong_AsLong(s[i]))
-#define UINT(i) ((uint32_t)PyLong_AsUnsignedLong(s[i]))
+#define INT(i) ((int32_t)in_range(s[i], INT32_MIN, INT32_MAX))
+#define UINT(i) ((uint32_t)in_range(s[i], 0, UINT32_MAX))
 #define END(call)                                                                      \
     if (PyErr_Occurred()) return NULL;                                                 \
     Py_BEGIN_ALLOW_THREADS;                                                            \

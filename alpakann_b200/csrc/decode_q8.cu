@@ -557,6 +557,16 @@ __global__ void __launch_bounds__(32 * W, Q8<D, R, W>::PER_SM) decode_q8_kernel(
             vbad = max(vbad, v);
             vtop = max(vtop, v < 0x7f800000u ? v : 0u);
         }
+        if (vbad >= 0x7f800000u) {  // NaN or infinity makes NaN of the rows that see its keys, and only of them
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int j = 0; j < C::NK; ++j)
+                    if (fmaxf(s[m][j][0], s[m][j][1]) > neg_inf(0.0f)) l_run[m] += vsc[j / 2] * 0.0f;
+#pragma unroll
+            for (int i = 0; i < C::KV; ++i)
+                if ((__float_as_uint(vsc[i]) & 0x7fffffffu) >= 0x7f800000u) vsc[i] = 0.0f;
+        }
         uint32_t pa[MT][C::KV][4];   // !INTV: k16 steps' fragments
         uint32_t pd[4];              // INTV: the k32 step's
         if constexpr (C::INTV) {
@@ -574,11 +584,6 @@ __global__ void __launch_bounds__(32 * W, Q8<D, R, W>::PER_SM) decode_q8_kernel(
                 if (grown) m_run[0] = top;
             }
             ++since;
-            if (vbad >= 0x7f800000u) {  // NaN or infinity makes NaN of the rows that see its keys
-#pragma unroll
-                for (int j = 0; j < C::NK; ++j)
-                    if (fmaxf(s[0][j][0], s[0][j][1]) > neg_inf(0.0f)) l_run[0] += vsc[j / 2] * 0.0f;
-            }
             float const base = m_run[0] == neg_inf(0.0f) ? 0.0f : m_run[0], vdown = pow2_biased(254 - ref) * 33554432.0f;
             uint32_t n[C::NK][2];  // p in whole numbers as signed base-256 digits; p * scale < 2^5, below 2^30
 #pragma unroll
@@ -1068,7 +1073,7 @@ int launch_shares(ann_stream stream, DecodeQ8Args& a, int64_t units) {
 template <int D, int R>
 int launch(ann_stream stream, DecodeQ8Args& a) {
     using C = Q8<D, R, 4>;
-    if (a.Tq > INT32_MAX / 2 / static_cast<int64_t>(a.g)) return fail(ANN_ENOTSUP, "attentionDecodeQ8: more than 2^30 rows.");
+    if (a.Tq > INT32_MAX / 2 / int64_t{a.g}) return fail(ANN_ENOTSUP, "attentionDecodeQ8: more than 2^30 rows.");
     a.row_tiles = ceil_div(a.Tq * a.g, C::ROWS);
     int64_t const units = a.B * a.Hkv * a.row_tiles, tiles = ceil_div(a.cap, C::KT);
     if (units > INT32_MAX) return fail(ANN_ENOTSUP, "attentionDecodeQ8: grid too large.");
@@ -1156,7 +1161,8 @@ int decode_q8(ann_stream stream, const ann_view* q_v, const ann_view* k_v, const
     a.B = B;
     a.Tq = q.ext[1];
     a.Hq = Hq;
-    a.Hkv = ceil_div(Hq, static_cast<int64_t>(g));  // KV heads that queries read
+    g = static_cast<uint32_t>(std::min<int64_t>(g, Hq));  // a larger group holds no more queries
+    a.Hkv = ceil_div(Hq, int64_t{g});  // KV heads that queries read
     a.cap = k.ext[tok];
     a.g = g;
     a.block_shift = __builtin_ctz(block);

@@ -346,7 +346,7 @@ int append(ann_stream stream, const ann_view* kn, const ann_view* vn, const ann_
     a.block = block;
     if (x[0].numel() == 0 || a.cap == 0) return ANN_OK;
     int64_t const per_block = std::min<int64_t>(block, a.cap) * a.D;
-    if (per_block > INT32_MAX) return fail(ANN_ENOTSUP, "kvCacheAppendQ8: a block of one head exceeds 2^31 values.");
+    if (per_block > INT32_MAX - kThreads) return fail(ANN_ENOTSUP, "kvCacheAppendQ8: a block of one head exceeds 2^31 values.");
     a.vec = 1;
     for (int k = 0; k < 2; ++k) {
         a.c[k] = tensor_of(q[k], s[k], layout);
@@ -394,7 +394,7 @@ int read_back(ann_stream stream, const ann_view* kc, const ann_view* vc, const a
     a.D = q[0].ext[3];
     a.Tout = o[0].ext[tok];
     if (o[0].numel() == 0) return ANN_OK;
-    if (a.Tout * a.D > INT32_MAX) return fail(ANN_ENOTSUP, "kvCacheReadQ8: a head of more than 2^31 values.");
+    if (a.Tout > INT32_MAX / a.D - kReadItems) return fail(ANN_ENOTSUP, "kvCacheReadQ8: a head of more than 2^31 values.");
     a.vec = 1;
     for (int k = 0; k < 2; ++k) {
         a.c[k] = tensor_of(q[k], s[k], layout);

@@ -83,6 +83,8 @@ struct Q4 {
     static constexpr size_t OFF_D = OFF_R + sizeof(float) * 2 * (ITEMS + kMaxCluster);
     static constexpr size_t ROOM = kMaxDigits < 227 * 1024 - OFF_D ? kMaxDigits : 227 * 1024 - OFF_D;
     static constexpr size_t QUAD = size_t{4} * NT * (32 * sizeof(uint2) + 4 * sizeof(int));
+    // Quads of inputs whose digits fit the largest cluster's CTAs (a CTA's share may be one longer).
+    static constexpr int64_t MAX_QUADS = kMaxCluster * (static_cast<int64_t>(ROOM / QUAD) - 1);
 };
 
 // c += a b, int8 products of depth 32, exact in int32.
@@ -475,10 +477,9 @@ int launch(ann_stream stream, LinearQ4Args& a) {
     int64_t const want = ceil_div(int64_t{2} * sm_count(), tiles * row_tiles);
     int64_t splits = std::max<int64_t>(1, std::min(want, quads / kWarps));
     int64_t const per_quad = static_cast<int64_t>(C::QUAD);
-    splits = std::max(splits, ceil_div((quads + kWarps) * per_quad, static_cast<int64_t>(C::ROOM)));
+    splits = std::max(splits, ceil_div(quads, C::MAX_QUADS / kMaxCluster));
     splits = std::min<int64_t>(splits, kMaxCluster);
     int64_t const mine = ceil_div(quads, splits) + 1;  // quads of a CTA at most
-    if (mine * per_quad > static_cast<int64_t>(C::ROOM)) return fail(ANN_ENOTSUP, "linearQ4: too many inputs (%lld).", static_cast<long long>(a.K));
     size_t const smem = C::OFF_D + static_cast<size_t>(mine * per_quad);
     a.splits = static_cast<int>(splits);
     // As many clusters as fit the GPU at once, each with the same number of tiles or one less.
@@ -507,10 +508,15 @@ int launch_vec(ann_stream stream, LinearQ4Args& a, bool vec) {
     return vec ? launch<CT, NT, true>(stream, a) : launch<CT, NT, false>(stream, a);
 }
 
+// The rows of a CTA: all of them up to eight, fewer where the inputs are so many
+// that the digits of eight rows do not fit.
 template <int CT>
 int launch_rows(ann_stream stream, LinearQ4Args& a, bool vec) {
-    if (a.M <= 2) return launch_vec<CT, 1>(stream, a, vec);
-    if (a.M <= 4) return launch_vec<CT, 2>(stream, a, vec);
+    int64_t const quads = ceil_div(a.K, 128);
+    if (quads > Q4<CT, 1>::MAX_QUADS)
+        return fail(ANN_ENOTSUP, "linearQ4: more than %lld inputs.", static_cast<long long>(128 * Q4<CT, 1>::MAX_QUADS));
+    if (a.M <= 2 || quads > Q4<CT, 2>::MAX_QUADS) return launch_vec<CT, 1>(stream, a, vec);
+    if (a.M <= 4 || quads > Q4<CT, 4>::MAX_QUADS) return launch_vec<CT, 2>(stream, a, vec);
     return launch_vec<CT, 4>(stream, a, vec);
 }
 
@@ -574,7 +580,6 @@ int linear_q4(ann_stream stream, const ann_view* x_v, const ann_view* p_v, const
     if (act < ANN_ACT_NONE || act > ANN_ACT_GELU) return fail(ANN_EINVAL, "linearQ4: unknown activation %d.", act);
     if (x.rank != 2 || y.rank != 2 || x.ext[1] != 8 * p.ext[0] || y.ext[0] != x.ext[0] || y.ext[1] != p.ext[1])
         return fail(ANN_EINVAL, "linearQ4 shape mismatch.");
-    if (x.ext[1] > INT32_MAX) return fail(ANN_ENOTSUP, "linearQ4: more than 2^31 inputs.");
     if (!writable(y)) return fail(ANN_EINVAL, "linearQ4: an output axis has a zero pitch.");
     LinearQ4Args a{};
     if (b_v != nullptr) {

@@ -468,8 +468,15 @@ int ann_signal_barrier_dev(ann_stream stream, uint32_t* signals, uint32_t* const
  * No reference counterpart: rotary positions with a position per token, the KV
  * cache in 8 bits and linear layers with 4-bit weights, for decode steps bound
  * by the cache's and the weights' bytes. Outputs must not have a zero pitch on
- * an axis longer than one; inputs may (a broadcast view). No call allocates
- * device memory or waits, so each can be captured in a CUDA graph.
+ * an axis longer than one; inputs may (a broadcast view). Outputs must not overlap
+ * inputs except where said. No call waits, each can be captured in a CUDA graph, and
+ * only attentionDecodeQ8 over long caches takes device memory: a few megabytes of
+ * scratch, allocated and freed in stream order from a pool that the library keeps
+ * for each device (in a captured call they become nodes of the graph, so such a
+ * graph cannot be a child graph). ANN_ENOTSUP where a grid or a 32-bit count would
+ * overflow: rotary from 2^39 vectors of a token on, append from 2^31 tokens or values
+ * of a head's block, read-back from 2^31 values of a head, attention from 2^30
+ * keys or query rows of a KV head.
  *
  * rotary: for pair p of a head vector at position t, a = t * frequencies[p] in
  * 64 bits, (x0, x1) -> magnitude * (x0 cos a - x1 sin a, x0 sin a + x1 cos a).
@@ -509,11 +516,11 @@ int ann_rotary_frequencies(ann_stream stream, const ann_view* frequencies, doubl
  * [positions[b], positions[b] + counts[b]) of sequence b (positions, counts:
  * int32 [B]; counts NULL = Tn, values are held to [0, Tn]; rows past the count
  * are padding and not read). A touched block's scale becomes the larger of
- * max|x| * (1/127), both in float32, over its new rows and, if it holds tokens before positions[b],
- * its old scale (its absolute value, should a caller have stored a negative
- * one); new values are the whole numbers nearest to the exact quotient
- * x / scale (ties to even, within [-127, 127]); where the scale grew, the
- * block's earlier values are rounded anew from n * old / new. Tokens of a
+ * max|x| * (1/127), both in float32, over its new rows and, if it holds tokens
+ * before positions[b], its old scale (its absolute value, should a caller have
+ * stored a negative one); new values are the whole numbers nearest to the exact
+ * quotient x / scale (ties to even, within [-127, 127]); where the scale grew,
+ * the block's earlier values are rounded anew from n * old / new. Tokens of a
  * touched block after the new rows are left as they were and are not part of
  * the sequence any more. A NaN or infinite input makes its block's scale NaN or
  * infinite and its integers 0. Rows outside [0, Tcap) are dropped and set
@@ -535,9 +542,11 @@ int ann_kv_cache_read_q8_f32(ann_stream stream, const ann_view* k_cache, const a
  * [B] keys per sequence, held to [0, Tcap] (NULL = Tcap). causal != 0: query i
  * sees the keys before lengths[b] - Tq + 1 + i (all of them for Tq = 1); else
  * every query sees lengths[b] keys. A query that sees no key gives a row of
- * zeros. Scores, softmax and sums are held to fp32 accuracy. ANN_ENOTSUP
- * unless D is 64, 128 or 256, tokens_per_scale a power of two of 16 or more,
- * and head vectors unit-stride with 16-byte aligned rows. */
+ * zeros. Scores, softmax and sums are held to fp32 accuracy, a query vector's
+ * elements to 2^-31 of its largest. A NaN or infinity in a query vector or in V's
+ * scale of keys that it sees, or a NaN in K's, makes its row NaN. ANN_ENOTSUP
+ * unless D is 64, 128 or 256, tokens_per_scale a power of two of 16 or more, and
+ * head vectors unit-stride with 16-byte aligned rows. */
 int ann_attention_decode_q8_f32(ann_stream stream, const ann_view* q, const ann_view* k_cache,
                                 const ann_view* v_cache, const ann_view* k_scale, const ann_view* v_scale,
                                 const ann_view* lengths, const ann_view* out, float scale,
@@ -556,8 +565,12 @@ int ann_attention_decode_q8_f32(ann_stream stream, const ann_view* q, const ann_
 int ann_pack_weight_q4_f32(ann_stream stream, const ann_view* weight, const ann_view* packed, const ann_view* scales,
                            uint32_t group_size);
 /* output [M,N] = act(input [M,K] . W + bias) + residual; bias (rank 1 [N]) and
- * residual ([M,N], may be output) may be NULL, act is ANN_ACT_*. Meant for the few rows of
- * a decode step (the weights are read once per 16 rows). */
+ * residual ([M,N], may be output) may be NULL, act is ANN_ACT_*. Sums are held to
+ * fp32 accuracy, inputs to 2^-31 of the largest of their row; a NaN or infinity in
+ * a row of the input makes that row's sums NaN (relu makes 0 of them, as elsewhere).
+ * Meant for the few rows of a decode step:
+ * the weights are read once for every eight rows, up to 57344 inputs (for four rows up
+ * to 129024, else two). ANN_ENOTSUP for K > 260096 and for more than 131070 rows. */
 int ann_linear_q4_f32(ann_stream stream, const ann_view* input, const ann_view* packed, const ann_view* scales,
                       const ann_view* bias, const ann_view* residual, const ann_view* output, uint32_t group_size,
                       int32_t act);
