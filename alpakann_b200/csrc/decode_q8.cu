@@ -15,6 +15,7 @@
 #include <set>
 
 #include "common.cuh"
+#include "pairs.cuh"
 #include "reduce.cuh"
 #include "tma.cuh"
 
@@ -165,34 +166,6 @@ __device__ __forceinline__ uint32_t halves_of(uint32_t w, uint32_t sel) {
     uint32_t const biased = __byte_perm(w, 0x64646464u, sel);
     __half2 const h = __hsub2(*reinterpret_cast<__half2 const*>(&biased), __half2half2(__ushort_as_half(0x6480)));
     return *reinterpret_cast<uint32_t const*>(&h);
-}
-
-// Two fp32 values in one 64-bit register: one instruction for both.
-using pair_t = unsigned long long;
-__device__ __forceinline__ pair_t pair(float x, float y) {
-    pair_t v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
-    return v;
-}
-__device__ __forceinline__ float2 unpair(pair_t v) {
-    float2 f;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-    return f;
-}
-__device__ __forceinline__ pair_t add2(pair_t a, pair_t b) {
-    pair_t v;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
-    return v;
-}
-__device__ __forceinline__ pair_t mul2(pair_t a, pair_t b) {
-    pair_t v;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
-    return v;
-}
-__device__ __forceinline__ pair_t fma2(pair_t a, pair_t b, pair_t c) {
-    pair_t v;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
-    return v;
 }
 
 // x, y -> their fp16 parts, high and low, each as a pair.
@@ -1018,8 +991,7 @@ int launch_cluster(ann_stream stream, DecodeQ8Args& a, int64_t units) {
     cfg.stream = as_stream(stream);
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    cudaError_t const e = cudaLaunchKernelEx(&cfg, kernel, a);
-    if (e != cudaSuccess) return fail(ANN_ECUDA, "attentionDecodeQ8: %s", cudaGetErrorString(e));
+    cudaLaunchKernelEx(&cfg, kernel, a);
     return check_launch("attentionDecodeQ8");
 }
 
@@ -1051,10 +1023,8 @@ int launch_shares(ann_stream stream, DecodeQ8Args& a, int64_t units) {
         cfg.stream = as_stream(stream);
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
-        cudaError_t const e = cudaLaunchKernelEx(&cfg, merge_kernel<D, C::ROWS, C::KT>, a, static_cast<int>(G), W,
-                                                 per_block);
-        rc = e != cudaSuccess ? fail(ANN_ECUDA, "attentionDecodeQ8: %s", cudaGetErrorString(e))
-                              : check_launch("attentionDecodeQ8");
+        cudaLaunchKernelEx(&cfg, merge_kernel<D, C::ROWS, C::KT>, a, static_cast<int>(G), W, per_block);
+        rc = check_launch("attentionDecodeQ8");
     }
     cudaFreeAsync(parts, as_stream(stream));
     return rc;

@@ -9,10 +9,13 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <array>
+#include <map>
 #include <mutex>
-#include <set>
+#include <type_traits>
 
 #include "common.cuh"
+#include "pairs.cuh"
 #include "tma.cuh"
 
 namespace cg = cooperative_groups;
@@ -30,8 +33,11 @@ struct LinearQ4Args {
     int64_t x_m, x_k, w_r, w_n, s_g, s_n, b_n, r_m, r_n, y_m, y_n;
     int64_t M, K, N;
     int group, act;
-    int x_vec;   // eight inputs are two aligned 16-byte loads
-    int splits;  // CTAs of a cluster that share the inputs
+    int x_vec;       // eight inputs are two aligned 16-byte loads
+    int splits;      // CTAs of a cluster that share the inputs
+    int share_log2;  // 2^this warps of a CTA share the inputs, the others have columns of their own
+    int ends;        // rows of scales that a quad needs at most
+    int off_r, off_s, off_d;  // shared memory: the cluster's sums, scales, digits
 };
 
 __device__ __forceinline__ float activate(float v, int act) {
@@ -43,55 +49,64 @@ __device__ __forceinline__ float activate(float v, int act) {
     }
 }
 
-// The product in whole numbers. A nibble u is an 8-bit operand as it is: two
-// masks unpack the eight of a word. A row of x is rounded to 31 bits of its
-// largest value (over a warp's inputs) and cut into four 8-bit digits, and
+// The product in whole numbers. With its top bit flipped a nibble u is u - 8 in two's
+// complement; in the upper half of a byte it is the int8 operand 16 (u - 8), so two
+// masks (and a shift) unpack the eight of a word. A row of x is rounded to 31 bits of its
+// largest value (over the inputs that the CTA shares, or the warp) and cut into four 8-bit digits, and
 // mma.sync.m16n8k32 on int8 multiplies, transposed: 16 columns of W by 8 slots,
-// the slots being the digits of two rows. The sums are exact in int32, the offset
-// of 8 included: a product with ones gives the digits' sums, of which eight times
-// are taken off. They become fp32 when their group of inputs ends and meet its
+// the slots being the digits of two rows. The sums are exact in int32, and become fp32
+// when their group of inputs or 128 of them end, to meet their
 // scale. The order of the summed index is free, so a lane takes the words as a
 // 16-byte load gives them, eight inputs (its octet of 32) of four neighbouring
 // columns; x's digits are laid out to match.
 //
-// A CTA stays and takes one tile of 32 CT columns after another. Each of its warps
-// (and each CTA of a cluster, where columns are few) has inputs of its own, whose
-// digits it prepares once; it streams their weights, 128 inputs at a time (a quad
-// of products' depth), through a ring in shared memory (cp.async, on across tiles),
-// 4 to 8 KB in flight a warp. The warps' sums of a
+// A CTA stays and takes one set of tiles of 32 CT columns after another. Its warps
+// have tiles of their own, or share one, each with inputs of its own (and the CTAs of a
+// cluster share them, where columns are few or the digits of all inputs do not fit).
+// The digits are prepared once; a warp streams its weights, 128 inputs at a time (a quad
+// of products' depth), and their scales through a ring in shared memory (cp.async, on
+// across tiles), 4 to 8 KB in flight a warp. The sums of a
 // tile meet in shared memory, across a cluster in the CTA that owns a share of the
 // columns, which applies bias, activation and residual. One launch, no scratch
 // memory, no atomics, a fixed order of sums.
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxCluster = 16;
-// Bytes of x's digits in a CTA: at most 68 steps of 32 inputs a warp, whose digits'
-// products with nibbles, |u d| <= 1920, sum up to less than 2^23: 256 times that
-// fits 32 bits.
-constexpr size_t kMaxDigits = 136 << 10;
+constexpr size_t kMaxSmem = 227 * 1024;
+
+// The int32 sums start at the bits of 1.5 * 2^23: with less than 2^22 added (128
+// products of at most 128 * 128), the bits are those of the fp32 value 1.5 * 2^23 +
+// sum, and no conversion is needed.
+constexpr int kStartBits = 0x4b400000;
 
 // Shared memory: rings [kWarps][DEPTH quads][4][CT][32] uint4, two buffers of sums
-// [kWarps][ROWS][COLS] and of the cluster's [per * splits]; then per quad of the
-// CTA digits uint2 [4][NT][32] and offsets int [4][NT][4].
-template <int CT, int NT>
+// [kWarps][ROWS][COLS]; by the call, two of the cluster's [per * splits], scales
+// [kWarps][DEPTH + 1][ends][COLS] and, per quad of the CTA, digits uint2 [4][NT][32].
+template <int CT, int NT, int QUADS = 4 / CT>
 struct Q4 {
     static constexpr int COLS = 32 * CT, ROWS = 2 * NT, ITEMS = ROWS * COLS;
-    static constexpr int DEPTH = 4 / CT;                            // quads in flight a warp
+    static constexpr int DEPTH = QUADS;                              // quads in flight a warp
     static constexpr size_t RING = size_t{16} * DEPTH * 4 * CT * 32;  // of a warp
     static constexpr size_t OFF_S = RING * kWarps;
-    static constexpr size_t OFF_R = OFF_S + sizeof(float) * 2 * kWarps * ITEMS;
-    static constexpr size_t OFF_D = OFF_R + sizeof(float) * 2 * (ITEMS + kMaxCluster);
-    static constexpr size_t ROOM = kMaxDigits < 227 * 1024 - OFF_D ? kMaxDigits : 227 * 1024 - OFF_D;
-    static constexpr size_t QUAD = size_t{4} * NT * (32 * sizeof(uint2) + 4 * sizeof(int));
-    // Quads of inputs whose digits fit the largest cluster's CTAs (a CTA's share may be one longer).
-    static constexpr int64_t MAX_QUADS = kMaxCluster * (static_cast<int64_t>(ROOM / QUAD) - 1);
+    static constexpr size_t FIXED = OFF_S + sizeof(float) * 2 * kWarps * ITEMS;
+    static constexpr size_t QUAD = size_t{4} * NT * 32 * sizeof(uint2);
+    static constexpr size_t scales(int ends) { return sizeof(float) * kWarps * (DEPTH + 1) * ends * COLS; }
+    static constexpr size_t received(int columns) { return sizeof(float) * 2 * (ROWS * columns + kMaxCluster); }
+    // Quads of inputs whose digits fit a CTA at the least.
+    static constexpr int64_t LEAST = (kMaxSmem - FIXED - scales(4) - received(COLS)) / QUAD;
 };
 
-// c += a b, int8 products of depth 32, exact in int32.
+// c += a b, or c = start + a b: int8 products of depth 32, exact in int32.
+template <bool FRESH>
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y));
+    if constexpr (FRESH)
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y), "r"(kStartBits));
+    else
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y));
 }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -102,23 +117,25 @@ __device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
 
 // CT: 16-byte words of columns per lane (32 CT columns a tile); NT: slots / 8 (2 NT
 // rows a CTA); VEC: words and scales of four columns are one aligned load.
-template <int CT, int NT, bool VEC>
+template <typename C, int CT, int NT, bool VEC>
 __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kernel(LinearQ4Args a) {
-    using C = Q4<CT, NT>;
     extern __shared__ __align__(16) unsigned char smem[];
     int const tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     int const split = static_cast<int>(blockIdx.x) % a.splits;
     if (a.splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // "this CTA runs"
     int64_t const row0 = static_cast<int64_t>(blockIdx.y) * C::ROWS;
-    // this warp's quads of 128 inputs, in steps of 32
-    int const quads = static_cast<int>((a.K + 127) / 128), parts = a.splits * kWarps, part = split * kWarps + warp;
-    int const first = static_cast<int>(static_cast<int64_t>(quads) * (split * kWarps) / parts);  // the CTA's first
-    int const q0 = static_cast<int>(static_cast<int64_t>(quads) * part / parts);
-    int const q1 = static_cast<int>(static_cast<int64_t>(quads) * (part + 1) / parts);
-    int const s0 = 4 * q0, s1 = min(4 * q1, static_cast<int>((a.K + 31) / 32));
+    // the CTA's quads of 128 inputs [first, last), the warp's [q0, q1), in steps of 32;
+    // `across` warps side by side have tiles of their own, `share` the same one
+    int const quads = static_cast<int>((a.K + 127) / 128), steps = static_cast<int>((a.K + 31) / 32);
+    int const first = static_cast<int>(static_cast<int64_t>(quads) * split / a.splits);
+    int const last = static_cast<int>(static_cast<int64_t>(quads) * (split + 1) / a.splits);
+    int const share = 1 << a.share_log2, across_log2 = 3 - a.share_log2, across = 1 << across_log2;
+    int const part = warp >> across_log2, mine = warp & (across - 1);
+    int const q0 = first + ((last - first) * part >> a.share_log2), q1 = first + ((last - first) * (part + 1) >> a.share_log2);
     int const octets = static_cast<int>(a.K / 8), per_group = a.group / 32;
     int const tiles = static_cast<int>((a.N + C::COLS - 1) / C::COLS);
-    int const tile0 = static_cast<int>(blockIdx.x) / a.splits, stride = static_cast<int>(gridDim.x) / a.splits;
+    int const sets = (tiles + across - 1) >> across_log2;  // a CTA's tiles at a time
+    int const set0 = static_cast<int>(blockIdx.x) / a.splits, stride = static_cast<int>(gridDim.x) / a.splits;
 
     // A lane copies 16 bytes of word row lane / 8 of four, so that eight lanes take
     // 128 consecutive bytes; the lane that uses them is (g, t) = (4 columns, row). The
@@ -127,48 +144,88 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
     int const fg = lane & 7, ft = lane >> 3;
     uint4* const ring = reinterpret_cast<uint4*>(smem + C::RING * warp) + 8 * t + (g ^ (2 * t));
     uint32_t const ring_u = smem_u32(smem + C::RING * warp) + 16 * (8 * ft + (fg ^ (2 * ft)));
-    unsigned char* const mine = smem + C::OFF_D + C::QUAD * (q0 - first);  // digits and offsets, quad by quad
-    // Quads are fetched in the order of their use, tile after tile.
+    int const place_size = a.ends * C::COLS;  // floats
+    float* const scale_ring = reinterpret_cast<float*>(smem + a.off_s) + warp * (C::DEPTH + 1) * place_size;
+    uint32_t const scale_ring_u = smem_u32(scale_ring);
+    // Sums meet their scale after the last step of a group and of a quad. The bits of
+    // such steps, given the steps left in the group; `passed`: groups that end.
+    int const left0 = per_group - 4 * q0 % per_group;
+    auto ends = [&](int quad, int& left, int& passed) {
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (--left == 0) m |= 1u << i, left = per_group;
+        passed = __popc(m);
+        unsigned const end = 1u << min(3, steps - 1 - 4 * quad);  // steps past K have no group
+        return (m & (end - 1u)) | end;
+    };
+    // Quads are fetched in the order of their use, tile after tile, each with the
+    // rows of scales that its sums meet. Scales have one place more than weights, as
+    // they are read until the quad's end, its weights only at its start.
     int64_t const w_step = 4 * a.w_r;
     uint32_t const* const w0 = a.w + (16 * static_cast<int64_t>(q0) + ft) * a.w_r + 4 * fg * a.w_n;
     uint32_t const* f_w = w0;
-    int f_tile = tile0, f_quad = q0, f_slot = 0, f_cols = 0;  // f_cols: columns from this lane's first on, 0: none
+    float const* f_s = a.s;
+    int f_tile = set0 * across + mine, f_quad = q0, f_slot = 0, f_place = 0, f_cols = 0, f_left = left0;  // f_cols: columns of the tile
     auto open_tile = [&]() {
         int64_t const col = static_cast<int64_t>(f_tile) * C::COLS;
         f_w = w0 + col * a.w_n;
-        f_cols = f_tile < tiles && q0 < q1 ? max(0, static_cast<int>(min(a.N - col, int64_t{C::COLS})) - 4 * fg) : 0;
+        f_s = a.s + static_cast<int64_t>(4 * q0 / per_group) * a.s_g + col * a.s_n;
+        f_cols = static_cast<int>(min(a.N - col, int64_t{C::COLS}));
         f_quad = q0;
+        f_left = left0;
     };
     auto fetch = [&]() {
         if (f_tile < tiles && q0 < q1) {
             uint32_t const dst = ring_u + static_cast<uint32_t>(f_slot) * (4 * CT * 512);
+            int const from = f_cols - 4 * fg;  // columns from this lane's first on
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 bool const in = 16 * f_quad + 4 * i + ft < octets;
 #pragma unroll
                 for (int c = 0; c < CT; ++c) {
                     if constexpr (VEC) {
-                        if (in && 32 * c < f_cols) copy16(dst + (i * CT + c) * 512, f_w + 32 * c);
+                        if (in && 32 * c < from) copy16(dst + (i * CT + c) * 512, f_w + 32 * c);
                     } else {
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            if (in && 32 * c + e < f_cols) copy4(dst + (i * CT + c) * 512 + 4 * e, f_w + (32 * c + e) * a.w_n);
+                            if (in && 32 * c + e < from) copy4(dst + (i * CT + c) * 512 + 4 * e, f_w + (32 * c + e) * a.w_n);
                     }
                 }
                 f_w += w_step;
             }
-            if (++f_quad == q1) f_tile += stride, open_tile();
+            int passed;
+            int const n = __popc(ends(f_quad, f_left, passed));  // rows of scales
+            uint32_t const dst_s = scale_ring_u + static_cast<uint32_t>(f_place * place_size) * 4;
+#pragma unroll
+            for (int e = 0; e < CT; ++e) {
+                int const i = lane + 32 * e, r = i / (8 * CT), c = 4 * (i % (8 * CT));
+                float const* const p = f_s + r * a.s_g + c * a.s_n;
+                if constexpr (VEC) {
+                    if (r < n && c < f_cols) copy16(dst_s + 16 * i, p);
+                } else {
+#pragma unroll
+                    for (int d = 0; d < 4; ++d)
+                        if (r < n && c + d < f_cols) copy4(dst_s + 16 * i + 4 * d, p + d * a.s_n);
+                }
+            }
+            f_s += passed * a.s_g;
+            if (++f_quad == q1) f_tile += stride * across, open_tile();
         }
         if (++f_slot == C::DEPTH) f_slot = 0;
+        if (++f_place == C::DEPTH + 1) f_place = 0;
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     open_tile();
 
-    // x's digits: a lane takes an octet of a row at a time, eight steps a warp. First
+    // x's digits: every warp prepares an eighth of the CTA's quads (its own, if all
+    // warps share a tile). A lane takes an octet of a row at a time, eight steps a warp. First
     // the rows' largest values (the first eight steps' inputs stay in registers, and
     // their loads go out before the weights'), then the digits. Lanes t and t + 1 of
     // a row's four slots hold its high and low digits, so a lane keeps the factor of
     // row t / 2 of its two.
+    int const s0 = 4 * (first + ((last - first) * warp >> 3)), s_end = 4 * (first + ((last - first) * (warp + 1) >> 3));
+    int const s1 = min(s_end, steps);
     float down[NT], up[C::ROWS];
     auto load_x = [&](int r, int base, float (&x)[8]) {
         int64_t const m = row0 + r, k = 32 * static_cast<int64_t>(base) + 8 * lane;
@@ -205,8 +262,19 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
             for (int r = 0; r < C::ROWS; ++r) raise(y[r], top[r]);
         }
 #pragma unroll
+        for (int r = 0; r < C::ROWS; ++r) top[r] = __reduce_max_sync(0xffffffffu, top[r]);
+        if (across > 1) {  // digits of one warp meet weights of another: one factor for all
+            unsigned int* const all = reinterpret_cast<unsigned int*>(smem + C::OFF_S);
+#pragma unroll
+            for (int r = 0; r < C::ROWS; ++r)
+                if (lane == 0) all[warp * C::ROWS + r] = top[r];
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < C::ROWS; ++r) top[r] = __reduce_max_sync(0xffffffffu, all[(lane & 7) * C::ROWS + r]);
+        }
+#pragma unroll
         for (int r = 0; r < C::ROWS; ++r) {
-            unsigned int const m = __reduce_max_sync(0xffffffffu, top[r]);
+            unsigned int const m = top[r];
             // the largest value into [2^29, 2^30): 2^(156 - e), e its biased exponent, where both factors are normal
             int const e = min(max(static_cast<int>(m >> 23), 31), 254);
             up[r] = __int_as_float((283 - e) << 23);
@@ -215,13 +283,13 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
             if ((t >> 1) == (r & 1)) down[r / 2] = back;
         }
     }
-    for (int base = s0; base < 4 * q1; base += 8) {
+    for (int base = s0; base < s_end; base += 8) {
         if (base != s0) {
 #pragma unroll
             for (int r = 0; r < C::ROWS; ++r) load_x(r, base, x[r]);
         }
-        int const st = base - s0 + (lane >> 2);
-        if (st >= 4 * (q1 - q0)) continue;
+        int const st = base - 4 * first + (lane >> 2);
+        if (st >= s_end - 4 * first) continue;
 #pragma unroll
         for (int r = 0; r < C::ROWS; ++r) {
             uint32_t n[8];  // signed base-256 digits: a carry out of the lower bytes, then their signs
@@ -239,125 +307,73 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
                 d[h][2] = __byte_perm(lo01, lo23, 0x7632);
                 d[h][3] = __byte_perm(lo01, lo23, 0x5410);
             }
-            uint2* const to = reinterpret_cast<uint2*>(mine + C::QUAD * (st / 4)) + ((st % 4) * NT + r / 2) * 32 + (r & 1) * 16 + t;
+            uint2* const to = reinterpret_cast<uint2*>(smem + a.off_d + C::QUAD * (st / 4)) + ((st % 4) * NT + r / 2) * 32 + (r & 1) * 16 + t;
 #pragma unroll
             for (int j = 0; j < 4; ++j) to[4 * j] = make_uint2(d[0][j], d[1][j]);
         }
     }
-    __syncwarp();
+    if (across > 1)
+        __syncthreads();
+    else
+        __syncwarp();
 
-    // Sums meet their scale after the last step of a group and after the range's
-    // last. The bits of such steps in a quad, given the steps left in its group.
-    int const left0 = per_group - s0 % per_group;
-    auto ends = [&](int quad, int& left) {
-        unsigned m = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (--left == 0) m |= 1u << i, left = per_group;
-        if (quad + 1 < q1) return m;
-        unsigned const last = 1u << (s1 - 1 - 4 * quad);  // steps past K have no group
-        return (m & (last - 1u)) | last;
-    };
-    // 256 times the high plus the low of a pair of digits' sums up to each of these
-    // steps: the nibbles' offset of 8, the same for all columns.
-    {
-        int ones[NT][4], left = left0;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) ones[nt][0] = ones[nt][1] = ones[nt][2] = ones[nt][3] = 0;
-        for (int quad = q0; quad < q1; ++quad) {
-            uint2 const* const dig = reinterpret_cast<uint2 const*>(mine + C::QUAD * (quad - q0)) + lane;
-            int* const off = reinterpret_cast<int*>(mine + C::QUAD * (quad - q0) + 4 * NT * 32 * sizeof(uint2));
-            unsigned const m = ends(quad, left);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                    mma_s8(ones[nt], 0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u, dig[(i * NT + nt) * 32]);
-                if (m >> i & 1u) {
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        if (g == 0) off[(i * NT + nt) * 4 + t] = 8 * (ones[nt][0] * 256 + ones[nt][1]);
-                        ones[nt][0] = ones[nt][1] = ones[nt][2] = ones[nt][3] = 0;
-                    }
-                }
-            }
-        }
-    }
-    __syncwarp();
-
+    unsigned char const* const digits = smem + a.off_d + C::QUAD * (q0 - first);
     int const rows = static_cast<int>(min(static_cast<int64_t>(C::ROWS), a.M - row0));
-    int const items = rows * C::COLS, per = (items + a.splits - 1) / a.splits;
-    int slot = 0;
-    for (int tile = tile0, round = 0; tile < tiles; tile += stride, round ^= 1) {
-        int64_t const col0 = static_cast<int64_t>(tile) * C::COLS;
-        int const cols = static_cast<int>(min(a.N - col0, int64_t{C::COLS})) - 4 * g;  // from this lane's first on
-        float const* ps = a.s + static_cast<int64_t>(s0 / per_group) * a.s_g + (col0 + 4 * g) * a.s_n;
-        float acc[NT][CT][4];
+    int const width_log2 = (CT == 1 ? 5 : 6) + across_log2, items = rows << width_log2;  // of a set
+    int const per = (items + a.splits - 1) / a.splits;
+    int slot = 0, place = 0;
+    pair_t const start = pair(-12582912.0f, -12582912.0f);
+    for (int set = set0, round = 0; set < sets; set += stride, round ^= 1) {
+        pair_t acc[NT][CT][4];  // a pair of digits, high and low, of columns 4g ..
         int c[NT][CT][2][4];  // columns 4g + {0, 1} and 4g + {2, 3}: rows g and g + 8 of two products
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int k = 0; k < CT; ++k)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[nt][k][e] = 0.0f, c[nt][k][0][e] = c[nt][k][1][e] = 0;
-        // The scales of a step's group, this lane's columns.
-        auto scales = [&](float const* p, float4 (&sc)[CT]) {
-#pragma unroll
-            for (int k = 0; k < CT; ++k) {
-                sc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                float const* pk = p + 32 * k * a.s_n;
-                if constexpr (VEC) {
-                    if (32 * k < cols) sc[k] = __ldg(reinterpret_cast<float4 const*>(pk));
-                } else {
-                    if (32 * k < cols) sc[k].x = __ldg(pk);
-                    if (32 * k + 1 < cols) sc[k].y = __ldg(pk + a.s_n);
-                    if (32 * k + 2 < cols) sc[k].z = __ldg(pk + 2 * a.s_n);
-                    if (32 * k + 3 < cols) sc[k].w = __ldg(pk + 3 * a.s_n);
-                }
-            }
-        };
+                for (int e = 0; e < 4; ++e) acc[nt][k][e] = pair(0.0f, 0.0f);
         // Octets past K and columns past N: whatever lies in the ring meets digits of
-        // 0, or is not stored.
-        auto multiply = [&](uint4 const (&w)[CT], uint2 const (&b)[NT]) {
+        // 0, or is not stored. FRESH: the first product of a sum.
+        auto multiply = [&]<bool FRESH>(std::bool_constant<FRESH>, uint4 const (&w)[CT], uint2 const (&b)[NT]) {
 #pragma unroll
             for (int k = 0; k < CT; ++k)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t const w0 = h ? w[k].z : w[k].x, w1 = h ? w[k].w : w[k].y;
-                    uint32_t const a0 = w0 & 0x0f0f0f0fu, a2 = (w0 >> 4) & 0x0f0f0f0fu;
-                    uint32_t const a1 = w1 & 0x0f0f0f0fu, a3 = (w1 >> 4) & 0x0f0f0f0fu;
+                    uint32_t const a0 = (w0 << 4 ^ 0x80808080u) & 0xf0f0f0f0u, a2 = (w0 ^ 0x80808080u) & 0xf0f0f0f0u;
+                    uint32_t const a1 = (w1 << 4 ^ 0x80808080u) & 0xf0f0f0f0u, a3 = (w1 ^ 0x80808080u) & 0xf0f0f0f0u;
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma_s8(c[nt][k][h], a0, a1, a2, a3, b[nt]);
+                    for (int nt = 0; nt < NT; ++nt) mma_s8<FRESH>(c[nt][k][h], a0, a1, a2, a3, b[nt]);
                 }
         };
-        auto flush = [&](int const* off, float4 const (&sc)[CT]) {
+        // Sums to fp32, with the scales sc[8 k] of column word k.
+        auto flush = [&](float4 const* sc) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                int const o = off[4 * nt];
+            for (int k = 0; k < CT; ++k) {
+                float4 const s4 = sc[8 * k];
+                pair_t const f[4] = {pair(s4.x, s4.x), pair(s4.y, s4.y), pair(s4.z, s4.z), pair(s4.w, s4.w)};
 #pragma unroll
-                for (int k = 0; k < CT; ++k) {
-                    float const f[4] = {sc[k].x, sc[k].y, sc[k].z, sc[k].w};
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        int (&q)[4] = c[nt][k][e / 2];
+                        int const (&q)[4] = c[nt][k][e / 2];
                         int const j = 2 * (e & 1);
-                        acc[nt][k][e] = fmaf(static_cast<float>(q[j] * 256 + q[j + 1] - o), f[e], acc[nt][k][e]);
-                        q[j] = q[j + 1] = 0;
+                        acc[nt][k][e] = fma2(add2(pair(__int_as_float(q[j]), __int_as_float(q[j + 1])), start), f[e], acc[nt][k][e]);
                     }
-                }
             }
         };
+        bool const given = (set << across_log2) + mine < tiles;
         int left = left0;
-        for (int quad = q0; quad < q1; ++quad) {
-            unsigned const m = ends(quad, left);
-            float4 sc[CT];
-            if (m != 0u) scales(ps, sc);  // of the first step that needs them; used when the weights have come
-            uint2 const* const dig = reinterpret_cast<uint2 const*>(mine + C::QUAD * (quad - q0)) + lane;
-            int const* const off = reinterpret_cast<int const*>(mine + C::QUAD * (quad - q0) + 4 * NT * 32 * sizeof(uint2)) + t;
+        for (int quad = q0; quad < q1 && given; ++quad) {
+            int passed;
+            unsigned const m = ends(quad, left, passed);
+            uint2 const* const dig = reinterpret_cast<uint2 const*>(digits + C::QUAD * (quad - q0)) + lane;
             asm volatile("cp.async.wait_group %0;" ::"n"(C::DEPTH - 1) : "memory");
             __syncwarp();
             uint4 const* const rs = ring + slot * (4 * CT * 32);
             if (++slot == C::DEPTH) slot = 0;
+            float4 const* sc = reinterpret_cast<float4 const*>(scale_ring + place * place_size) + g;
+            if (++place == C::DEPTH + 1) place = 0;
             uint4 w[4][CT];
             uint2 b[4][NT];  // all at once, or with four n-tiles a step's at a time
             auto load_b = [&](int i) {
@@ -372,35 +388,37 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
             }
             __syncwarp();  // the warp has read the quad; its place takes another
             fetch();
-            if ((m & 7u) == 0u) {  // groups of 128 inputs or more: no sum ends within the quad
+            constexpr std::true_type fresh{};
+            constexpr std::false_type more{};
+            if (m == 8u) {  // groups of 128 inputs or more
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     if constexpr (NT > 2) load_b(i);
-                    multiply(w[i], b[i]);
+                    if (i == 0) multiply(fresh, w[i], b[i]);
+                    else multiply(more, w[i], b[i]);
                 }
-                if (m != 0u) {
-                    flush(off + 12 * NT, sc);
-                    ps += a.s_g;
+                flush(sc);
+            } else if (m == 10u) {  // of 64
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (NT > 2) load_b(i);
+                    if (i % 2 == 0) multiply(fresh, w[i], b[i]);
+                    else multiply(more, w[i], b[i]), flush(sc), sc += 8 * CT;
                 }
             } else {
+                bool begins = true;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    float4 next[CT];
-                    bool const ends_here = m >> i & 1u, another = ends_here && m >> (i + 1) != 0u;
-                    if (another) scales(ps + a.s_g, next);
                     if constexpr (NT > 2) load_b(i);
-                    multiply(w[i], b[i]);
-                    if (!ends_here) continue;
-                    flush(off + 4 * NT * i, sc);
-                    ps += a.s_g;
-                    if (another) {
-#pragma unroll
-                        for (int k = 0; k < CT; ++k) sc[k] = next[k];
-                    }
+                    if (begins) multiply(fresh, w[i], b[i]);
+                    else multiply(more, w[i], b[i]);
+                    begins = m >> i & 1u;
+                    if (begins) flush(sc), sc += 8 * CT;
                 }
             }
         }
-        // Warps to CTA: high and low digits, the row's factor, then the sums.
+        // Warps to CTA: high and low digits, the row's factor (and the 16 of the
+        // operands), then the sums.
         float* const sums = reinterpret_cast<float*>(smem + C::OFF_S) + round * (kWarps * C::ITEMS);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -409,23 +427,25 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
                 float v[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float const low = __shfl_down_sync(0xffffffffu, acc[nt][k][e], 1);
-                    v[e] = fmaf(acc[nt][k][e], 65536.0f, low) * down[nt];
+                    float2 const d = unpair(acc[nt][k][e]);
+                    float const two = fmaf(d.x, 256.0f, d.y), low = __shfl_down_sync(0xffffffffu, two, 1);
+                    v[e] = fmaf(two, 4096.0f, low * 0.0625f) * down[nt];
                 }
                 if ((t & 1) == 0)
                     *reinterpret_cast<float4*>(sums + (warp * C::ROWS + 2 * nt + t / 2) * C::COLS + 32 * k + 4 * g) =
                         make_float4(v[0], v[1], v[2], v[3]);
             }
         __syncthreads();
+        // item i of a set: row i >> width_log2, then the columns of its tiles
         auto sum_warps = [&](int i) {
+            int const r = i >> width_log2, col = i & ((1 << width_log2) - 1);
+            float const* p = sums + (col / C::COLS * C::ROWS + r) * C::COLS + col % C::COLS;
             float v = 0.0f;
-#pragma unroll
-            for (int k = 0; k < kWarps; ++k) v += sums[k * C::ITEMS + i];
+            for (int k = 0; k < share; ++k) v += p[k * (C::ITEMS << across_log2)];
             return v;
         };
         auto store = [&](int i, float v) {
-            int const r = i / C::COLS;
-            int64_t const m = row0 + r, n = col0 + i - r * C::COLS;
+            int64_t const m = row0 + (i >> width_log2), n = (static_cast<int64_t>(set) << width_log2) + (i & ((1 << width_log2) - 1));
             if (n >= a.N) return;
             if (a.bias != nullptr) v += a.bias[n * a.b_n];
             v = activate(v, a.act);
@@ -438,8 +458,8 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
         }
         // CTAs of the cluster: CTA s takes items [s * per, (s + 1) * per) of all of them.
         cg::cluster_group cluster = cg::this_cluster();
-        float* const recv = reinterpret_cast<float*>(smem + C::OFF_R) + round * (C::ITEMS + kMaxCluster);
-        if (tile == tile0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA runs
+        float* const recv = reinterpret_cast<float*>(smem + a.off_r) + round * ((C::ROWS << width_log2) + kMaxCluster);
+        if (set == set0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA runs
         for (int i = tid; i < items; i += kThreads) {
             int const to = i / per;
             cluster.map_shared_rank(recv, to)[split * per + i - to * per] = sum_warps(i);
@@ -453,70 +473,114 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
     }
 }
 
-template <int CT, int NT, bool VEC>
+// Clusters of 1 .. kMaxCluster CTAs that the device holds at once, with one and two
+// CTAs an SM.
+using Room = std::array<std::array<int, kMaxCluster + 1>, 2>;
+constexpr size_t kHalfSmem = 113 * 1024;
+
+template <typename C, int CT, int NT, bool VEC>
 int launch(ann_stream stream, LinearQ4Args& a) {
-    using C = Q4<CT, NT>;
-    auto const kernel = linear_q4_kernel<CT, NT, VEC>;
-    static std::mutex mu;
-    static std::set<int> ready;  // devices whose kernel attributes are set
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return fail(ANN_ECUDA, "linearQ4: no CUDA device.");
-    {
-        std::lock_guard<std::mutex> lock(mu);
-        if (ready.count(dev) == 0) {
-            cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 static_cast<int>(C::OFF_D + C::ROOM));
-            if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-            if (e != cudaSuccess) return fail(ANN_ECUDA, "linearQ4 setup: %s", cudaGetErrorString(e));
-            ready.insert(dev);
-        }
-    }
-    int64_t const tiles = ceil_div(a.N, C::COLS), row_tiles = ceil_div(a.M, C::ROWS), quads = ceil_div(a.K, 128);
-    // Splits of the inputs: until every SM has two CTAs, as long as a warp keeps a
-    // quad; and as many as x's digits need to fit a CTA.
-    int64_t const want = ceil_div(int64_t{2} * sm_count(), tiles * row_tiles);
-    int64_t splits = std::max<int64_t>(1, std::min(want, quads / kWarps));
-    int64_t const per_quad = static_cast<int64_t>(C::QUAD);
-    splits = std::max(splits, ceil_div(quads, C::MAX_QUADS / kMaxCluster));
-    splits = std::min<int64_t>(splits, kMaxCluster);
-    int64_t const mine = ceil_div(quads, splits) + 1;  // quads of a CTA at most
-    size_t const smem = C::OFF_D + static_cast<size_t>(mine * per_quad);
-    a.splits = static_cast<int>(splits);
-    // As many clusters as fit the GPU at once, each with the same number of tiles or one less.
-    int64_t const room = std::max<int64_t>(1, int64_t{sm_count()} * (smem <= (110u << 10) && NT * CT < 4 ? 2 : 1) / (splits * row_tiles));
-    int64_t const rounds = ceil_div(tiles, room), clusters = ceil_div(tiles, rounds);
-    if (tiles > INT32_MAX || row_tiles > 65535) return fail(ANN_ENOTSUP, "linearQ4: grid too large.");
+    auto const kernel = linear_q4_kernel<C, CT, NT, VEC>;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = static_cast<unsigned>(a.splits);
     attr.val.clusterDim.y = 1;
     attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(clusters * splits), static_cast<unsigned>(row_tiles));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = as_stream(stream);
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    cudaError_t const e = cudaLaunchKernelEx(&cfg, kernel, a);
-    if (e != cudaSuccess) return fail(ANN_ECUDA, "linearQ4: %s", cudaGetErrorString(e));
+    static std::mutex mu;
+    static std::map<int, Room> rooms;  // devices whose kernel attributes are set
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return fail(ANN_ECUDA, "linearQ4: no CUDA device.");
+    Room const* room = nullptr;
+    {
+        std::lock_guard<std::mutex> lock(mu);
+        auto it = rooms.find(dev);
+        if (it == rooms.end()) {
+            Room r{};
+            cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMaxSmem));
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            for (int two = 0; two < 2; ++two)
+                for (int n = 1; n <= kMaxCluster && e == cudaSuccess; ++n) {
+                    attr.val.clusterDim.x = static_cast<unsigned>(n);
+                    cfg.gridDim = dim3(static_cast<unsigned>(n));
+                    cfg.dynamicSmemBytes = two ? kHalfSmem : kMaxSmem;
+                    e = cudaOccupancyMaxActiveClusters(&r[two][n], kernel, &cfg);
+                }
+            if (e != cudaSuccess) return fail(ANN_ECUDA, "linearQ4 setup: %s", cudaGetErrorString(e));
+            it = rooms.emplace(dev, r).first;
+        }
+        room = &it->second;
+    }
+    int64_t const tiles = ceil_div(a.N, C::COLS), row_tiles = ceil_div(a.M, C::ROWS), quads = ceil_div(a.K, 128);
+    if (tiles > INT32_MAX || row_tiles > 65535) return fail(ANN_ENOTSUP, "linearQ4: grid too large.");
+    a.ends = a.group == 32 ? 4 : a.group % 128 == 0 ? 1 : 2;
+    // How many warps of a CTA and CTAs of a cluster share the inputs: the least of
+    // these estimates (us, fitted to 14 shapes at 64 choices each; the estimate's best is
+    // within 3 % of the measured best there). A quad takes a warp its memory's latency
+    // with two in flight, or its turn among the SM's warps; preparing a quad's digits,
+    // and what a set of tiles costs to sum and store, count beside it. (8 x 4096 x
+    // 16384: two by two 19 us, all eight warps of two CTAs 23, one of four 20; 1 x 4096 x
+    // 4096: 4 by 4 5.8, eight of one CTA 7.6; 1 x 4096 x 65536: one of two 28, eight of one 31.)
+    size_t smem = 0;
+    int64_t clusters = 0;
+    double best = 1e300;
+    for (int share_log2 = 3; share_log2 >= 0; --share_log2) {
+        int const across = kWarps >> share_log2;
+        size_t const fixed = C::FIXED + C::scales(a.ends);
+        for (int splits = 1; splits <= kMaxCluster; ++splits) {
+            int64_t const in_cta = ceil_div(quads, splits), in_warp = ceil_div(in_cta, int64_t{1} << share_log2);
+            size_t const recv = splits > 1 ? C::received(C::COLS * across) : 0;
+            size_t const need = fixed + recv + static_cast<size_t>(in_cta) * C::QUAD;
+            if (need > kMaxSmem || (splits > 1 && splits > quads)) continue;
+            int const most = (*room)[need <= kHalfSmem][splits];
+            if (most == 0) continue;
+            // as many clusters as fit the GPU at once, each with the same number of sets or one less
+            int64_t const at_once = std::max<int64_t>(1, most / row_tiles), sets = ceil_div(tiles, across);
+            int64_t const rounds = ceil_div(sets, at_once), used = ceil_div(sets, rounds);
+            double const load = std::min<double>(need <= kHalfSmem && NT * CT < 4 ? 2 : 1, static_cast<double>(ceil_div(used * splits * row_tiles, sm_count())));
+            double const quad = std::max(0.8, kWarps * load * (0.02 + 0.0225 * NT) * CT);
+            double const prepare = (0.3 + 0.1 * NT) * load * static_cast<double>(in_cta) / kWarps;
+            double const finish = 1.5 + 0.06 * NT * CT * across * load + (splits > 1 ? 0.4 : 0.0);
+            double const cost = prepare + static_cast<double>(rounds) * (static_cast<double>(in_warp) * quad + finish);
+            if (cost >= best) continue;
+            best = cost;
+            a.share_log2 = share_log2;
+            a.splits = splits;
+            a.off_r = static_cast<int>(C::FIXED);
+            a.off_s = static_cast<int>(C::FIXED + recv);
+            a.off_d = static_cast<int>(fixed + recv);
+            smem = need;
+            clusters = used;
+        }
+    }
+    if (clusters == 0) return fail(ANN_ENOTSUP, "linearQ4: no cluster holds the inputs.");
+    attr.val.clusterDim.x = static_cast<unsigned>(a.splits);
+    cfg.gridDim = dim3(static_cast<unsigned>(clusters * a.splits), static_cast<unsigned>(row_tiles));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = as_stream(stream);
+    cudaLaunchKernelEx(&cfg, kernel, a);
     return check_launch("linearQ4");
 }
 
-template <int CT, int NT>
+template <int CT, int NT, int QUADS = 4 / CT>
 int launch_vec(ann_stream stream, LinearQ4Args& a, bool vec) {
-    return vec ? launch<CT, NT, true>(stream, a) : launch<CT, NT, false>(stream, a);
+    using C = Q4<CT, NT, QUADS>;
+    return vec ? launch<C, CT, NT, true>(stream, a) : launch<C, CT, NT, false>(stream, a);
 }
 
 // The rows of a CTA: all of them up to eight, fewer where the inputs are so many
-// that the digits of eight rows do not fit.
+// that the digits of eight rows do not fit; at last with a shorter ring beside them.
 template <int CT>
 int launch_rows(ann_stream stream, LinearQ4Args& a, bool vec) {
+    using Longest = Q4<1, 1, 2>;
     int64_t const quads = ceil_div(a.K, 128);
-    if (quads > Q4<CT, 1>::MAX_QUADS)
-        return fail(ANN_ENOTSUP, "linearQ4: more than %lld inputs.", static_cast<long long>(128 * Q4<CT, 1>::MAX_QUADS));
-    if (a.M <= 2 || quads > Q4<CT, 2>::MAX_QUADS) return launch_vec<CT, 1>(stream, a, vec);
-    if (a.M <= 4 || quads > Q4<CT, 4>::MAX_QUADS) return launch_vec<CT, 2>(stream, a, vec);
+    if (quads > kMaxCluster * Longest::LEAST)
+        return fail(ANN_ENOTSUP, "linearQ4: more than %lld inputs.", static_cast<long long>(128 * kMaxCluster * Longest::LEAST));
+    if (quads > kMaxCluster * Q4<CT, 1>::LEAST) return launch_vec<1, 1, 2>(stream, a, vec);
+    if (a.M <= 2 || quads > kMaxCluster * Q4<CT, 2>::LEAST) return launch_vec<CT, 1>(stream, a, vec);
+    if (a.M <= 4 || quads > kMaxCluster * Q4<CT, 4>::LEAST) return launch_vec<CT, 2>(stream, a, vec);
     return launch_vec<CT, 4>(stream, a, vec);
 }
 
