@@ -9,6 +9,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <array>
 #include <cmath>
 #include <map>
 #include <mutex>
@@ -970,30 +971,56 @@ int prepare(K kernel, size_t smem, bool wide_cluster, std::set<int>& ready, std:
 
 // One launch, a cluster of CTAs per KV head: for calls of little work.
 template <int D, int R>
-int launch_cluster(ann_stream stream, DecodeQ8Args& a, int64_t units) {
-    constexpr int W = 4;
+struct Clusters {
+    static constexpr int W = 4;
     using C = Q8<D, R, W>;
-    auto const kernel = decode_q8_kernel<D, R, W, false>;
-    static std::mutex mu;
-    static std::set<int> ready;
-    ANN_TRY(prepare(kernel, C::SMEM, true, ready, mu));
-    int64_t const grid = units * a.splits;
-    if (grid > INT32_MAX) return fail(ANN_ENOTSUP, "attentionDecodeQ8: grid too large.");
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = static_cast<unsigned>(a.splits);
-    attr.val.clusterDim.y = 1;
-    attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(grid));
-    cfg.blockDim = dim3(C::THREADS);
-    cfg.dynamicSmemBytes = C::SMEM;
-    cfg.stream = as_stream(stream);
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, kernel, a);
-    return check_launch("attentionDecodeQ8");
-}
+
+    explicit Clusters(int splits) {
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = static_cast<unsigned>(splits);
+        attr.val.clusterDim.y = 1;
+        attr.val.clusterDim.z = 1;
+        cfg.gridDim = dim3(static_cast<unsigned>(splits));
+        cfg.blockDim = dim3(C::THREADS);
+        cfg.dynamicSmemBytes = C::SMEM;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+    }
+    Clusters(Clusters const&) = delete;
+
+    // Clusters of 1 .. kMaxCluster CTAs that the device holds at once.
+    static int room(const std::array<int, kMaxCluster + 1>*& out) {
+        static std::mutex mu;
+        static std::set<int> ready;
+        static std::map<int, std::array<int, kMaxCluster + 1>> rooms;
+        auto const kernel = decode_q8_kernel<D, R, W, false>;
+        ANN_TRY(prepare(kernel, C::SMEM, true, ready, mu));
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess) return fail(ANN_ECUDA, "attentionDecodeQ8: no CUDA device.");
+        std::lock_guard<std::mutex> lock(mu);
+        auto it = rooms.find(dev);
+        if (it == rooms.end()) {
+            std::array<int, kMaxCluster + 1> r{};
+            for (int s = 1; s <= kMaxCluster; ++s) {
+                Clusters of(s);
+                cudaError_t const e = cudaOccupancyMaxActiveClusters(&r[s], kernel, &of.cfg);
+                if (e != cudaSuccess) return fail(ANN_ECUDA, "attentionDecodeQ8 setup: %s", cudaGetErrorString(e));
+            }
+            it = rooms.emplace(dev, r).first;
+        }
+        out = &it->second;
+        return ANN_OK;
+    }
+    int launch(ann_stream stream, const DecodeQ8Args& a, int64_t units) {
+        if (units * a.splits > INT32_MAX) return fail(ANN_ENOTSUP, "attentionDecodeQ8: grid too large.");
+        cfg.gridDim = dim3(static_cast<unsigned>(units * a.splits));
+        cfg.stream = as_stream(stream);
+        cudaLaunchKernelEx(&cfg, decode_q8_kernel<D, R, W, false>, a);
+        return check_launch("attentionDecodeQ8");
+    }
+};
 
 // Even shares of all keys for as many CTAs as fit the GPU, then the merge of the
 // rows that several CTAs share.
@@ -1048,15 +1075,18 @@ int launch(ann_stream stream, DecodeQ8Args& a) {
     int64_t const units = a.B * a.Hkv * a.row_tiles, tiles = ceil_div(a.cap, C::KT);
     if (units > INT32_MAX) return fail(ANN_ENOTSUP, "attentionDecodeQ8: grid too large.");
     double const slots = static_cast<double>(sm_count()) * C::PER_SM, all = static_cast<double>(units) * tiles;
+    const std::array<int, kMaxCluster + 1>* room = nullptr;
+    ANN_TRY((Clusters<D, R>::room(room)));
     double best = 1e300;
     for (int s = 1; s <= kMaxCluster && (s == 1 || (s - 1) * 4 < tiles); ++s) {
+        if ((*room)[s] == 0) continue;
         double const ctas = static_cast<double>(units) * s, full = std::min(1.0, ctas / slots);
-        double const cost = std::ceil(ctas / slots) * (std::ceil(tiles / (4.0 * s)) * std::max(0.45, 0.3 + 0.7 * full) + 1.0);
+        double const cost = std::ceil(static_cast<double>(units) / (*room)[s]) * (std::ceil(tiles / (4.0 * s)) * std::max(0.45, 0.3 + 0.7 * full) + 1.0);
         if (cost < best) best = cost, a.splits = s;
     }
     // the shares' tiles are counted in 32 bits
     double const shares = all > INT32_MAX / 2 ? 1e300 : all / (4.0 * slots) + 1.5 * (2.0 + static_cast<double>(units) / slots);
-    if (best <= shares) return launch_cluster<D, R>(stream, a, units);
+    if (best <= shares) return Clusters<D, R>(a.splits).launch(stream, a, units);
     return launch_shares<D, R>(stream, a, units);
 }
 

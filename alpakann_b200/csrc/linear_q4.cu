@@ -517,8 +517,8 @@ int launch(ann_stream stream, LinearQ4Args& a) {
     if (tiles > INT32_MAX || row_tiles > 65535) return fail(ANN_ENOTSUP, "linearQ4: grid too large.");
     a.ends = a.group == 32 ? 4 : a.group % 128 == 0 ? 1 : 2;
     // How many warps of a CTA and CTAs of a cluster share the inputs: the least of
-    // these estimates (us, fitted to 14 shapes at 64 choices each; the estimate's best is
-    // within 3 % of the measured best there). A quad takes a warp its memory's latency
+    // these estimates (us, fitted to 20 shapes at up to 36 choices each; the estimate's
+    // best is within 3 % of the measured best there). A quad takes a warp its memory's latency
     // with two in flight, or its turn among the SM's warps; preparing a quad's digits,
     // and what a set of tiles costs to sum and store, count beside it. (8 x 4096 x
     // 16384: two by two 19 us, all eight warps of two CTAs 23, one of four 20; 1 x 4096 x
@@ -539,10 +539,10 @@ int launch(ann_stream stream, LinearQ4Args& a) {
             // as many clusters as fit the GPU at once, each with the same number of sets or one less
             int64_t const at_once = std::max<int64_t>(1, most / row_tiles), sets = ceil_div(tiles, across);
             int64_t const rounds = ceil_div(sets, at_once), used = ceil_div(sets, rounds);
-            double const load = std::min<double>(need <= kHalfSmem && NT * CT < 4 ? 2 : 1, static_cast<double>(ceil_div(used * splits * row_tiles, sm_count())));
-            double const quad = std::max(0.8, kWarps * load * (0.02 + 0.0225 * NT) * CT);
+            int const load = need <= kHalfSmem && NT * CT < 4 && used * row_tiles > (*room)[0][splits] ? 2 : 1;  // CTAs of an SM
+            double const quad = std::max(0.8 + 0.1 * a.ends, kWarps * load * (0.017 + 0.0275 * NT + 0.003 * a.ends) * CT);
             double const prepare = (0.3 + 0.1 * NT) * load * static_cast<double>(in_cta) / kWarps;
-            double const finish = 1.5 + 0.06 * NT * CT * across * load + (splits > 1 ? 0.4 : 0.0);
+            double const finish = 1.5 + 0.06 * NT * CT * across * load + (splits > 1 ? 0.4 + 0.05 * splits : 0.0);
             double const cost = prepare + static_cast<double>(rounds) * (static_cast<double>(in_warp) * quad + finish);
             if (cost >= best) continue;
             best = cost;
