@@ -860,27 +860,46 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(DecodeQ8Args a,
 #pragma unroll
     for (int i = 0; i < LV; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (given) {
-        for (int k = lane; k < parts; k += 32) top = fmaxf(top, stats[slot(k) * 2 * ROWS + r]);
+        // Parts are loaded AT_ONCE at a time, the first ones together with the statistics.
+        constexpr int AT_ONCE = 8 / LV, HELD = 4;
+        float m[AT_ONCE];
+        float4 y[AT_ONCE][LV];
+        auto load = [&](int k0) {
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                int const k = k0 + u * wpr;
+                int64_t const sl = slot(min(k, parts - 1));
+                if (k < parts) {
+                    m[u] = stats[sl * 2 * ROWS + r];
+                    float4 const* po = reinterpret_cast<float4 const*>(a.parts) + (sl * ROWS + r) * (D / 4);
+#pragma unroll
+                    for (int i = 0; i < LV; ++i) y[u][i] = po[min(32 * i + lane, D / 4 - 1)];
+                }
+            }
+        };
+        if (sub < parts) load(sub);
+        float pm[HELD], pl[HELD];  // of parts lane + 32 e
+#pragma unroll
+        for (int e = 0; e < HELD; ++e) {
+            bool const in = lane + 32 * e < parts;
+            float const* ps = stats + slot(in ? lane + 32 * e : 0) * 2 * ROWS + r;
+            pm[e] = in ? ps[0] : neg_inf(0.0f);
+            pl[e] = in ? ps[ROWS] : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < HELD; ++e) top = fmaxf(top, pm[e]);
+        for (int k = lane + 32 * HELD; k < parts; k += 32) top = fmaxf(top, stats[slot(k) * 2 * ROWS + r]);
         top = warp_max(top);
         auto weight = [&](float m) { return top == neg_inf(0.0f) ? 0.0f : exp2_neg(m - top); };
-        for (int k = lane; k < parts; k += 32) {
+#pragma unroll
+        for (int e = 0; e < HELD; ++e) l = fmaf(weight(pm[e]), pl[e], l);
+        for (int k = lane + 32 * HELD; k < parts; k += 32) {
             float const* ps = stats + slot(k) * 2 * ROWS + r;
             l = fmaf(weight(ps[0]), ps[ROWS], l);
         }
         l = warp_sum(l);
-        constexpr int AT_ONCE = 4;  // parts whose loads go out together
         for (int k0 = sub; k0 < parts; k0 += AT_ONCE * wpr) {
-            float m[AT_ONCE];
-            float4 y[AT_ONCE][LV];
-#pragma unroll
-            for (int u = 0; u < AT_ONCE; ++u) {
-                int const k = min(k0 + u * wpr, parts - 1);
-                int64_t const sl = slot(k);
-                m[u] = k0 + u * wpr < parts ? stats[sl * 2 * ROWS + r] : neg_inf(0.0f);
-                float4 const* po = reinterpret_cast<float4 const*>(a.parts) + (sl * ROWS + r) * (D / 4);
-#pragma unroll
-                for (int i = 0; i < LV; ++i) y[u][i] = po[min(32 * i + lane, D / 4 - 1)];
-            }
+            if (k0 != sub) load(k0);
 #pragma unroll
             for (int u = 0; u < AT_ONCE; ++u) {
                 if (k0 + u * wpr >= parts) break;
