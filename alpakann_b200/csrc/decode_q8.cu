@@ -1078,7 +1078,8 @@ int launch_shares(ann_stream stream, DecodeQ8Args& a, int64_t units) {
 
 // Which way, and how many splits: the least of these costs, in tiles' times of a
 // warp on a full SM (2.2 us for 8 KB: 12 warps share an SM's part of HBM).
-//  * Clusters of S: rounds of CTAs, each ceil(tiles / 4 S) tiles a warp and about
+//  * Clusters of S: rounds of as many as the device holds at once (of six CTAs, two an
+//    SM, 45 and not 49), each ceil(tiles / 4 S) tiles a warp and about
 //    one tile's time to start and to merge. A tile takes less where the grid
 //    does not fill the GPU, though not in proportion, and no less than 0.45.
 //  * Even shares: their tiles a warp, and about 1.5 tiles' times for the second
@@ -1087,33 +1088,69 @@ int launch_shares(ann_stream stream, DecodeQ8Args& a, int64_t units) {
 // 36; 12 x 4096 keys of 64, 4 heads, four tokens 15 / 21; 31 x 7345 keys of 64, 6
 // heads 41 / 46; 16 x 32768 keys, 8 heads 183 / 173; 1 x 131072 keys, 4 heads 76 / 39.
 template <int D, int R>
-int launch(ann_stream stream, DecodeQ8Args& a) {
+struct Plan {
     using C = Q8<D, R, 4>;
-    if (a.Tq > INT32_MAX / 2 / int64_t{a.g}) return fail(ANN_ENOTSUP, "attentionDecodeQ8: more than 2^30 rows.");
-    a.row_tiles = ceil_div(a.Tq * a.g, C::ROWS);
-    int64_t const units = a.B * a.Hkv * a.row_tiles, tiles = ceil_div(a.cap, C::KT);
-    if (units > INT32_MAX) return fail(ANN_ENOTSUP, "attentionDecodeQ8: grid too large.");
-    double const slots = static_cast<double>(sm_count()) * C::PER_SM, all = static_cast<double>(units) * tiles;
-    const std::array<int, kMaxCluster + 1>* room = nullptr;
-    ANN_TRY((Clusters<D, R>::room(room)));
-    double best = 1e300;
-    for (int s = 1; s <= kMaxCluster && (s == 1 || (s - 1) * 4 < tiles); ++s) {
-        if ((*room)[s] == 0) continue;
-        double const ctas = static_cast<double>(units) * s, full = std::min(1.0, ctas / slots);
-        double const cost = std::ceil(static_cast<double>(units) / (*room)[s]) * (std::ceil(tiles / (4.0 * s)) * std::max(0.45, 0.3 + 0.7 * full) + 1.0);
-        if (cost < best) best = cost, a.splits = s;
+    int64_t row_tiles = 0, units = 0;
+    int splits = 0;      // 0: even shares
+    double cost = 1e300;
+
+    int make(const DecodeQ8Args& a) {
+        row_tiles = ceil_div(a.Tq * a.g, C::ROWS);
+        units = a.B * a.Hkv * row_tiles;
+        int64_t const tiles = ceil_div(a.cap, C::KT);
+        if (units > INT32_MAX) return fail(ANN_ENOTSUP, "attentionDecodeQ8: grid too large.");
+        double const slots = static_cast<double>(sm_count()) * C::PER_SM, all = static_cast<double>(units) * tiles;
+        const std::array<int, kMaxCluster + 1>* room = nullptr;
+        ANN_TRY((Clusters<D, R>::room(room)));
+        for (int s = 1; s <= kMaxCluster && (s == 1 || (s - 1) * 4 < tiles); ++s) {
+            if ((*room)[s] == 0) continue;
+            double const full = std::min(1.0, static_cast<double>(units) * s / slots);
+            double const c = std::ceil(static_cast<double>(units) / (*room)[s]) *
+                             (std::ceil(tiles / (4.0 * s)) * std::max(0.45, 0.3 + 0.7 * full) + 1.0);
+            if (c < cost) cost = c, splits = s;
+        }
+        // the shares' tiles are counted in 32 bits
+        double const shares = all > INT32_MAX / 2 ? 1e300 : all / (4.0 * slots) + 1.5 * (2.0 + static_cast<double>(units) / slots);
+        if (shares < cost) cost = shares, splits = 0;
+        return ANN_OK;
     }
-    // the shares' tiles are counted in 32 bits
-    double const shares = all > INT32_MAX / 2 ? 1e300 : all / (4.0 * slots) + 1.5 * (2.0 + static_cast<double>(units) / slots);
-    if (best <= shares) return Clusters<D, R>(a.splits).launch(stream, a, units);
-    return launch_shares<D, R>(stream, a, units);
+    int launch(ann_stream stream, DecodeQ8Args& a) const {
+        a.row_tiles = row_tiles;
+        a.splits = std::max(1, splits);
+        return splits > 0 ? Clusters<D, R>(splits).launch(stream, a, units) : launch_shares<D, R>(stream, a, units);
+    }
+};
+
+template <int D, int R>
+int launch(ann_stream stream, DecodeQ8Args& a) {
+    Plan<D, R> plan;
+    ANN_TRY(plan.make(a));
+    return plan.launch(stream, a);
 }
 
+// Query rows of a CTA. Sixteen read the cache half as often as eight, but a tile takes
+// a warp 1.1 times as long, the start and the end one microsecond (0.6 tiles) more, and
+// their registers leave 8 warps an SM instead of 12 (16 x 16384 keys of 64, 8 heads of
+// sixteen rows: 90 us against 111; 12 x 4096, 4 heads: 17.0 against 15.9; 1 x 300, 3
+// heads: 6.7 against 5.3). Heads of 256 take eight: sixteen rows' fragments leave no
+// registers for q's (2 x 65536 keys, 2 heads of sixteen rows: 76 us against 53; 16 x
+// 8192, 4 heads: 85 against 93).
 template <int D>
 int launch_rows(ann_stream stream, DecodeQ8Args& a) {
-    if constexpr (D <= 128)
-        if (a.Tq * a.g <= 4) return launch<D, 4>(stream, a);
-    return a.Tq * a.g <= 8 ? launch<D, 8>(stream, a) : launch<D, 16>(stream, a);
+    if (a.Tq > INT32_MAX / 2 / int64_t{a.g}) return fail(ANN_ENOTSUP, "attentionDecodeQ8: more than 2^30 rows.");
+    int64_t const rows = a.Tq * a.g;
+    if constexpr (D <= 128) {
+        if (rows <= 4) return launch<D, 4>(stream, a);
+        if (rows > 8) {
+            Plan<D, 8> eight;
+            Plan<D, 16> sixteen;
+            ANN_TRY(eight.make(a));
+            ANN_TRY(sixteen.make(a));
+            if (1.1 * sixteen.cost + 0.6 <= eight.cost) return sixteen.launch(stream, a);
+            return eight.launch(stream, a);
+        }
+    }
+    return launch<D, 8>(stream, a);
 }
 
 int decode_q8(ann_stream stream, const ann_view* q_v, const ann_view* k_v, const ann_view* v_v, const ann_view* ks_v,
