@@ -63,7 +63,7 @@ struct DecodeQ8Args {
 // halves, 24.8 in digits. With eight rows the int32 sums take 128 registers a thread
 // and leave 8 warps an SM: 16 x 32768 keys, 64/8 heads 169 us in halves, 176 in
 // digits.)
-// With more rows, and with heads of 256, p.v runs in halves: a cached value is exact
+// With more rows (and eight at most with heads of 256) p.v runs in halves: a cached value is exact
 // in fp16, a probability is the sum of two fp16 parts (22 bits), and
 // mma.sync.m16n8k16 adds the exact products in fp32, both parts of eight rows in one
 // product, from a fresh accumulator for each tile, so that no sum of more than KT
@@ -1084,9 +1084,9 @@ int launch_shares(ann_stream stream, DecodeQ8Args& a, int64_t units) {
 //    does not fill the GPU, though not in proportion, and no less than 0.45.
 //  * Even shares: their tiles a warp, and about 1.5 tiles' times for the second
 //    launch and for each part of a KV head that a CTA meets.
-// Measured (us, clusters at their best S / shares): 8 x 2048 keys, 32 KV heads 32 /
-// 36; 12 x 4096 keys of 64, 4 heads, four tokens 15 / 21; 31 x 7345 keys of 64, 6
-// heads 41 / 46; 16 x 32768 keys, 8 heads 183 / 173; 1 x 131072 keys, 4 heads 76 / 39.
+// Measured (us, clusters at their best S / shares): 8 x 2048 keys, 32 KV heads 25 /
+// 39; 12 x 4096 keys of 64, 4 heads, four tokens 16 / 20; 31 x 7345 keys of 64, 6
+// heads 36 / 43; 16 x 32768 keys, 8 heads 178 / 169; 1 x 131072 keys, 4 heads 72 / 36.
 template <int D, int R>
 struct Plan {
     using C = Q8<D, R, 4>;

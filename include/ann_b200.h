@@ -569,8 +569,8 @@ int ann_pack_weight_q4_f32(ann_stream stream, const ann_view* weight, const ann_
  * fp32 accuracy, inputs to 2^-31 of the largest of their row; a NaN or infinity in
  * a row of the input makes that row's sums NaN (relu makes 0 of them, as elsewhere).
  * Meant for the few rows of a decode step:
- * the weights are read once for every eight rows, up to 57344 inputs (for four rows up
- * to 129024, else two). ANN_ENOTSUP for K > 260096 and for more than 131070 rows. */
+ * the weights are read once for every eight rows, up to 51200 inputs (for four rows up
+ * to 122880, else two). ANN_ENOTSUP for K > 364544 and for more than 131070 rows. */
 int ann_linear_q4_f32(ann_stream stream, const ann_view* input, const ann_view* packed, const ann_view* scales,
                       const ann_view* bias, const ann_view* residual, const ann_view* output, uint32_t group_size,
                       int32_t act);

@@ -24,7 +24,7 @@ def nn():
 
 @pytest.mark.parametrize("M,K,N,group", [(8, 57344, 40, 128), (8, 57472, 40, 128), (5, 130000, 33, 64),
                                          (3, 240000, 36, 4096), (1, 253952, 36, 32), (11, 58368, 2048, 128),
-                                         (2, 253952, 2048, 128)])
+                                         (2, 253952, 2048, 128), (1, 364544, 36, 32), (3, 300000, 2052, 96)])
 def test_linear_many_inputs(nn, M, K, N, group):
     """Rows that do not fit a CTA's memory eight at a time are taken fewer at a
     time. The sums in 64 bits are formed on the device, columns in slices."""
@@ -63,6 +63,13 @@ def test_attention_groups_past_the_heads(nn, group):
     nn.attentionDecodeQ8(None, None, q, kc, vc, ks, vs, want, 16, queriesPerKvGroup=6)
     nn.attentionDecodeQ8(None, None, q, kc, vc, ks, vs, out, 16, queriesPerKvGroup=group)
     assert torch.equal(out, want) and want.isfinite().all()
+
+
+@pytest.mark.parametrize("B,Tq,g_,Hkv,D,T", [(2, 5, 5, 8, 128, 4096), (4, 4, 4, 4, 64, 16384), (2, 8, 2, 2, 128, 60000)])
+def test_attention_many_rows_of_a_head(nn, B, Tq, g_, Hkv, D, T):
+    """Sixteen rows a CTA, in clusters and in even shares."""
+    from tests.test_gpu_q8 import run_attend
+    run_attend(nn, B, Tq, g_, Hkv, D, T, 64, [T - 37 * b for b in range(B)])
 
 
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
