@@ -84,10 +84,12 @@ BINDING = os.path.join(OUT_DIR, "_ann_binding.so")
 def build_binding() -> str:
     """The CPython module of the short calls (binding/binding.c), next to the
     library it links, for the interpreter that runs this build."""
+    import importlib.util
     import sysconfig
+    torch = importlib.util.find_spec("torch").submodule_search_locations[0]
     if _stale(BINDING, [BINDING_SRC, __file__, os.path.join(INCLUDE, "ann_b200.h")]):
         cmd = [cxx().replace("g++", "gcc"), "-O2", "-Wall", "-fPIC", "-shared", "-I", INCLUDE, "-I",
-               sysconfig.get_paths()["include"], BINDING_SRC, "-o", BINDING, "-L", OUT_DIR, "-lann_b200",
+               sysconfig.get_paths()["include"], "-I", os.path.join(torch, "include"), BINDING_SRC, "-o", BINDING, "-L", OUT_DIR, "-lann_b200",
                "-Wl,-rpath,$ORIGIN"]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:

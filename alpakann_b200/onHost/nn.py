@@ -297,7 +297,8 @@ class RotaryPairs(enum.IntEnum):
     halves = 1       # (p, p + P), P = number of frequencies
 
 
-binding.types(torch.float32, torch.float64, torch.int8, torch.int32, torch.uint32)
+binding.setup(torch.Tensor, torch._C._cuda_getDevice)
+_MISMATCH, _ELSEWHERE = -1, -3  # the binding called nothing
 
 
 def _refuse(name, dtypes, tensors):
@@ -319,23 +320,23 @@ def _refuse(name, dtypes, tensors):
     raise TypeError(f"{name}: a tensor of more than 8 dimensions, or an argument that is no tensor")
 
 
-def _run(name, entry, dtypes, queue, tensors, *scalars):
-    """One call of the binding on `queue`, or on the current stream of the tensors'
-    device (the first tensor's; the binding refuses others)."""
+def _again(rc, name, entry, dtypes, queue, tensors, *scalars):
+    """A call of the binding that is not on the current stream of the current device
+    with fitting tensors: words its error, or calls it on `queue` or on the current
+    stream of the tensors' device."""
+    if rc > 0:
+        check(rc)
     values = tensors.values()
     dev = next(iter(values)).get_device()
-    if queue is None:
-        stream = torch._C._cuda_getCurrentRawStream(dev) if dev >= 0 else 0
-    else:
-        stream = handle(queue)
+    if queue is not None:
         if isinstance(queue, torch.cuda.Stream) and queue.device.index != dev and dev >= 0:
             raise ValueError(f"{name}: the stream is on {queue.device}, the tensors on cuda:{dev}")
-    if dev < 0 or torch._C._cuda_getDevice() == dev:
-        rc = entry(stream, *values, *scalars)
-    else:
-        with torch.cuda.device(dev):
-            rc = entry(stream, *values, *scalars)
-    if rc == -1:
+        queue = handle(queue)
+    if dev < 0:
+        _refuse(name, dtypes, tensors)
+    with torch.cuda.device(dev):
+        rc = entry(queue, *values, *scalars)
+    if rc < 0:
         _refuse(name, dtypes, tensors)
     check(rc)
 
@@ -365,11 +366,15 @@ def rotary(queue, exec, q, k, positions, frequencies, outQ, outK, pairs=RotaryPa
     int32 [B,T] or [T]; frequencies: float64, P <= D/2 pairs; elements from 2P
     on are copied. inverse applies the transposed rotation: the gradients of q
     and k from those of outQ and outK."""
-    if q.dtype not in _ROTARY_TYPES:
-        suffix(q)
-    _run("rotary", binding.rotary_f32 if q.dtype == torch.float32 else binding.rotary_f64, _ROTARY_TYPES[q.dtype],
-         queue, {"q": q, "k": k, "positions": positions, "frequencies": frequencies, "outQ": outQ, "outK": outK},
-         int(pairs), int(layout), float(magnitude), 1 if inverse else 0)
+    entry = binding.rotary_f64 if q.dtype == torch.float64 else binding.rotary_f32
+    rc = _ELSEWHERE if queue is not None else entry(None, q, k, positions, frequencies, outQ, outK, pairs, layout,
+                                                    magnitude, inverse)
+    if rc:
+        if q.dtype not in _ROTARY_TYPES:
+            suffix(q)
+        _again(rc, "rotary", entry, _ROTARY_TYPES[q.dtype], queue,
+               {"q": q, "k": k, "positions": positions, "frequencies": frequencies, "outQ": outQ, "outK": outK},
+               pairs, layout, magnitude, inverse)
 
 
 _CACHE_TYPES = {"kCache": torch.int8, "vCache": torch.int8, "positions": torch.int32, "counts": torch.int32,
@@ -383,9 +388,12 @@ def kvCacheAppendQ8(queue, exec, kNew, vNew, kCache, vCache, kScale, vScale, pos
     defaults to Tn). kScale, vScale: float32 [B, Hkv, ceil(Tcap /
     tokensPerScale)], one scale per head and block of tokens; a block whose
     scale grows has its earlier tokens rounded anew."""
-    _run("kvCacheAppendQ8", binding.kv_cache_append_q8, _CACHE_TYPES, queue,
-         {"kNew": kNew, "vNew": vNew, "kCache": kCache, "vCache": vCache, "kScale": kScale, "vScale": vScale,
-          "positions": positions, "counts": counts}, int(tokensPerScale), int(kvLayout))
+    rc = _ELSEWHERE if queue is not None else binding.kv_cache_append_q8(
+        None, kNew, vNew, kCache, vCache, kScale, vScale, positions, counts, tokensPerScale, kvLayout)
+    if rc:
+        _again(rc, "kvCacheAppendQ8", binding.kv_cache_append_q8, _CACHE_TYPES, queue,
+               {"kNew": kNew, "vNew": vNew, "kCache": kCache, "vCache": vCache, "kScale": kScale, "vScale": vScale,
+                "positions": positions, "counts": counts}, tokensPerScale, kvLayout)
 
 
 def kvCacheReadQ8(queue, exec, kCache, vCache, kScale, vScale, kOut, vOut, tokensPerScale, lengths=None,
@@ -393,9 +401,12 @@ def kvCacheReadQ8(queue, exec, kCache, vCache, kScale, vScale, kOut, vOut, token
     """The float32 rows that an 8-bit cache stands for, for the tokens before
     lengths[b] (int32 [B], default all of kOut); rows behind are left as they
     were. Feeds attentionPrefill with a cached prefix."""
-    _run("kvCacheReadQ8", binding.kv_cache_read_q8, _CACHE_TYPES, queue,
-         {"kCache": kCache, "vCache": vCache, "kScale": kScale, "vScale": vScale, "kOut": kOut, "vOut": vOut,
-          "lengths": lengths}, int(tokensPerScale), int(kvLayout))
+    rc = _ELSEWHERE if queue is not None else binding.kv_cache_read_q8(
+        None, kCache, vCache, kScale, vScale, kOut, vOut, lengths, tokensPerScale, kvLayout)
+    if rc:
+        _again(rc, "kvCacheReadQ8", binding.kv_cache_read_q8, _CACHE_TYPES, queue,
+               {"kCache": kCache, "vCache": vCache, "kScale": kScale, "vScale": vScale, "kOut": kOut, "vOut": vOut,
+                "lengths": lengths}, tokensPerScale, kvLayout)
 
 
 def attentionDecodeQ8(queue, exec, Q, kCache, vCache, kScale, vScale, out, tokensPerScale, lengths=None, scale=None,
@@ -407,9 +418,12 @@ def attentionDecodeQ8(queue, exec, Q, kCache, vCache, kScale, vScale, out, token
     to 1/sqrt(D)."""
     if scale is None:
         scale = 1.0 / math.sqrt(Q.shape[3])
-    _run("attentionDecodeQ8", binding.attention_decode_q8, _CACHE_TYPES, queue,
-         {"Q": Q, "kCache": kCache, "vCache": vCache, "kScale": kScale, "vScale": vScale, "lengths": lengths,
-          "out": out}, float(scale), int(queriesPerKvGroup), int(tokensPerScale), int(kvLayout), 1 if causal else 0)
+    rc = _ELSEWHERE if queue is not None else binding.attention_decode_q8(
+        None, Q, kCache, vCache, kScale, vScale, lengths, out, scale, queriesPerKvGroup, tokensPerScale, kvLayout, causal)
+    if rc:
+        _again(rc, "attentionDecodeQ8", binding.attention_decode_q8, _CACHE_TYPES, queue,
+               {"Q": Q, "kCache": kCache, "vCache": vCache, "kScale": kScale, "vScale": vScale, "lengths": lengths,
+                "out": out}, scale, queriesPerKvGroup, tokensPerScale, kvLayout, causal)
 
 
 def packWeightQ4(queue, exec, weight, packed, scales, groupSize):
@@ -433,9 +447,12 @@ def linearQ4(queue, exec, input, packed, scales, output, groupSize, bias=None, a
     """output = activation(input . W + bias) + residual with W in 4 bits
     (packWeightQ4): linear, linearBias and outputProjectionResidual for the few
     rows of a decode step. residual may be output."""
-    _run("linearQ4", binding.linear_q4, _LINEAR_TYPES, queue,
-         {"input": input, "packed": packed, "scales": scales, "bias": bias, "residual": residual, "output": output},
-         int(groupSize), int(activation))
+    rc = _ELSEWHERE if queue is not None else binding.linear_q4(
+        None, input, packed, scales, bias, residual, output, groupSize, activation)
+    if rc:
+        _again(rc, "linearQ4", binding.linear_q4, _LINEAR_TYPES, queue,
+               {"input": input, "packed": packed, "scales": scales, "bias": bias, "residual": residual,
+                "output": output}, groupSize, activation)
 
 
 def raise_shape(msg):

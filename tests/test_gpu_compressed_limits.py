@@ -125,3 +125,29 @@ def test_first_call_of_a_process_is_captured(nn):
     """Kernel attributes and the scratch pool are made under the capture."""
     r = subprocess.run([sys.executable, "-c", CAPTURED_FIRST], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "equal" in r.stdout, r.stdout + r.stderr
+
+
+def test_streams_devices_and_leaves(nn):
+    """The current stream by default, a given one as a queue, and tensors that require gradients."""
+    x, w, s = torch.randn(1, 4096, device="cuda"), torch.randint(0, 2**31, (512, 512), dtype=torch.int32, device="cuda"), \
+        torch.rand(32, 512, device="cuda")
+    want = torch.zeros(1, 512, device="cuda")
+    nn.linearQ4(None, None, x, w, s, want, 128)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for queue in (None, side, side.cuda_stream):
+        out = torch.zeros_like(want)
+        late = x.clone().zero_()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):  # the input comes late on the side stream
+            torch.cuda._sleep(10_000_000)
+            late.copy_(x)
+            if queue is None:
+                nn.linearQ4(None, None, late, w, s, out, 128)
+        if queue is not None:
+            nn.linearQ4(queue, None, late, w, s, out, 128)
+        side.synchronize()
+        assert torch.equal(out, want)
+    leaf, out = torch.nn.Parameter(x), torch.zeros_like(want)
+    nn.linearQ4(None, None, leaf, w, s, out, 128)
+    assert torch.equal(out, want)
