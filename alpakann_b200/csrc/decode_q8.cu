@@ -16,6 +16,7 @@
 #include <set>
 
 #include "common.cuh"
+#include "overlap.cuh"
 #include "pairs.cuh"
 #include "reduce.cuh"
 #include "tma.cuh"
@@ -264,6 +265,8 @@ __global__ void __launch_bounds__(32 * W, Q8<D, R, W>::PER_SM) decode_q8_kernel(
     int const tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     int const split = SHARES ? 0 : static_cast<int>(blockIdx.x) % a.splits;
     if (!SHARES && a.splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // "this CTA runs"
+
+    prior_kernels_done();
 
     int64_t b;            // sequence
     int unit, units = 0;  // KV head and row tile in it
@@ -845,7 +848,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(DecodeQ8Args a,
     int const c0 = n > 0 ? sh.owner(p0) : 0, c1 = n > 0 ? sh.owner(p0 + n - 1) : 0;
     // The shares are done and visible. Every block waits for that, those without work
     // too: this grid's end has to mean that the shares have ended.
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    prior_kernels_done();
     if (n > 0 && c0 == c1) return;  // a whole unit: written by its CTA
     int const rt = static_cast<int>(a.row_tiles), kvh = u / rt;
     uint32_t const row = static_cast<uint32_t>((u - kvh * rt) * ROWS + r);
@@ -994,9 +997,10 @@ struct Clusters {
     static constexpr int W = 4;
     using C = Q8<D, R, W>;
     cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr{};
+    cudaLaunchAttribute attrs[2] = {{}, overlapping()};
 
     explicit Clusters(int splits) {
+        cudaLaunchAttribute& attr = attrs[0];
         attr.id = cudaLaunchAttributeClusterDimension;
         attr.val.clusterDim.x = static_cast<unsigned>(splits);
         attr.val.clusterDim.y = 1;
@@ -1004,8 +1008,8 @@ struct Clusters {
         cfg.gridDim = dim3(static_cast<unsigned>(splits));
         cfg.blockDim = dim3(C::THREADS);
         cfg.dynamicSmemBytes = C::SMEM;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
+        cfg.attrs = attrs;
+        cfg.numAttrs = 2;
     }
     Clusters(Clusters const&) = delete;
 
@@ -1055,21 +1059,14 @@ int launch_shares(ann_stream stream, DecodeQ8Args& a, int64_t units) {
     void* parts = nullptr;
     ANN_TRY(scratch_alloc(&parts, sizeof(float) * 2 * G * (C::ROWS * D + 2 * C::ROWS), as_stream(stream)));
     a.parts = static_cast<float*>(parts);
-    kernel<<<static_cast<unsigned>(G), C::THREADS, C::SMEM, as_stream(stream)>>>(a);
+    launch_overlapping(kernel, dim3(static_cast<unsigned>(G)), C::THREADS, C::SMEM, as_stream(stream), a);
     int rc = check_launch("attentionDecodeQ8");
     if (rc == ANN_OK) {
-        cudaLaunchConfig_t cfg{};
-        cudaLaunchAttribute attr{};
-        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its launch overlaps the shares' end
-        attr.val.programmaticStreamSerializationAllowed = 1;
         // few units: many parts each, so all warps of a block to one row
         int const rows = static_cast<int>(std::min<int64_t>(C::ROWS, a.Tq * a.g)), per_block = units < G / 8 ? 1 : std::min(8, C::ROWS);
-        cfg.gridDim = dim3(static_cast<unsigned>(units), static_cast<unsigned>(ceil_div(rows, per_block)));
-        cfg.blockDim = dim3(32 * kMergeWarps);
-        cfg.stream = as_stream(stream);
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
-        cudaLaunchKernelEx(&cfg, merge_kernel<D, C::ROWS, C::KT>, a, static_cast<int>(G), W, per_block);
+        dim3 const grid(static_cast<unsigned>(units), static_cast<unsigned>(ceil_div(rows, per_block)));
+        launch_overlapping(merge_kernel<D, C::ROWS, C::KT>, grid, 32 * kMergeWarps, 0, as_stream(stream), a,
+                           static_cast<int>(G), W, per_block);
         rc = check_launch("attentionDecodeQ8");
     }
     cudaFreeAsync(parts, as_stream(stream));

@@ -17,6 +17,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "overlap.cuh"
 #include "reduce.cuh"
 
 namespace ann {
@@ -99,6 +100,7 @@ __global__ void __launch_bounds__(kThreads, 5) append_kernel(AppendArgs a) {
     uint32_t const ub = a.heads.div(bhk >> 1);
     int64_t const b = ub, h = (bhk >> 1) - ub * a.heads.d;
 
+    prior_kernels_done();
     int64_t const start = a.pos[b * a.pos_s];
     int64_t count = a.Tn;
     if (a.counts != nullptr) count = min(a.Tn, max(int64_t{0}, static_cast<int64_t>(a.counts[b * a.counts_s])));
@@ -242,6 +244,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(ReadArgs a) {
         t = STEP ? t0 + u * (kThreads / per) : a.row.div(base + u * kThreads);
         col = STEP ? c0 : base + u * kThreads - t * per;
     };
+    prior_kernels_done();
     // All loads of a thread at once, the length among them: rows past it are read
     // (they are part of the cache) and not written.
     int64_t const q_u = STEP ? kThreads / per * c.q_t : 0, o_u = STEP ? kThreads / per * o_t : 0;
@@ -366,7 +369,7 @@ int append(ann_stream stream, const ann_view* kn, const ann_view* vn, const ann_
     a.blocks = FastDiv::make(block);
     if (grid > INT32_MAX) return fail(ANN_ENOTSUP, "kvCacheAppendQ8: grid too large.");
     auto const kernel = kThreads % a.row.d == 0 ? append_kernel<true> : append_kernel<false>;
-    kernel<<<static_cast<unsigned>(grid), kThreads, 0, as_stream(stream)>>>(a);
+    launch_overlapping(kernel, dim3(static_cast<unsigned>(grid)), kThreads, 0, as_stream(stream), a);
     return check_launch(what);
 }
 
@@ -414,7 +417,7 @@ int read_back(ann_stream stream, const ann_view* kc, const ann_view* vc, const a
     bool const step = kThreads % a.row.d == 0;
     auto const kernel = a.vec ? (step ? read_kernel<true, true> : read_kernel<true, false>)
                               : (step ? read_kernel<false, true> : read_kernel<false, false>);
-    kernel<<<static_cast<unsigned>(grid), kThreads, 0, as_stream(stream)>>>(a);
+    launch_overlapping(kernel, dim3(static_cast<unsigned>(grid)), kThreads, 0, as_stream(stream), a);
     return check_launch(what);
 }
 

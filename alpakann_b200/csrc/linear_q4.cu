@@ -15,6 +15,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "overlap.cuh"
 #include "pairs.cuh"
 #include "tma.cuh"
 
@@ -217,6 +218,7 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     open_tile();
+    prior_kernels_done();
 
     // x's digits: every warp prepares an eighth of the CTA's quads (its own, if all
     // warps share a tile). A lane takes an octet of a row at a time, eight steps a warp. First
@@ -482,13 +484,13 @@ template <typename C, int CT, int NT, bool VEC>
 int launch(ann_stream stream, LinearQ4Args& a) {
     auto const kernel = linear_q4_kernel<C, CT, NT, VEC>;
     cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr{};
+    cudaLaunchAttribute attrs[2] = {{}, overlapping()}, &attr = attrs[0];
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.y = 1;
     attr.val.clusterDim.z = 1;
     cfg.blockDim = dim3(kThreads);
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cfg.attrs = attrs;
+    cfg.numAttrs = 2;
     static std::mutex mu;
     static std::map<int, Room> rooms;  // devices whose kernel attributes are set
     int dev = 0;

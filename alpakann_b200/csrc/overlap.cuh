@@ -1,0 +1,34 @@
+// overlap.cuh -- launches whose blocks are set up while the kernel before them in
+// the stream ends. Such a kernel calls prior_kernels_done() in every thread before it
+// touches global memory: until then the writes of earlier kernels may be missing, and
+// memory that they read may not be written.
+#pragma once
+
+#include <cuda_runtime.h>
+
+namespace ann {
+
+__device__ __forceinline__ void prior_kernels_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+inline cudaLaunchAttribute overlapping() {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    return attr;
+}
+
+// One such launch; the error, if any, is the thread's last one.
+template <typename... P, typename... A>
+void launch_overlapping(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream, A... args) {
+    cudaLaunchAttribute attr = overlapping();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
+}  // namespace ann

@@ -18,6 +18,7 @@
 #include <cmath>
 
 #include "common.cuh"
+#include "overlap.cuh"
 #include "reduce.cuh"
 
 namespace ann {
@@ -76,6 +77,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a, T mag) {
     using V = typename Vec16<T>::type;
     constexpr int NV = Vec16<T>::n;
     constexpr int E = 2 * VP;
+    prior_kernels_done();
     int64_t const id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
     if (id >= a.tokens * a.groups) return;
     int64_t const token = id / a.groups, grp = id - token * a.groups;
@@ -249,7 +251,7 @@ int rotary(ann_stream stream, const ann_view* q_v, const ann_view* k_v, const an
         bool const halves = pairs == ANN_ROTARY_HALVES;
         auto const kernel = vec ? (halves ? rotary_kernel<T, NV, true, true> : rotary_kernel<T, NV, true, false>)
                                 : (halves ? rotary_kernel<T, 1, false, true> : rotary_kernel<T, 1, false, false>);
-        kernel<<<grid, kThreads, 0, as_stream(stream)>>>(a, mag);
+        launch_overlapping(kernel, grid, kThreads, 0, as_stream(stream), a, mag);
     }
     return check_launch("rotary");
 }

@@ -151,3 +151,61 @@ def test_streams_devices_and_leaves(nn):
     leaf, out = torch.nn.Parameter(x), torch.zeros_like(want)
     nn.linearQ4(None, None, leaf, w, s, out, 128)
     assert torch.equal(out, want)
+
+
+def test_chained_calls_wait_for_their_inputs(nn):
+    """Every operator right behind the kernel that writes its input, on one stream, replayed, and
+    behind a joined stream: launches overlap the end of the kernels before them, their reads must not."""
+    B, D, T = 2, 128, 2048
+    g = torch.Generator("cuda").manual_seed(2)
+    rnd = lambda *shape: torch.randn(*shape, generator=g, device="cuda")
+    x, w4 = rnd(B, 4096), torch.randint(-2**31, 2**31, (512, 4096), generator=g, device="cuda").to(torch.int32)
+    ws, freq = torch.rand(32, 4096, generator=g, device="cuda") * 0.01, torch.rand(64, dtype=torch.float64, device="cuda")
+    pos, lens = torch.tensor([1900, 7], dtype=torch.int32, device="cuda"), torch.tensor([1901, 8], dtype=torch.int32, device="cuda")
+    kc0, vc0 = (torch.randint(-127, 128, (B, 8, T, D), generator=g, device="cuda").to(torch.int8) for _ in range(2))
+    sc0 = torch.rand(B, 8, T // 64, generator=g, device="cuda") * 0.01
+    kn0 = rnd(B, 1, 8, D)
+    side = torch.cuda.Stream()
+
+    def chain(join, sync):
+        wait = torch.cuda.synchronize if sync else (lambda: None)
+        kc, vc, ks, vs = kc0.clone(), vc0.clone(), sc0.clone(), sc0.clone()
+        y, q, kn, out, back = (torch.zeros(n, device="cuda") for n in (B * 4096, B * 4096, B * 8 * D, B * 4096, 2 * B * 8 * T * D))
+        back = back.view(2, B, 8, T, D)
+        x1 = torch.zeros_like(x)
+        if join:
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                x1.copy_(x)
+            torch.cuda.current_stream().wait_stream(side)
+        else:
+            x1.copy_(x)
+        for _ in range(3):
+            wait()
+            nn.linearQ4(None, None, x1, w4, ws, y.view(B, 4096), 128)
+            wait()
+            nn.rotary(None, None, y.view(B, 1, 32, D), kn0, pos.view(B, 1), freq, q.view(B, 1, 32, D), kn.view(B, 1, 8, D))
+            wait()
+            nn.kvCacheAppendQ8(None, None, kn.view(B, 1, 8, D), kn.view(B, 1, 8, D), kc, vc, ks, vs, pos, 64)
+            wait()
+            nn.attentionDecodeQ8(None, None, q.view(B, 1, 32, D), kc, vc, ks, vs, out.view(B, 1, 32, D), 64, lens,
+                                 queriesPerKvGroup=4)
+            wait()
+            nn.linearQ4(None, None, out.view(B, 4096), w4, ws, x1, 128)
+            wait()
+            nn.kvCacheReadQ8(None, None, kc, vc, ks, vs, back[0], back[1], 64)
+        return x1, out, back
+
+    want = chain(False, True)
+    for join in (False, True):
+        for _ in range(20):
+            got = chain(join, False)
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = chain(join, False)
+        for _ in range(20):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
