@@ -84,10 +84,18 @@ struct DecodeQ8Args {
 // are placed so that both kinds of reads are free of bank conflicts.
 //
 // Every warp keeps a running maximum and sum per row (base 2). Warps meet in
-// shared memory; the CTAs of a
-// cluster (the key range's splits) send their parts into each other's shared
-// memory, where each CTA sums its share of the output: one cluster barrier, no
-// scratch memory, no atomics, one launch, and a fixed order of sums.
+// shared memory; the CTAs of a cluster (the key range's splits) send their parts into
+// each other's shared memory, where each CTA sums its share of the output: one cluster
+// barrier, no scratch memory, no atomics, one launch, and a fixed order of sums. Long
+// caches go in even shares over all CTAs instead, with a second kernel for the parts.
+//
+// Bound by the cache's bytes, 2 D a key and KV head. Measured (us, of the bytes' time
+// at the copy rate): 16 x 32768 keys, 64/8 heads 170 (0.98; 210 with launches back to
+// back for seconds, when the power limit lowers the clock), 8 x 2048, 32/32 24.8 (0.84),
+// 1 x 131072, 32/4 35.5 (0.59: ten rounds of tiles a warp where 9.2 would do, and 5 us
+// for the merge), 12 x 4096 of 64, four tokens, 16/4 12.1 (0.17: the start, and 8 warps'
+// chains of product, maximum, exponential, product), 1 x 300, 32/8 5.2 (launch, two turns
+// of memory, the cluster's barrier).
 constexpr int kMaxCluster = 16;
 constexpr int kMaxShares = 1024;
 constexpr float kLog2e = 1.4426950408889634f;

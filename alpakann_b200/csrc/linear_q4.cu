@@ -70,6 +70,13 @@ __device__ __forceinline__ float activate(float v, int act) {
 // tile meet in shared memory, across a cluster in the CTA that owns a share of the
 // columns, which applies bias, activation and residual. One launch, no scratch
 // memory, no atomics, a fixed order of sums.
+//
+// Bound by the weights' bytes, K N (1/2 + 4 / group), for one row; eight rows' products
+// take the tensor pipes two thirds of the bytes' time, but with two warps a scheduler
+// (256 registers) 0.4 instructions a cycle are issued, and that bounds it. Measured (K x N, groups of 128, us, of the bytes' time at the copy rate): one
+// row 4096 x 65536 27.0 (0.82), 4096 x 16384 10.7 (0.51), 4096 x 4096 5.3 (0.26: launch,
+// digits, one turn of memory); eight rows 4096 x 16384, groups of 64, 18.6 (0.32), 4096 x
+// 65536 55.8 (0.42).
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxCluster = 16;
@@ -678,9 +685,9 @@ int linear_q4(ann_stream stream, const ann_view* x_v, const ann_view* p_v, const
     a.x_vec = a.x_k == 1 && a.x_m % 4 == 0 && aligned(x.data, 16);
     bool const vec = a.w_n == 1 && a.w_r % 4 == 0 && aligned(p.data, 16) && a.s_n == 1 && a.s_g % 4 == 0 &&
                      aligned(s.data, 16) && a.N % 4 == 0;
-    // Few columns: tiles of 32 give twice the CTAs (1024 x 1024, one row: 3.9 us
-    // against 4.2); else 64, whose copies, digits and loops serve twice the weights
-    // (4096 x 65536: 30 us against 34).
+    // Few columns: tiles of 32 give twice the CTAs (1024 x 1024: 3.5 us against 3.7,
+    // eight rows 5.4 against 6.2); else 64, whose copies, digits and loops serve twice
+    // the weights (4096 x 65536: 27.4 us against 31.9; 4096 x 2048: 4.5 against 5.1).
     return a.N < 2048 ? launch_rows<1>(stream, a, vec) : launch_rows<2>(stream, a, vec);
 }
 
