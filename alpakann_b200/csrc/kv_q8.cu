@@ -14,10 +14,11 @@
 //
 // Both are bound by HBM: append reads 4 bytes and writes 1 per value, the
 // read-back reads 1 and writes 4. Measured at 4 x 2048 tokens, 8 heads of 128: append
-// 25 us (0.52 of the bytes' time at the copy rate: the block's largest value has to be
-// known before the first is written, so loads and stores alternate), read-back 28 us (0.69
-// of the bytes of 4 x 3048 tokens); one token of 8 sequences 2.8 and 4.4 us, a launch each.
+// 24 us (0.54 of the bytes' time at the copy rate: the block's largest value has to be
+// known before the first is written, so loads and stores alternate), read-back 23 us (0.84
+// of the bytes of 4 x 3048 tokens); one token of 8 sequences 2.5 and 4.0 us, a launch each.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "overlap.cuh"
@@ -29,7 +30,7 @@ namespace {
 __device__ unsigned int g_kv_q8_error;
 
 constexpr int kThreads = 256;
-constexpr int kHeld = 4;  // 16-byte vectors of a thread kept between append's two passes
+constexpr int kHeld = 8;  // 16-byte vectors of a thread kept between append's two passes
 
 struct CacheTensor {
     int8_t* q;
@@ -49,6 +50,7 @@ struct AppendArgs {
     FastDiv touched, heads;  // blocks a sequence's rows can reach, KV heads
     FastDiv blocks;          // by a block's tokens
     FastDiv row;             // by the items of a row: 4 aligned values (vec) or one
+    int rows;                // whole rows of one item a thread (STEP)
     int vec;
 };
 
@@ -96,7 +98,7 @@ __device__ __forceinline__ int nearest64(double x, double s) {
 
 // STEP: a row's items divide the block's threads, which then step over rows.
 template <bool STEP>
-__global__ void __launch_bounds__(kThreads, 5) append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) append_kernel(AppendArgs const __grid_constant__ a) {
     __shared__ unsigned int red[kThreads / 32];
     uint32_t const bhk = a.touched.div(blockIdx.x), jb = blockIdx.x - bhk * a.touched.d;
     int const kv = static_cast<int>(bhk & 1u);
@@ -114,22 +116,22 @@ __global__ void __launch_bounds__(kThreads, 5) append_kernel(AppendArgs a) {
     int64_t const lo = max(first, j * a.block), hi = min(end, (j + 1) * a.block);
     if (lo >= hi) return;
 
-    CacheTensor const& c = kv ? a.c[1] : a.c[0];
-    float const* x = (kv ? a.x[1] : a.x[0]) + b * (kv ? a.x_b[1] : a.x_b[0]) + h * (kv ? a.x_h[1] : a.x_h[0]);
-    int64_t const x_t = kv ? a.x_t[1] : a.x_t[0], x_d = kv ? a.x_d[1] : a.x_d[0];
+    CacheTensor const& c = a.c[kv];
+    float const* x = a.x[kv] + b * a.x_b[kv] + h * a.x_h[kv];
+    int64_t const x_t = a.x_t[kv], x_d = a.x_d[kv];
     x += (lo - start) * x_t;
     int8_t* q = c.q + b * c.q_b + h * c.q_h;
     float* scale = c.scale + b * c.s_b + h * c.s_h + j * c.s_j;
     int const rows = static_cast<int>(hi - lo), D = static_cast<int>(a.D);
 
     // The first kHeld items of a thread stay in registers between the two passes,
-    // loaded at once; later ones are read again, from L2. (More registers for items
-    // mean fewer CTAs an SM: 8 held 29 us, 4 held 26 us at 4 x 2048 tokens.)
+    // loaded at once; later ones are read again, from L2. (Four held and five blocks an
+    // SM: 27 us, eight and four 24, at 4 x 2048 tokens in blocks of 64.)
     int const per = static_cast<int>(a.row.d), items = rows * per;  // of a row, of the new rows
     int const r0 = static_cast<int>(a.row.div(threadIdx.x)), c0 = static_cast<int>(threadIdx.x) - r0 * per;
     auto place = [&](int u, int& r, int& col) {  // item threadIdx.x + u * kThreads
         if constexpr (STEP) {
-            r = r0 + u * (kThreads / per);
+            r = r0 + u * a.rows;
             col = c0;
         } else {
             int const i = static_cast<int>(threadIdx.x) + u * kThreads;
@@ -138,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, 5) append_kernel(AppendArgs a) {
         }
     };
     int const mine = (items - static_cast<int>(threadIdx.x) + kThreads - 1) / kThreads;  // items of this thread
-    int64_t const x_u = STEP ? kThreads / per * x_t : 0, q_u = STEP ? kThreads / per * c.q_t : 0;
+    int64_t const x_u = STEP ? a.rows * x_t : 0, q_u = STEP ? a.rows * c.q_t : 0;
     float const* const x0 = x + r0 * x_t + 4 * c0;
     int8_t* const q0 = q + (lo + r0) * c.q_t + 4 * c0;
     auto vector = [&](int u) {
@@ -155,7 +157,13 @@ __global__ void __launch_bounds__(kThreads, 5) append_kernel(AppendArgs a) {
         for (int u = 0; u < kHeld; ++u) held[u] = u < mine ? vector(u) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int u = 0; u < kHeld; ++u) raise(held[u]);
-        for (int u = kHeld; u < mine; ++u) raise(vector(u));
+        if constexpr (STEP) {
+            float const* p = x0 + kHeld * x_u;
+#pragma unroll 4
+            for (int u = kHeld; u < mine; ++u, p += x_u) raise(*reinterpret_cast<float4 const*>(p));
+        } else {
+            for (int u = kHeld; u < mine; ++u) raise(vector(u));
+        }
     } else {
         for (int u = 0; u < mine; ++u) {
             int r, col;
@@ -189,9 +197,7 @@ __global__ void __launch_bounds__(kThreads, 5) append_kernel(AppendArgs a) {
     bool const usual = finite && s >= 1e-30f;
     float const inv = 1.0f / s;
     auto round1 = [&](float v) { return usual ? nearest(v, s, inv) : finite ? nearest64(v, s) : 0; };
-    auto write4 = [&](int u, float4 v) {
-        int r, col;
-        place(u, r, col);
+    auto four = [&](float4 v) {
         uint32_t bytes;
         if (usual) {
             bytes = nearest4(v, s, inv);
@@ -199,13 +205,26 @@ __global__ void __launch_bounds__(kThreads, 5) append_kernel(AppendArgs a) {
             char4 const n = make_char4(round1(v.x), round1(v.y), round1(v.z), round1(v.w));
             bytes = *reinterpret_cast<uint32_t const*>(&n);
         }
-        *reinterpret_cast<uint32_t*>(STEP ? q0 + u * q_u : q + (lo + r) * c.q_t + 4 * col) = bytes;
+        return bytes;
+    };
+    auto write4 = [&](int u, float4 v) {
+        int r, col;
+        place(u, r, col);
+        *reinterpret_cast<uint32_t*>(STEP ? q0 + u * q_u : q + (lo + r) * c.q_t + 4 * col) = four(v);
     };
     if (a.vec) {
 #pragma unroll
         for (int u = 0; u < kHeld; ++u)
             if (u < mine) write4(u, held[u]);
-        for (int u = kHeld; u < mine; ++u) write4(u, vector(u));
+        if constexpr (STEP) {
+            float const* p = x0 + kHeld * x_u;
+            int8_t* to = q0 + kHeld * q_u;
+#pragma unroll 2
+            for (int u = kHeld; u < mine; ++u, p += x_u, to += q_u)
+                *reinterpret_cast<uint32_t*>(to) = four(*reinterpret_cast<float4 const*>(p));
+        } else {
+            for (int u = kHeld; u < mine; ++u) write4(u, vector(u));
+        }
     } else {
         for (int u = 0; u < mine; ++u) {
             int r, col;
@@ -222,63 +241,82 @@ struct ReadArgs {
     const int32_t* lengths;  // may be null: every row
     int64_t len_s;
     int64_t D, Tout;
-    FastDiv chunks, heads;  // chunks of kReadItems items per (batch, head), KV heads
+    FastDiv chunks, heads;  // chunks of a thread block's items per (batch, head), KV heads
     FastDiv row, block;     // by the items of a row (4 aligned values, or one), by a block's tokens
+    uint32_t rows;          // whole rows of one item a thread (STEP)
     int vec;
 };
 
-constexpr int kReadEach = 4;  // items of a thread
-constexpr int kReadItems = kThreads * kReadEach;
 
-template <bool VEC, bool STEP>
-__global__ void __launch_bounds__(kThreads) read_kernel(ReadArgs a) {
+constexpr int kReadAtOnce = 4;  // items of a thread whose loads go out together (eight: 23.5 us for 23.0 below)
+
+// Signed byte `at` of w as fp32: its bits with the sign flipped, 128 + n, are the low
+// ones of 2^23 + 128 + n.
+__device__ __forceinline__ float byte_of(uint32_t w, uint32_t at) {
+    return __uint_as_float(__byte_perm(w ^ 0x80808080u, 0x4b000000u, 0x7650 | at)) - 8388736.0f;
+}
+
+// A thread takes EACH items, which share what it computes of its place.
+template <bool VEC, bool STEP, int EACH>
+__global__ void __launch_bounds__(kThreads) read_kernel(ReadArgs const __grid_constant__ a) {
     uint32_t const bhk = a.chunks.div(blockIdx.x), chunk = blockIdx.x - bhk * a.chunks.d;
     int const kv = static_cast<int>(bhk & 1u);
     uint32_t const ub = a.heads.div(bhk >> 1);
     int64_t const b = ub, h = (bhk >> 1) - ub * a.heads.d;
-    CacheTensor const& c = kv ? a.c[1] : a.c[0];
+    CacheTensor const& c = a.c[kv];
     int8_t const* q = c.q + b * c.q_b + h * c.q_h;
     float const* scale = c.scale + b * c.s_b + h * c.s_h;
-    float* out = (kv ? a.out[1] : a.out[0]) + b * (kv ? a.o_b[1] : a.o_b[0]) + h * (kv ? a.o_h[1] : a.o_h[0]);
-    int64_t const o_t = kv ? a.o_t[1] : a.o_t[0], o_d = kv ? a.o_d[1] : a.o_d[0];
-    uint32_t const per = a.row.d, base = chunk * kReadItems + threadIdx.x;
-    uint32_t const t0 = a.row.div(base), c0 = base - t0 * per, all = static_cast<uint32_t>(a.Tout);
-    auto place = [&](int u, uint32_t& t, uint32_t& col) {
-        t = STEP ? t0 + u * (kThreads / per) : a.row.div(base + u * kThreads);
-        col = STEP ? c0 : base + u * kThreads - t * per;
-    };
+    float* out = a.out[kv] + b * a.o_b[kv] + h * a.o_h[kv];
+    int64_t const o_t = a.o_t[kv], o_d = a.o_d[kv];
+    uint32_t const per = a.row.d, base = chunk * (kThreads * EACH) + threadIdx.x;
+    uint32_t t = a.row.div(base), col = base - t * per;
+    uint32_t const all = static_cast<uint32_t>(a.Tout);
+    int64_t const q_u = STEP ? a.rows * c.q_t : 0, o_u = STEP ? a.rows * o_t : 0;
+    int8_t const* p = q + t * c.q_t + (VEC ? 4 * col : col * c.q_d);
+    float* o = out + t * o_t + (VEC ? 4 * col : col * o_d);
     prior_kernels_done();
-    // All loads of a thread at once, the length among them: rows past it are read
-    // (they are part of the cache) and not written.
-    int64_t const q_u = STEP ? kThreads / per * c.q_t : 0, o_u = STEP ? kThreads / per * o_t : 0;
-    int8_t const* q0 = q + t0 * c.q_t + (VEC ? 4 * c0 : c0 * c.q_d);
-    float* o0 = out + t0 * o_t + (VEC ? 4 * c0 : c0 * o_d);
-    float s[kReadEach];
-    char4 n[kReadEach];
+    // The length is on its way with the first loads: rows past it are read (they are
+    // part of the cache) and not written.
+    uint32_t const length = a.lengths != nullptr ? static_cast<uint32_t>(max(0, a.lengths[b * a.len_s])) : all;
+#pragma unroll 1
+    for (int u0 = 0; u0 < EACH && t < all; u0 += kReadAtOnce) {
+        float s[kReadAtOnce];
+        uint32_t n[kReadAtOnce];
+        uint32_t const t0 = t;
 #pragma unroll
-    for (int u = 0; u < kReadEach; ++u) {
-        uint32_t t, col;
-        place(u, t, col);
-        bool const in = t < all;
-        int8_t const* p = STEP ? q0 + u * q_u : q + t * c.q_t + (VEC ? 4 * col : col * c.q_d);
-        s[u] = in ? scale[a.block.div(t) * c.s_j] : 0.0f;
-        if constexpr (VEC)
-            n[u] = in ? *reinterpret_cast<char4 const*>(p) : make_char4(0, 0, 0, 0);
-        else
-            n[u].x = in ? *p : 0;
-    }
-    uint32_t rows = all;
-    if (a.lengths != nullptr) rows = min(rows, static_cast<uint32_t>(max(0, a.lengths[b * a.len_s])));
+        for (int u = 0; u < kReadAtOnce; ++u) {
+            bool const in = t < all;
+            s[u] = in ? __ldg(scale + a.block.div(t) * c.s_j) : 0.0f;
+            if constexpr (VEC)
+                n[u] = in ? __ldg(reinterpret_cast<uint32_t const*>(p)) : 0u;
+            else
+                n[u] = in ? static_cast<uint32_t>(static_cast<int>(__ldg(p))) : 0u;
+            if constexpr (STEP) {
+                t += a.rows, p += q_u;
+            } else {
+                uint32_t const i = base + (u0 + u + 1) * kThreads;
+                t = a.row.div(i), col = i - t * per;
+                p = q + t * c.q_t + (VEC ? 4 * col : col * c.q_d);
+            }
+        }
+        uint32_t const rows = min(all, length);
+        uint32_t tu = t0;
 #pragma unroll
-    for (int u = 0; u < kReadEach; ++u) {
-        uint32_t t, col;
-        place(u, t, col);
-        float* p = STEP ? o0 + u * o_u : out + t * o_t + (VEC ? 4 * col : col * o_d);
-        if (t >= rows) continue;
-        if constexpr (VEC)
-            *reinterpret_cast<float4*>(p) = make_float4(n[u].x * s[u], n[u].y * s[u], n[u].z * s[u], n[u].w * s[u]);
-        else
-            *p = n[u].x * s[u];
+        for (int u = 0; u < kReadAtOnce; ++u) {
+            if constexpr (!STEP) {
+                uint32_t const i = base + (u0 + u) * kThreads;
+                tu = a.row.div(i), col = i - tu * per;
+                o = out + tu * o_t + (VEC ? 4 * col : col * o_d);
+            }
+            if (tu < rows) {
+                if constexpr (VEC)
+                    *reinterpret_cast<float4*>(o) = make_float4(byte_of(n[u], 0) * s[u], byte_of(n[u], 1) * s[u],
+                                                                byte_of(n[u], 2) * s[u], byte_of(n[u], 3) * s[u]);
+                else
+                    *o = static_cast<float>(static_cast<int>(n[u])) * s[u];
+            }
+            if constexpr (STEP) tu += a.rows, o += o_u;
+        }
     }
 }
 
@@ -364,6 +402,7 @@ int append(ann_stream stream, const ann_view* kn, const ann_view* vn, const ann_
         if (!rows4(x[k], sizeof(float)) || !rows4(q[k], 1)) a.vec = 0;
     }
     a.row = FastDiv::make(static_cast<uint32_t>(a.vec ? a.D / 4 : a.D));
+    a.rows = static_cast<int>(kThreads / a.row.d);
     // Rows start anywhere in a block: at most this many blocks hold some of them.
     int64_t const touched = std::min(ceil_div(a.cap, block), ceil_div(a.Tn - 1, block) + 1), grid = B * H * 2 * touched;
     if (a.cap > INT32_MAX) return fail(ANN_ENOTSUP, "kvCacheAppendQ8: more than 2^31 tokens.");
@@ -400,7 +439,7 @@ int read_back(ann_stream stream, const ann_view* kc, const ann_view* vc, const a
     a.D = q[0].ext[3];
     a.Tout = o[0].ext[tok];
     if (o[0].numel() == 0) return ANN_OK;
-    if (a.Tout > INT32_MAX / a.D - kReadItems) return fail(ANN_ENOTSUP, "kvCacheReadQ8: a head of more than 2^31 values.");
+    if (a.Tout > INT32_MAX / a.D - 8 * kThreads) return fail(ANN_ENOTSUP, "kvCacheReadQ8: a head of more than 2^31 values.");
     a.vec = 1;
     for (int k = 0; k < 2; ++k) {
         a.c[k] = tensor_of(q[k], s[k], layout);
@@ -413,13 +452,22 @@ int read_back(ann_stream stream, const ann_view* kc, const ann_view* vc, const a
     }
     a.row = FastDiv::make(static_cast<uint32_t>(a.vec ? a.D / 4 : a.D));
     a.block = FastDiv::make(block);
-    int64_t const chunks = ceil_div(a.Tout * a.row.d, kReadItems), grid = q[0].ext[0] * H * 2 * chunks;
+    bool const step = kThreads % a.row.d == 0;
+    a.rows = kThreads / a.row.d;
+    // Eight items a thread where that leaves four blocks an SM and more (4 x 3048
+    // tokens, 8 heads of 128: 23.0 us against 27.5; sixteen: 24.5), else four.
+    int64_t const heads = q[0].ext[0] * H * 2, items = a.Tout * a.row.d;
+    bool const many = heads * ceil_div(items, 8 * kThreads) >= int64_t{4} * sm_count();
+    int64_t const chunks = ceil_div(items, (many ? 8 : 4) * kThreads), grid = heads * chunks;
     a.chunks = FastDiv::make(static_cast<uint32_t>(chunks));
     a.heads = FastDiv::make(static_cast<uint32_t>(H));
     if (grid > INT32_MAX) return fail(ANN_ENOTSUP, "kvCacheReadQ8: grid too large.");
-    bool const step = kThreads % a.row.d == 0;
-    auto const kernel = a.vec ? (step ? read_kernel<true, true> : read_kernel<true, false>)
-                              : (step ? read_kernel<false, true> : read_kernel<false, false>);
+    auto const pick = [&](auto each) {
+        constexpr int E = decltype(each)::value;
+        return a.vec ? (step ? read_kernel<true, true, E> : read_kernel<true, false, E>)
+                     : (step ? read_kernel<false, true, E> : read_kernel<false, false, E>);
+    };
+    auto const kernel = many ? pick(std::integral_constant<int, 8>{}) : pick(std::integral_constant<int, 4>{});
     launch_overlapping(kernel, dim3(static_cast<unsigned>(grid)), kThreads, 0, as_stream(stream), a);
     return check_launch(what);
 }
