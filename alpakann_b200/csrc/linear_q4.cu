@@ -74,9 +74,9 @@ __device__ __forceinline__ float activate(float v, int act) {
 // Bound by the weights' bytes, K N (1/2 + 4 / group), for one row; eight rows' products
 // take the tensor pipes two thirds of the bytes' time, but with two warps a scheduler
 // (256 registers) 0.4 instructions a cycle are issued, and that bounds it. Measured (K x N, groups of 128, us, of the bytes' time at the copy rate): one
-// row 4096 x 65536 27.0 (0.82), 4096 x 16384 10.7 (0.51), 4096 x 4096 5.3 (0.26: launch,
-// digits, one turn of memory); eight rows 4096 x 16384, groups of 64, 18.6 (0.32), 4096 x
-// 65536 55.8 (0.42).
+// row 4096 x 65536 25.2 (0.88), 4096 x 16384 9.8 (0.56), 4096 x 4096 5.2 (0.27: launch,
+// digits, one turn of memory); eight rows 4096 x 16384, groups of 64, 18.2 (0.33), 4096 x
+// 65536 54.2 (0.44).
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxCluster = 16;
@@ -124,8 +124,11 @@ __device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
 }
 
 // CT: 16-byte words of columns per lane (32 CT columns a tile); NT: slots / 8 (2 NT
-// rows a CTA); VEC: words and scales of four columns are one aligned load.
-template <typename C, int CT, int NT, bool VEC>
+// rows a CTA); VEC: words and scales of four columns are one aligned load; ENDS: groups
+// that end in a quad, 1 (groups of 128, 256, ..), 2 (64), 4 (32) or 0 (any). Code for one
+// kind of group only is a third of the instructions to fetch (4096 x 65536, one row, groups
+// of 64: 26.5 us against 27.9).
+template <typename C, int CT, int NT, bool VEC, int ENDS>
 __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kernel(LinearQ4Args a) {
     extern __shared__ __align__(16) unsigned char smem[];
     int const tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -140,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
     int const share = 1 << a.share_log2, across_log2 = 3 - a.share_log2, across = 1 << across_log2;
     int const part = warp >> across_log2, mine = warp & (across - 1);
     int const q0 = first + ((last - first) * part >> a.share_log2), q1 = first + ((last - first) * (part + 1) >> a.share_log2);
-    int const octets = static_cast<int>(a.K / 8), per_group = a.group / 32;
+    int const octets = static_cast<int>(a.K / 8), per_group = a.group / 32, groups = (steps + per_group - 1) / per_group;
     int const tiles = static_cast<int>((a.N + C::COLS - 1) / C::COLS);
     int const sets = (tiles + across - 1) >> across_log2;  // a CTA's tiles at a time
     int const set0 = static_cast<int>(blockIdx.x) / a.splits, stride = static_cast<int>(gridDim.x) / a.splits;
@@ -156,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
     float* const scale_ring = reinterpret_cast<float*>(smem + a.off_s) + warp * (C::DEPTH + 1) * place_size;
     uint32_t const scale_ring_u = smem_u32(scale_ring);
     // Sums meet their scale after the last step of a group and of a quad. The bits of
-    // such steps, given the steps left in the group; `passed`: groups that end.
+    // such steps (ENDS == 0), given the steps left in the group; `passed`: groups that end.
     int const left0 = per_group - 4 * q0 % per_group;
     auto ends = [&](int quad, int& left, int& passed) {
         unsigned m = 0;
@@ -202,13 +205,21 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
                 }
                 f_w += w_step;
             }
-            int passed;
-            int const n = __popc(ends(f_quad, f_left, passed));  // rows of scales
+            // rows of scales; of groups that K leaves out the last one's, which meets sums of 0
+            int passed = ENDS, n = ENDS, most = 3;
+            if constexpr (ENDS == 0) {
+                n = __popc(ends(f_quad, f_left, passed));
+            } else if constexpr (ENDS == 1) {
+                passed = (f_left -= 4) == 0;
+                if (passed) f_left = per_group;
+            } else {
+                most = groups - 1 - ENDS * f_quad;
+            }
             uint32_t const dst_s = scale_ring_u + static_cast<uint32_t>(f_place * place_size) * 4;
 #pragma unroll
             for (int e = 0; e < CT; ++e) {
                 int const i = lane + 32 * e, r = i / (8 * CT), c = 4 * (i % (8 * CT));
-                float const* const p = f_s + r * a.s_g + c * a.s_n;
+                float const* const p = f_s + min(r, most) * a.s_g + c * a.s_n;
                 if constexpr (VEC) {
                     if (r < n && c < f_cols) copy16(dst_s + 16 * i, p);
                 } else {
@@ -374,8 +385,6 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
         bool const given = (set << across_log2) + mine < tiles;
         int left = left0;
         for (int quad = q0; quad < q1 && given; ++quad) {
-            int passed;
-            unsigned const m = ends(quad, left, passed);
             uint2 const* const dig = reinterpret_cast<uint2 const*>(digits + C::QUAD * (quad - q0)) + lane;
             asm volatile("cp.async.wait_group %0;" ::"n"(C::DEPTH - 1) : "memory");
             __syncwarp();
@@ -399,22 +408,18 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
             fetch();
             constexpr std::true_type fresh{};
             constexpr std::false_type more{};
-            if (m == 8u) {  // groups of 128 inputs or more
+            if constexpr (ENDS > 0) {
+                constexpr int LONG = 4 / ENDS;  // steps of a sum
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     if constexpr (NT > 2) load_b(i);
-                    if (i == 0) multiply(fresh, w[i], b[i]);
+                    if (i % LONG == 0) multiply(fresh, w[i], b[i]);
                     else multiply(more, w[i], b[i]);
-                }
-                flush(sc);
-            } else if (m == 10u) {  // of 64
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if constexpr (NT > 2) load_b(i);
-                    if (i % 2 == 0) multiply(fresh, w[i], b[i]);
-                    else multiply(more, w[i], b[i]), flush(sc), sc += 8 * CT;
+                    if (i % LONG == LONG - 1) flush(sc + i / LONG * (8 * CT));
                 }
             } else {
+                int passed;
+                unsigned const m = ends(quad, left, passed);
                 bool begins = true;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -487,9 +492,9 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
 using Room = std::array<std::array<int, kMaxCluster + 1>, 2>;
 constexpr size_t kHalfSmem = 113 * 1024;
 
-template <typename C, int CT, int NT, bool VEC>
+template <typename C, int CT, int NT, bool VEC, int ENDS>
 int launch(ann_stream stream, LinearQ4Args& a) {
-    auto const kernel = linear_q4_kernel<C, CT, NT, VEC>;
+    auto const kernel = linear_q4_kernel<C, CT, NT, VEC, ENDS>;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attrs[2] = {{}, overlapping()}, &attr = attrs[0];
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -576,7 +581,11 @@ int launch(ann_stream stream, LinearQ4Args& a) {
 template <int CT, int NT, int QUADS = 4 / CT>
 int launch_vec(ann_stream stream, LinearQ4Args& a, bool vec) {
     using C = Q4<CT, NT, QUADS>;
-    return vec ? launch<C, CT, NT, true>(stream, a) : launch<C, CT, NT, false>(stream, a);
+    if (!vec) return launch<C, CT, NT, false, 0>(stream, a);
+    if (a.group % 128 == 0) return launch<C, CT, NT, true, 1>(stream, a);
+    if (a.group == 64) return launch<C, CT, NT, true, 2>(stream, a);
+    if (a.group == 32) return launch<C, CT, NT, true, 4>(stream, a);
+    return launch<C, CT, NT, true, 0>(stream, a);
 }
 
 // The rows of a CTA: all of them up to eight, fewer where the inputs are so many
