@@ -76,6 +76,15 @@ inline bool same_extents(const Dims& a, const Dims& b) {
     return true;
 }
 
+// The same; axes of one element get stride 0, so that theirs (a slice keeps its
+// parent's) has no say in alignment.
+inline int to_dims_flat(const ann_view* v, size_t elem_bytes, const char* what, Dims& out) {
+    int const rc = to_dims(v, elem_bytes, what, out);
+    for (int a = 0; rc == ANN_OK && a < out.rank; ++a)
+        if (out.ext[a] == 1) out.str[a] = 0;
+    return rc;
+}
+
 // An output in which no two elements share an address through a zero pitch.
 inline bool writable(const Dims& d) {
     if (d.numel() == 0) return true;

@@ -1166,12 +1166,12 @@ int decode_q8(ann_stream stream, const ann_view* q_v, const ann_view* k_v, const
         return fail(ANN_EINVAL, "attentionDecodeQ8: invalid kv layout.");
     if (block == 0u) return fail(ANN_EINVAL, "attentionDecodeQ8 requires tokensPerScale > 0.");
     Dims q, k, v, ks, vs, o;
-    ANN_TRY(to_dims(q_v, sizeof(float), "attentionDecodeQ8 Q", q));
-    ANN_TRY(to_dims(k_v, 1, "attentionDecodeQ8 K", k));
-    ANN_TRY(to_dims(v_v, 1, "attentionDecodeQ8 V", v));
-    ANN_TRY(to_dims(ks_v, sizeof(float), "attentionDecodeQ8 K scales", ks));
-    ANN_TRY(to_dims(vs_v, sizeof(float), "attentionDecodeQ8 V scales", vs));
-    ANN_TRY(to_dims(o_v, sizeof(float), "attentionDecodeQ8 out", o));
+    ANN_TRY(to_dims_flat(q_v, sizeof(float), "attentionDecodeQ8 Q", q));
+    ANN_TRY(to_dims_flat(k_v, 1, "attentionDecodeQ8 K", k));
+    ANN_TRY(to_dims_flat(v_v, 1, "attentionDecodeQ8 V", v));
+    ANN_TRY(to_dims_flat(ks_v, sizeof(float), "attentionDecodeQ8 K scales", ks));
+    ANN_TRY(to_dims_flat(vs_v, sizeof(float), "attentionDecodeQ8 V scales", vs));
+    ANN_TRY(to_dims_flat(o_v, sizeof(float), "attentionDecodeQ8 out", o));
     if (q.rank != 4 || k.rank != 4 || v.rank != 4 || o.rank != 4 || ks.rank != 3 || vs.rank != 3)
         return fail(ANN_EINVAL, "attentionDecodeQ8 expects rank-4 tensors and rank-3 scales.");
     if (!same_extents(q, o)) return fail(ANN_EINVAL, "attentionDecodeQ8: out must have the extents of Q.");
@@ -1189,7 +1189,7 @@ int decode_q8(ann_stream stream, const ann_view* q_v, const ann_view* k_v, const
     DecodeQ8Args a{};
     if (len_v != nullptr) {
         Dims len;
-        ANN_TRY(to_dims(len_v, sizeof(int32_t), "attentionDecodeQ8 lengths", len));
+        ANN_TRY(to_dims_flat(len_v, sizeof(int32_t), "attentionDecodeQ8 lengths", len));
         if (len.rank != 1 || len.ext[0] != B)
             return fail(ANN_EINVAL, "attentionDecodeQ8 lengths must be rank 1 with one entry per sequence.");
         a.lengths = static_cast<const int32_t*>(len.data);

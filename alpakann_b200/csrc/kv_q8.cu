@@ -326,8 +326,8 @@ int cache_tensors(const char* what, const ann_view* const qv[2], const ann_view*
     if (layout != ANN_LAYOUT_BTHD && layout != ANN_LAYOUT_BHTD) return fail(ANN_EINVAL, "%s: invalid kv layout.", what);
     if (block == 0) return fail(ANN_EINVAL, "%s requires tokensPerScale > 0.", what);
     for (int k = 0; k < 2; ++k) {
-        ANN_TRY(to_dims(qv[k], 1, what, q[k]));
-        ANN_TRY(to_dims(sv[k], sizeof(float), what, s[k]));
+        ANN_TRY(to_dims_flat(qv[k], 1, what, q[k]));
+        ANN_TRY(to_dims_flat(sv[k], sizeof(float), what, s[k]));
     }
     if (q[0].rank != 4 || q[1].rank != 4) return fail(ANN_EINVAL, "%s expects rank-4 caches.", what);
     if (!same_extents(q[0], q[1])) return fail(ANN_EINVAL, "%s: K and V cache extents differ.", what);
@@ -349,7 +349,7 @@ CacheTensor tensor_of(const Dims& q, const Dims& s, int layout) {
 // A rank-1 int32 view with one entry per sequence.
 int per_sequence(const ann_view* v, const char* what, int64_t B, const int32_t*& p, int64_t& stride) {
     Dims d;
-    ANN_TRY(to_dims(v, sizeof(int32_t), what, d));
+    ANN_TRY(to_dims_flat(v, sizeof(int32_t), what, d));
     if (d.rank != 1 || d.ext[0] != B) return fail(ANN_EINVAL, "%s must be rank 1 with one entry per sequence.", what);
     p = static_cast<const int32_t*>(d.data);
     stride = d.str[0];
@@ -366,8 +366,8 @@ int append(ann_stream stream, const ann_view* kn, const ann_view* vn, const ann_
            int layout) {
     char const* what = "kvCacheAppendQ8";
     Dims x[2], q[2], s[2];
-    ANN_TRY(to_dims(kn, sizeof(float), what, x[0]));
-    ANN_TRY(to_dims(vn, sizeof(float), what, x[1]));
+    ANN_TRY(to_dims_flat(kn, sizeof(float), what, x[0]));
+    ANN_TRY(to_dims_flat(vn, sizeof(float), what, x[1]));
     const ann_view* const qv[2] = {kc, vc};
     const ann_view* const sv[2] = {ks, vs};
     ANN_TRY(cache_tensors(what, qv, sv, block, layout, q, s));
@@ -432,8 +432,8 @@ int read_back(ann_stream stream, const ann_view* kc, const ann_view* vc, const a
     const ann_view* const qv[2] = {kc, vc};
     const ann_view* const sv[2] = {ks, vs};
     ANN_TRY(cache_tensors(what, qv, sv, block, layout, q, s));
-    ANN_TRY(to_dims(ko, sizeof(float), what, o[0]));
-    ANN_TRY(to_dims(vo, sizeof(float), what, o[1]));
+    ANN_TRY(to_dims_flat(ko, sizeof(float), what, o[0]));
+    ANN_TRY(to_dims_flat(vo, sizeof(float), what, o[1]));
     int const tok = layout == ANN_LAYOUT_BTHD ? 1 : 2, head = 3 - tok;
     for (int k = 0; k < 2; ++k) {
         if (o[k].rank != 4 || o[k].ext[0] != q[k].ext[0] || o[k].ext[head] != q[k].ext[head] ||

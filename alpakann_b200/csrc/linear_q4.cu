@@ -642,8 +642,8 @@ __global__ void __launch_bounds__(kPackThreads) pack_kernel(PackArgs a) {
 
 // packed [K/8, N] and scales [ceil(K/group), N].
 int check_packed(const char* what, const ann_view* p_v, const ann_view* s_v, uint32_t group, Dims& p, Dims& s) {
-    ANN_TRY(to_dims(p_v, sizeof(uint32_t), what, p));
-    ANN_TRY(to_dims(s_v, sizeof(float), what, s));
+    ANN_TRY(to_dims_flat(p_v, sizeof(uint32_t), what, p));
+    ANN_TRY(to_dims_flat(s_v, sizeof(float), what, s));
     if (p.rank != 2 || s.rank != 2) return fail(ANN_EINVAL, "%s expects rank-2 packed weights and scales.", what);
     if (group == 0 || group % 32 != 0 || group > (1u << 30))
         return fail(ANN_EINVAL, "%s requires a group size that is a positive multiple of 32.", what);
@@ -656,22 +656,22 @@ int check_packed(const char* what, const ann_view* p_v, const ann_view* s_v, uin
 int linear_q4(ann_stream stream, const ann_view* x_v, const ann_view* p_v, const ann_view* s_v, const ann_view* b_v,
               const ann_view* r_v, const ann_view* y_v, uint32_t group, int act) {
     Dims x, p, s, b, r, y;
-    ANN_TRY(to_dims(x_v, sizeof(float), "linearQ4 input", x));
+    ANN_TRY(to_dims_flat(x_v, sizeof(float), "linearQ4 input", x));
     ANN_TRY(check_packed("linearQ4", p_v, s_v, group, p, s));
-    ANN_TRY(to_dims(y_v, sizeof(float), "linearQ4 output", y));
+    ANN_TRY(to_dims_flat(y_v, sizeof(float), "linearQ4 output", y));
     if (act < ANN_ACT_NONE || act > ANN_ACT_GELU) return fail(ANN_EINVAL, "linearQ4: unknown activation %d.", act);
     if (x.rank != 2 || y.rank != 2 || x.ext[1] != 8 * p.ext[0] || y.ext[0] != x.ext[0] || y.ext[1] != p.ext[1])
         return fail(ANN_EINVAL, "linearQ4 shape mismatch.");
     if (!writable(y)) return fail(ANN_EINVAL, "linearQ4: an output axis has a zero pitch.");
     LinearQ4Args a{};
     if (b_v != nullptr) {
-        ANN_TRY(to_dims(b_v, sizeof(float), "linearQ4 bias", b));
+        ANN_TRY(to_dims_flat(b_v, sizeof(float), "linearQ4 bias", b));
         if (b.rank != 1 || b.ext[0] != y.ext[1]) return fail(ANN_EINVAL, "linearQ4 expects a 1D bias matching the output.");
         a.bias = static_cast<const float*>(b.data);
         a.b_n = b.str[0];
     }
     if (r_v != nullptr) {
-        ANN_TRY(to_dims(r_v, sizeof(float), "linearQ4 residual", r));
+        ANN_TRY(to_dims_flat(r_v, sizeof(float), "linearQ4 residual", r));
         if (!same_extents(r, y)) return fail(ANN_EINVAL, "linearQ4: the residual must have the extents of the output.");
         a.res = static_cast<const float*>(r.data);
         a.r_m = r.str[0];
@@ -702,7 +702,7 @@ int linear_q4(ann_stream stream, const ann_view* x_v, const ann_view* p_v, const
 
 int pack_q4(ann_stream stream, const ann_view* w_v, const ann_view* p_v, const ann_view* s_v, uint32_t group) {
     Dims w, p, s;
-    ANN_TRY(to_dims(w_v, sizeof(float), "packWeightQ4 weight", w));
+    ANN_TRY(to_dims_flat(w_v, sizeof(float), "packWeightQ4 weight", w));
     ANN_TRY(check_packed("packWeightQ4", p_v, s_v, group, p, s));
     if (w.rank != 2 || w.ext[0] != 8 * p.ext[0] || w.ext[1] != p.ext[1])
         return fail(ANN_EINVAL, "packWeightQ4: weight %s does not match packed %s (eight inputs a word).",

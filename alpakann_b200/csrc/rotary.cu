@@ -178,16 +178,16 @@ template <typename T>
 int rotary(ann_stream stream, const ann_view* q_v, const ann_view* k_v, const ann_view* pos_v, const ann_view* freq_v,
            const ann_view* oq_v, const ann_view* ok_v, int pairs, int layout, T mag, int inverse) {
     Dims in[2], out[2], pos, freq;
-    ANN_TRY(to_dims(q_v, sizeof(T), "rotary q", in[0]));
-    ANN_TRY(to_dims(oq_v, sizeof(T), "rotary output q", out[0]));
+    ANN_TRY(to_dims_flat(q_v, sizeof(T), "rotary q", in[0]));
+    ANN_TRY(to_dims_flat(oq_v, sizeof(T), "rotary output q", out[0]));
     if ((k_v == nullptr) != (ok_v == nullptr)) return fail(ANN_EINVAL, "rotary: k and its output come together.");
     int const n = k_v != nullptr ? 2 : 1;
     if (n == 2) {
-        ANN_TRY(to_dims(k_v, sizeof(T), "rotary k", in[1]));
-        ANN_TRY(to_dims(ok_v, sizeof(T), "rotary output k", out[1]));
+        ANN_TRY(to_dims_flat(k_v, sizeof(T), "rotary k", in[1]));
+        ANN_TRY(to_dims_flat(ok_v, sizeof(T), "rotary output k", out[1]));
     }
-    ANN_TRY(to_dims(pos_v, sizeof(int32_t), "rotary positions", pos));
-    ANN_TRY(to_dims(freq_v, sizeof(double), "rotary frequencies", freq));
+    ANN_TRY(to_dims_flat(pos_v, sizeof(int32_t), "rotary positions", pos));
+    ANN_TRY(to_dims_flat(freq_v, sizeof(double), "rotary frequencies", freq));
     if (pairs != ANN_ROTARY_INTERLEAVED && pairs != ANN_ROTARY_HALVES) return fail(ANN_EINVAL, "rotary pairs are invalid.");
     if (layout != ANN_LAYOUT_BTHD && layout != ANN_LAYOUT_BHTD) return fail(ANN_EINVAL, "rotary layout is invalid.");
     int const ta = layout == ANN_LAYOUT_BTHD ? 1 : 2, ha = 3 - ta;
@@ -277,7 +277,7 @@ __global__ void frequencies_kernel(double* f, int64_t stride, int64_t n, double 
 int frequencies(ann_stream stream, const ann_view* f_v, double base, double factor, double trained, double low,
                 double high) {
     Dims f;
-    ANN_TRY(to_dims(f_v, sizeof(double), "rotaryFrequencies", f));
+    ANN_TRY(to_dims_flat(f_v, sizeof(double), "rotaryFrequencies", f));
     if (f.rank != 1) return fail(ANN_EINVAL, "rotaryFrequencies expects a rank-1 output.");
     if (!writable(f)) return fail(ANN_EINVAL, "rotaryFrequencies: the output has a zero pitch.");
     if (!(base > 0.0) || !std::isfinite(base) || !(factor > 0.0) || !std::isfinite(factor))

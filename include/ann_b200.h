@@ -468,7 +468,8 @@ int ann_signal_barrier_dev(ann_stream stream, uint32_t* signals, uint32_t* const
  * No reference counterpart: rotary positions with a position per token, the KV
  * cache in 8 bits and linear layers with 4-bit weights, for decode steps bound
  * by the cache's and the weights' bytes. Outputs must not have a zero pitch on
- * an axis longer than one; inputs may (a broadcast view). Outputs must not overlap
+ * an axis longer than one; inputs may (a broadcast view); the pitch of an axis of
+ * extent one does not matter. Outputs must not overlap
  * inputs except where said. No call waits, each can be captured in a CUDA graph, and
  * only attentionDecodeQ8 over long caches takes device memory: a few megabytes of
  * scratch, allocated and freed in stream order from a pool that the library keeps

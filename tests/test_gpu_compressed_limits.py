@@ -209,3 +209,37 @@ def test_chained_calls_wait_for_their_inputs(nn):
             graph.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_slices_of_one_sequence_keep_odd_strides(nn):
+    """One sequence, token or row of a tensor whose stride along that axis is odd: extent 1, no matter."""
+    g = torch.Generator("cuda").manual_seed(3)
+
+    def odd(t, *axes):
+        """t's values under odd strides along axes of extent 1."""
+        strides = [7 if i in axes else s for i, s in enumerate(t.stride())]
+        return t.as_strided(t.shape, strides)
+
+    q = torch.randn(1, 1, 4, 64, generator=g, device="cuda")
+    kc, vc = (torch.randint(-127, 128, (1, 2, 48, 64), generator=g, device="cuda").to(torch.int8) for _ in range(2))
+    ks = torch.rand(1, 2, 3, generator=g, device="cuda") * 0.01
+    want, out = torch.zeros_like(q), torch.zeros_like(q)
+    nn.attentionDecodeQ8(None, None, q, kc, vc, ks, ks, want, 16, queriesPerKvGroup=2)
+    nn.attentionDecodeQ8(None, None, odd(q, 0, 1), odd(kc, 0), odd(vc, 0), odd(ks, 0), ks, odd(out, 0, 1), 16,
+                         queriesPerKvGroup=2)
+    assert torch.equal(out, want) and want.any()
+    back = torch.zeros(2, 2, 1, 2, 48, 64, device="cuda")
+    nn.kvCacheReadQ8(None, None, kc, vc, ks, ks, back[0, 0], back[0, 1], 16)
+    nn.kvCacheReadQ8(None, None, odd(kc, 0), odd(vc, 0), odd(ks, 0), ks, odd(back[1, 0], 0), back[1, 1], 16)
+    assert torch.equal(back[0], back[1])
+    x, w = torch.randn(1, 256, generator=g, device="cuda"), torch.randint(0, 2**31, (32, 64), generator=g, device="cuda",
+                                                                        dtype=torch.int32)
+    s, y = torch.rand(1, 64, generator=g, device="cuda"), torch.zeros(2, 1, 64, device="cuda")
+    nn.linearQ4(None, None, x, w, s, y[0], 256)
+    nn.linearQ4(None, None, odd(x, 0), w, odd(s, 0), odd(y[1], 0), 256)
+    assert torch.equal(y[0], y[1])
+    f, pos = torch.rand(32, dtype=torch.float64, generator=g, device="cuda"), torch.tensor([[5]], dtype=torch.int32, device="cuda")
+    turned = torch.zeros(2, 1, 1, 4, 64, device="cuda")
+    nn.rotary(None, None, q, None, pos, f, turned[0], None)
+    nn.rotary(None, None, odd(q, 0, 1), None, odd(pos, 0, 1), f, odd(turned[1], 0, 1), None)
+    assert torch.equal(turned[0], turned[1])
