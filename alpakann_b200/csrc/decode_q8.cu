@@ -850,6 +850,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(DecodeQ8Args a,
     int const r = blockIdx.y * per_block + warp / wpr, sub = warp % wpr;
     int64_t const b = blockIdx.x / static_cast<uint32_t>(units);
     int const u = static_cast<int>(blockIdx.x % static_cast<uint32_t>(units));
+    // The lengths are read ahead of the wait: this grid starts when every block of the
+    // shares' has ended, and each of those has waited for the kernels that wrote them.
     int const n = static_cast<int>((keys_of(a, b) + KT - 1) / KT);
     Shares const sh(tiles_before<KT>(a, a.B) * units, G, W);
     int const p0 = tiles_before<KT>(a, b) * units + u * n;

@@ -286,11 +286,11 @@ __global__ void __launch_bounds__(kThreads) read_kernel(ReadArgs const __grid_co
 #pragma unroll
         for (int u = 0; u < kReadAtOnce; ++u) {
             bool const in = t < all;
-            s[u] = in ? __ldg(scale + a.block.div(t) * c.s_j) : 0.0f;
+            s[u] = in ? scale[a.block.div(t) * c.s_j] : 0.0f;
             if constexpr (VEC)
-                n[u] = in ? __ldg(reinterpret_cast<uint32_t const*>(p)) : 0u;
+                n[u] = in ? *reinterpret_cast<uint32_t const*>(p) : 0u;
             else
-                n[u] = in ? static_cast<uint32_t>(static_cast<int>(__ldg(p))) : 0u;
+                n[u] = in ? static_cast<uint32_t>(static_cast<int>(*p)) : 0u;
             if constexpr (STEP) {
                 t += a.rows, p += q_u;
             } else {

@@ -1,7 +1,11 @@
 // overlap.cuh -- launches whose blocks are set up while the kernel before them in
 // the stream ends. Such a kernel calls prior_kernels_done() in every thread before it
 // touches global memory: until then the writes of earlier kernels may be missing, and
-// memory that they read may not be written.
+// memory that they read may not be written. Its loads are plain ones: a read-only load
+// (__ldg, a __restrict__ pointer to const) says that the data does not change while the
+// kernel runs, which is not so before the wait, and the compiler may move it ahead.
+// What the kernels before the one before wrote may be read without the wait, if every
+// block of the kernel before has waited in its turn (merge_kernel in decode_q8.cu).
 #pragma once
 
 #include <cuda_runtime.h>
