@@ -50,28 +50,27 @@ struct DecodeQ8Args {
     float scale;
 };
 
-// How the products are formed. In whole numbers: a row of q is rounded to 31 bits
+// How the products are formed. q.k in whole numbers: a row of q is rounded to 31 bits
 // of its largest value and cut into four 8-bit digits, so that mma.sync.m16n8k32 on
 // int8 multiplies the cache's bytes as they are, and the sums are exact. With up to
 // four query rows of a KV head (R = 4) one product holds all their digits; with up to
 // eight one holds the high two, another the low two.
-// p.v with R = 4 goes the same way: a probability, relative to a reference that the
-// running maximum passes by at most 2^4, times V's scale, relative to a power of
-// two, is rounded to 2^-25 and cut into digits; the sums over keys stay in int32 for
-// up to 2^16 keys and until the maximum (or V's scale) outgrows its reference. Only
-// then, a few times a call, are they converted: a converted sum per tile would cost
-// more instructions than the tile's products. (8 x 2048 keys, 32 heads: 29.6 us in
-// halves, 24.8 in digits. With eight rows the int32 sums take 128 registers a thread
-// and leave 8 warps an SM: 16 x 32768 keys, 64/8 heads 169 us in halves, 176 in
-// digits.)
-// With more rows (and eight at most with heads of 256) p.v runs in halves: a cached value is exact
-// in fp16, a probability is the sum of two fp16 parts (22 bits), and
+// p.v in halves: a cached value is exact in fp16, a probability (times V's scale, relative
+// to the tile's largest of both) is the sum of two fp16 parts (22 bits), and
 // mma.sync.m16n8k16 adds the exact products in fp32, both parts of eight rows in one
 // product, from a fresh accumulator for each tile, so that no sum of more than KT
-// products is left to the tensor core's own rounding.
+// products is left to the tensor core's own rounding. Every key has to keep its own
+// bits: a column of V may be 0 wherever the probabilities are large. The low part is held
+// 2^13 times finer than the high one, so 22 bits reach 2^-30 (20 nats) below the
+// tile's largest; what a tile with scores further apart loses is added in a second turn
+// over such tiles (R = 4: in the rows of the product that four query rows leave free,
+// down to 2^-81). (8 x 2048 keys, 32 heads: 27.8 us for scores of 2 nats' spread, 30.3 for
+// 9; 1 x 131072, eight rows: 37.5, 47 and 58 for 2, 4.5 and 9.)
+// (Digits for p.v too, against one reference for the row, would be 3 us less for 8 x 2048
+// keys, but hold every key to the same step, 2^-25 of the largest.)
 // (On this GPU an int8 product of depth 32 and an fp16 one of depth 16 take the same
 // time, 2.1 cycles of an SM: 8 KB of cache cost 64 of them, 0.4 of the time that HBM
-// takes to deliver it; 32 with R = 4.)
+// takes to deliver it; 48 with R = 4.)
 //
 // How the cache reaches the fragments. The order of the summed index and of the
 // output columns of a matrix product is free as long as both operands agree, so
@@ -90,20 +89,20 @@ struct DecodeQ8Args {
 // caches go in even shares over all CTAs instead, with a second kernel for the parts.
 //
 // Bound by the cache's bytes, 2 D a key and KV head. Measured (us, of the bytes' time
-// at the copy rate): 16 x 32768 keys, 64/8 heads 170 (0.98; 210 with launches back to
-// back for seconds, when the power limit lowers the clock), 8 x 2048, 32/32 24.8 (0.84),
-// 1 x 131072, 32/4 35.5 (0.59: ten rounds of tiles a warp where 9.2 would do, and 5 us
-// for the merge), 12 x 4096 of 64, four tokens, 16/4 12.1 (0.17: the start, and 8 warps'
-// chains of product, maximum, exponential, product), 1 x 300, 32/8 5.2 (launch, two turns
+// at the copy rate): 16 x 32768 keys, 64/8 heads 173 (0.96; 210 with launches back to
+// back for seconds, when the power limit lowers the clock), 8 x 2048, 32/32 27.8 (0.75),
+// 1 x 131072, 32/4 37.5 (0.55: ten rounds of tiles a warp where 9.2 would do, and 5 us
+// for the merge), 12 x 4096 of 64, four tokens, 16/4 12.7 (0.16: the start, and 8 warps'
+// chains of product, maximum, exponential, product), 1 x 300, 32/8 5.3 (launch, two turns
 // of memory, the cluster's barrier).
 constexpr int kMaxCluster = 16;
 constexpr int kMaxShares = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kFiner = 1.0f / 2251799813685248.0f, kSmall = 1.0f / 65536.0f;  // 2^-51, 2^-16: see rest
 
 template <int D, int R, int W>
 struct Q8 {
     static constexpr int THREADS = 32 * W;
-    static constexpr bool INTV = R == 4;           // p.v in whole numbers (D <= 128)
     static constexpr int MT = R == 16 ? 2 : 1;     // groups of eight rows
     static constexpr int KT = D <= 128 ? 32 : 16;  // keys per tile of a warp
     static constexpr int ROWS = R;                 // query rows of a CTA
@@ -113,7 +112,9 @@ struct Q8 {
     static constexpr int KV = KT / 16;             // k16 steps of p.v, groups of 16 keys
     static constexpr int VW = D / 32;              // words of V per lane and key
     static constexpr int KW = D / 16;              // words of K per lane and key
-    static constexpr bool QREG = MT * KS <= 4;     // q's fragments in registers
+    // q's fragments in registers, or read again for each tile (in registers 16 x 32768 keys of
+    // 128, eight rows a head: 180 us against 171, 9 x 16576: 59 against 56)
+    static constexpr bool QREG = MT * KS <= 2;
     static constexpr int TILE = KT * D;            // bytes of a tile of K or V
     static constexpr int RING = 4 * TILE;          // K, V, K, V of a warp; its output rows at the end
     static constexpr int PER_SM = R <= 8 && D <= 128 ? 3 : 2;  // CTAs, by registers
@@ -124,7 +125,6 @@ struct Q8 {
     static constexpr size_t OFF_X = OFF_F + sizeof(float) * ROWS;              // float [kMaxCluster][2][ROWS]: max, sum
     static constexpr size_t SMEM = OFF_X + sizeof(float) * kMaxCluster * 2 * ROWS;
     static_assert(RING >= static_cast<int>(sizeof(float)) * ROWS * D, "a warp's output rows fit its ring");
-    static_assert(!INTV || D <= 128, "int32 sums of whole rows fit the registers");
     // 16-byte piece c of row r of a tile, with the pieces of a 128-byte line
     // permuted: K is read by 8 lanes as two rows x every other piece (or four), V
     // as every other row of 8 x two neighbouring pieces (or halves of them).
@@ -178,13 +178,22 @@ __device__ __forceinline__ uint32_t halves_of(uint32_t w, uint32_t sel) {
     return *reinterpret_cast<uint32_t const*>(&h);
 }
 
-// x, y -> their fp16 parts, high and low, each as a pair.
+// x, y -> their fp16 parts, high and low, each as a pair; the low ones in units 2^13 times
+// finer, so that they too are normal numbers: below 2^15 for x and y below 2^14.
+constexpr float kLowUnit = 1.0f / 8192.0f;
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
     __half2 const h = __floats2half2_rn(x, y);
     float2 const f = __half22float2(h);
-    __half2 const l = __floats2half2_rn(x - f.x, y - f.y);
+    __half2 const l = __floats2half2_rn((x - f.x) * (1.0f / kLowUnit), (y - f.y) * (1.0f / kLowUnit));
     hi = *reinterpret_cast<uint32_t const*>(&h);
     lo = *reinterpret_cast<uint32_t const*>(&l);
+}
+
+// What two parts leave of x below 2^-16, in units 2^51 times finer: exact, and at most 2^13.
+__device__ __forceinline__ float rest(float x) {
+    float const r = x - __half2float(__float2half_rn(x));
+    float const l = __half2float(__float2half_rn(r * (1.0f / kLowUnit)));
+    return fabsf(x) < kSmall ? fmaf(l, -kLowUnit, r) * (1.0f / kFiner) : 0.0f;
 }
 
 // 16 bytes from global to shared memory, asynchronously, in the thread's open group.
@@ -436,50 +445,17 @@ __global__ void __launch_bounds__(32 * W, Q8<D, R, W>::PER_SM) decode_q8_kernel(
         seen[m] = r < rows ? visible(r) : 0;
     }
 
-    float m_run[MT], l_run[MT];  // INTV: the reference of the row's probabilities, and their sum
-    pair_t o[C::INTV ? 1 : MT][D / 8];  // !INTV: columns 2t and 2t + 1 of n-tile n
-    int acc[D / 8][4];                  // INTV: digits' sums
-    float oh[C::INTV ? D / 8 : 1];      // INTV: fp32 sums of row g % 4, column 2t + g / 4 of n-tile n
-    int ref = 26, since = 0;  // INTV: biased exponent of V's scales' reference, tiles since the last conversion
+    float m_run[MT], l_run[MT];  // m_run: a whole number at or above the largest score, so that all factors are powers of two
+    pair_t o[MT][D / 8];         // columns 2t and 2t + 1 of n-tile n
     constexpr int STRETCH = D == 64 ? 8 : 16;  // n-tiles of a lane's consecutive elements
 #pragma unroll
-    for (int m = 0; m < MT; ++m) m_run[m] = neg_inf(0.0f), l_run[m] = 0.0f;
+    for (int m = 0; m < MT; ++m) {
+        m_run[m] = neg_inf(0.0f), l_run[m] = 0.0f;
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n) {
-        if constexpr (C::INTV) {
-            acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0;
-            oh[n] = 0.0f;
-        } else {
-#pragma unroll
-            for (int m = 0; m < MT; ++m) o[m][n] = pair(0.0f, 0.0f);
-        }
+        for (int n = 0; n < D / 8; ++n) o[m][n] = pair(0.0f, 0.0f);
     }
-    // INTV: the digits' sums join the fp32 ones, which are scaled by `by` for the
-    // rows' new reference; V's scales go over to the exponent `to` from here on.
-    auto convert = [&](float by, int to) {
-        if constexpr (C::INTV) {
-            float const unit = pow2_biased(ref - 25);  // 2^(ref - 127) 2^-25
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n) {
-                float const x0 = fmaf(static_cast<float>(acc[n][0]), 65536.0f, static_cast<float>(acc[n][2]));
-                float const x1 = fmaf(static_cast<float>(acc[n][1]), 65536.0f, static_cast<float>(acc[n][3]));
-                // lanes g < 4 hold digits 3 and 1 and keep column 2t, the others 2 and 0 and column 2t + 1
-                float const mine = g < 4 ? x0 : x1, theirs = __shfl_xor_sync(0xffffffffu, g < 4 ? x1 : x0, 16);
-                float const v = g < 4 ? fmaf(mine, 256.0f, theirs) : fmaf(theirs, 256.0f, mine);
-                oh[n] = fmaf(v, unit, oh[n]) * by;
-                acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0;
-            }
-            ref = max(ref, to);
-            since = 0;
-        }
-    };
-
-    for (int stage = 0; tile < t1_seen; tile += W, stage ^= 1) {
-        unsigned char const* const tk = ring + stage * 2 * C::TILE;
-        unsigned char const* const tv = tk + C::TILE;
-        // scores of 8 MT rows and KT keys
-        float s[MT][C::NK][2];
-        copies_landed<3>();
+    // scores of 8 MT rows and the KT keys of a tile in the ring
+    auto scores_of = [&](unsigned char const* tk, float (&s)[MT][C::NK][2]) {
 #pragma unroll
         for (int j = 0; j < C::NK; ++j) {
             uint32_t kr[C::KW];
@@ -523,112 +499,52 @@ __global__ void __launch_bounds__(32 * W, Q8<D, R, W>::PER_SM) decode_q8_kernel(
                 }
             }
         }
-        __syncwarp();  // the warp has read K; its place takes the tile after the next
-        if (tile + 2 * W < t1_seen) fetch(ring_u + stage * 2 * C::TILE, kb, a.k_t, tile + 2 * W);
-        copies_close();
-        if ((tile + 1) * C::KT > least) {
+    };
+    auto mask = [&](int tile, float (&s)[MT][C::NK][2]) {
+        if ((tile + 1) * C::KT <= least) return;
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int j = 0; j < C::NK; ++j)
+            for (int j = 0; j < C::NK; ++j)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        if (tile * C::KT + 8 * j + 2 * t + e >= seen[m]) s[m][j][e] = neg_inf(0.0f);
-        }
-        unsigned vtop = 0, vbad = 0;  // the largest finite |scale| of V's groups and the largest, on the bit patterns
+                for (int e = 0; e < 2; ++e)
+                    if (tile * C::KT + 8 * j + 2 * t + e >= seen[m]) s[m][j][e] = neg_inf(0.0f);
+    };
+    // V's scales relative to a power of two, whose biased exponent is returned: w < 2^14.
+    auto weights = [&](float (&w)[C::KV]) {
+        unsigned top = 0;  // the largest |scale| on the bit patterns
 #pragma unroll
-        for (int i = 0; i < C::KV; ++i) {
-            unsigned const v = __float_as_uint(vsc[i]) & 0x7fffffffu;
-            vbad = max(vbad, v);
-            vtop = max(vtop, v < 0x7f800000u ? v : 0u);
-        }
-        if (vbad >= 0x7f800000u) {  // NaN or infinity makes NaN of the rows that see its keys, and only of them
+        for (int i = 0; i < C::KV; ++i) top = max(top, __float_as_uint(vsc[i]) & 0x7fffffffu);
+        int const e = min(max(static_cast<int>(top >> 23), 15), 253);
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+        for (int i = 0; i < C::KV; ++i) w[i] = vsc[i] * (pow2_biased(254 - e) * 8192.0f);
+        return e;
+    };
+    // a row's largest score of a tile (four lanes share a row)
+    auto largest = [&](float const (&s)[C::NK][2]) {
+        float top = neg_inf(0.0f);
 #pragma unroll
-                for (int j = 0; j < C::NK; ++j)
-                    if (fmaxf(s[m][j][0], s[m][j][1]) > neg_inf(0.0f)) l_run[m] += vsc[j / 2] * 0.0f;
+        for (int j = 0; j < C::NK; ++j) top = fmaxf(top, fmaxf(s[j][0], s[j][1]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        return fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    };
+    // What a key adds to a row's output is its whole numbers times x = p vs, with p
+    // relative to the whole number `local` next to the tile's largest score: x < 2^14.
+    // Returns the lane's sum of p.
+    auto terms = [&](float const (&s)[C::NK][2], float local, float const (&w)[C::KV], float (&x)[C::KV][4]) {
+        float l = 0.0f;
 #pragma unroll
-            for (int i = 0; i < C::KV; ++i)
-                if ((__float_as_uint(vsc[i]) & 0x7fffffffu) >= 0x7f800000u) vsc[i] = 0.0f;
-        }
-        uint32_t pa[MT][C::KV][4];   // !INTV: k16 steps' fragments
-        uint32_t pd[4];              // INTV: the k32 step's
-        if constexpr (C::INTV) {
-            float top = neg_inf(0.0f);
+        for (int i = 0; i < C::KV; ++i)
 #pragma unroll
-            for (int j = 0; j < C::NK; ++j) top = fmaxf(top, fmaxf(s[0][j][0], s[0][j][1]));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            int const ve = min(static_cast<int>(vtop >> 23), 253);
-            bool const grown = top > m_run[0] + 4.0f;  // -infinity: the first key seen
-            if (__any_sync(0xffffffffu, grown) || ve > ref || since == 2048) {
-                float const by = grown ? exp2_neg(m_run[0] - top) : 1.0f;  // nothing before the first key: 0
-                convert(by, max(ve, 26));
-                l_run[0] *= by;
-                if (grown) m_run[0] = top;
+            for (int h = 0; h < 2; ++h) {
+                float const p0 = exp2_neg(s[2 * i + h][0] - local), p1 = exp2_neg(s[2 * i + h][1] - local);
+                l += p0 + p1;
+                float2 const v = unpair(mul2(pair(p0, p1), pair(w[i], w[i])));
+                x[i][2 * h] = v.x, x[i][2 * h + 1] = v.y;
             }
-            ++since;
-            float const base = m_run[0] == neg_inf(0.0f) ? 0.0f : m_run[0], vdown = pow2_biased(254 - ref) * 33554432.0f;
-            uint32_t n[C::NK][2];  // p in whole numbers as signed base-256 digits; p * scale < 2^5, below 2^30
-#pragma unroll
-            for (int j = 0; j < C::NK; ++j) {
-                float const w = vsc[j / 2] * vdown;
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float const p = exp2_neg(s[0][j][e] - base);
-                    l_run[0] += p;
-                    n[j][e] = (static_cast<uint32_t>(__float2int_rn(p * w)) + 0x00808080u) ^ 0x00808080u;
-                }
-            }
-            // a lane's four keys of each group of 16 are four bytes of a fragment
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                uint32_t const* const k0 = n[2 * i];
-                uint32_t const* const k1 = n[2 * i + 1];
-                uint32_t const lo01 = __byte_perm(k0[0], k0[1], 0x5140), hi01 = __byte_perm(k0[0], k0[1], 0x7362);
-                uint32_t const lo23 = __byte_perm(k1[0], k1[1], 0x5140), hi23 = __byte_perm(k1[0], k1[1], 0x7362);
-                uint32_t const pick = g < 4 ? 0x7632 : 0x5410;  // as q's rows: digits 3 and 1, or 2 and 0
-                pd[2 * i] = __byte_perm(hi01, hi23, pick);
-                pd[2 * i + 1] = __byte_perm(lo01, lo23, pick);
-            }
-        }
-        // !INTV: V's scales relative to a power of two, so that p * scale fits fp16
-        int const ve = min(max(static_cast<int>(vtop >> 23), 15), 253);
-        float const vdown = pow2_biased(254 - ve), back = pow2_biased(ve - 13);
-        if constexpr (!C::INTV) {
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            float top = neg_inf(0.0f);
-#pragma unroll
-            for (int j = 0; j < C::NK; ++j) top = fmaxf(top, fmaxf(s[m][j][0], s[m][j][1]));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            float const m_new = fmaxf(m_run[m], top);
-            float const base = m_new == neg_inf(0.0f) ? 0.0f : m_new;
-            if (__any_sync(0xffffffffu, m_new > m_run[m])) {
-                float const alpha = exp2_neg(m_run[m] - base);
-                l_run[m] *= alpha;
-#pragma unroll
-                for (int n = 0; n < D / 8; ++n) o[m][n] = mul2(o[m][n], pair(alpha, alpha));
-                m_run[m] = m_new;
-            }
-#pragma unroll
-            for (int i = 0; i < C::KV; ++i) {
-                float const w = vsc[i] * vdown * 8192.0f;  // p * w < 2^14
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float const p0 = exp2_neg(s[m][2 * i + h][0] - base), p1 = exp2_neg(s[m][2 * i + h][1] - base);
-                    l_run[m] += p0 + p1;
-                    float2 const pw = unpair(mul2(pair(p0, p1), pair(w, w)));
-                    split2(pw.x, pw.y, pa[m][i][2 * h], pa[m][i][2 * h + 1]);
-                }
-            }
-        }
-        }
-        if (tile + W < t1_seen) scales(tile + W);
-        copies_landed<3>();
-        uint32_t vr[C::KV][4][C::VW];
+        return l;
+    };
+    auto load_v = [&](unsigned char const* tv, uint32_t (&vr)[C::KV][4][C::VW]) {
 #pragma unroll
         for (int i = 0; i < C::KV; ++i)
 #pragma unroll
@@ -646,29 +562,16 @@ __global__ void __launch_bounds__(32 * W, Q8<D, R, W>::PER_SM) decode_q8_kernel(
                     }
                 }
             }
-        __syncwarp();
-        if (tile + 2 * W < t1_seen) fetch(ring_u + (stage * 2 + 1) * C::TILE, vb, a.v_t, tile + 2 * W);
-        copies_close();
-        // o += p V, one word of V (four columns of lanes) at a time
-        if constexpr (C::INTV) {
-            // four keys' words to four columns' bytes
+    };
+    // fragments of k16 steps: high parts in row g, low ones in row g + 8
+    auto fragments = [&](float const (&x)[C::KV][4], uint32_t (&pa)[C::KV][4]) {
 #pragma unroll
-            for (int w = 0; w < C::VW; ++w) {
-                uint32_t b[2][4];
+        for (int i = 0; i < C::KV; ++i)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    uint32_t const x01 = __byte_perm(vr[i][0][w], vr[i][1][w], 0x5140), y01 = __byte_perm(vr[i][0][w], vr[i][1][w], 0x7362);
-                    uint32_t const x23 = __byte_perm(vr[i][2][w], vr[i][3][w], 0x5140), y23 = __byte_perm(vr[i][2][w], vr[i][3][w], 0x7362);
-                    b[i][0] = __byte_perm(x01, x23, 0x5410);
-                    b[i][1] = __byte_perm(x01, x23, 0x7632);
-                    b[i][2] = __byte_perm(y01, y23, 0x5410);
-                    b[i][3] = __byte_perm(y01, y23, 0x7632);
-                }
-#pragma unroll
-                for (int n = 0; n < 4; ++n)
-                    mma_s8(acc[4 * w + n], make_uint4(pd[0], pd[1], pd[2], pd[3]), b[0][n], b[1][n]);
-            }
-        } else {
+            for (int h = 0; h < 2; ++h) split2(x[i][2 * h], x[i][2 * h + 1], pa[i][2 * h], pa[i][2 * h + 1]);
+    };
+    // o += x V in units of `unit`, one word of V (four columns of lanes) at a time
+    auto multiply = [&](uint32_t const (&pa)[MT][C::KV][4], float const (&unit)[MT], uint32_t const (&vr)[C::KV][4][C::VW]) {
 #pragma unroll
         for (int w = 0; w < C::VW; ++w) {
             float c[MT][4][4];
@@ -695,22 +598,196 @@ __global__ void __launch_bounds__(32 * W, Q8<D, R, W>::PER_SM) decode_q8_kernel(
             for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int n = 0; n < 4; ++n)
-                    o[m][4 * w + n] = fma2(add2(pair(c[m][n][0], c[m][n][1]), pair(c[m][n][2], c[m][n][3])),
-                                           pair(back, back), o[m][4 * w + n]);
+                    o[m][4 * w + n] = fma2(fma2(pair(c[m][n][2], c[m][n][3]), pair(kLowUnit, kLowUnit), pair(c[m][n][0], c[m][n][1])),
+                                           pair(unit[m], unit[m]), o[m][4 * w + n]);
         }
+    };
+    // Tiles of the warp that are looked at again below: bit k % 32 of lane k / 32, the last
+    // bit for all from there on.
+    constexpr int kMarks = 1023;
+    unsigned marks = 0;
+    int k = 0;  // the warp's k-th tile
+    for (int stage = 0; tile < t1_seen; tile += W, stage ^= 1, ++k) {
+        unsigned char const* const tk = ring + stage * 2 * C::TILE;
+        float s[MT][C::NK][2];
+        copies_landed<3>();
+        scores_of(tk, s);
+        __syncwarp();  // the warp has read K; its place takes the tile after the next
+        if (tile + 2 * W < t1_seen) fetch(ring_u + stage * 2 * C::TILE, kb, a.k_t, tile + 2 * W);
+        copies_close();
+        // the smallest score of each group of 16 keys, before the mask: keys past the end repeat the last one
+        float low[MT][C::KV];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int i = 0; i < C::KV; ++i)
+                low[m][i] = fminf(fminf(s[m][2 * i][0], s[m][2 * i][1]), fminf(s[m][2 * i + 1][0], s[m][2 * i + 1][1]));
+        mask(tile, s);
+        unsigned vbad = 0;  // the largest |scale| of V's groups on the bit patterns
+#pragma unroll
+        for (int i = 0; i < C::KV; ++i) vbad = max(vbad, __float_as_uint(vsc[i]) & 0x7fffffffu);
+        if (vbad >= 0x7f800000u) {  // NaN or infinity makes NaN of the rows that see its keys, and only of them
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int j = 0; j < C::NK; ++j)
+                    if (fmaxf(s[m][j][0], s[m][j][1]) > neg_inf(0.0f)) l_run[m] += vsc[j / 2] * 0.0f;
+#pragma unroll
+            for (int i = 0; i < C::KV; ++i)
+                if ((__float_as_uint(vsc[i]) & 0x7fffffffu) >= 0x7f800000u) vsc[i] = 0.0f;
         }
+        float w[C::KV], reach[C::KV], unit[MT];  // reach: scores further than that from the largest have x < 2^-16
+        int const ve = weights(w);
+#pragma unroll
+        for (int i = 0; i < C::KV; ++i)
+            reach[i] = w[i] == 0.0f ? neg_inf(0.0f) : static_cast<float>(112 - static_cast<int>(__float_as_uint(fabsf(w[i])) >> 23));
+        bool small = false;
+        uint32_t pa[MT][C::KV][4];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            float const top = largest(s[m]);
+#pragma unroll
+            for (int i = 0; i < C::KV; ++i) small |= low[m][i] < top + reach[i];
+            float const m_new = fmaxf(m_run[m], ceilf(top));
+            float const base = m_new == neg_inf(0.0f) ? 0.0f : m_new;
+            if (__any_sync(0xffffffffu, m_new > m_run[m])) {
+                float const alpha = exp2_neg(m_run[m] - base);
+                l_run[m] *= alpha;
+#pragma unroll
+                for (int n = 0; n < D / 8; ++n) o[m][n] = mul2(o[m][n], pair(alpha, alpha));
+                m_run[m] = m_new;
+            }
+            float const local = top == neg_inf(0.0f) ? base : ceilf(top), factor = exp2_neg(local - base);
+            unit[m] = factor * pow2_biased(ve - 13);
+            float x[C::KV][4];
+            float w0[C::KV];
+#pragma unroll
+            for (int i = 0; i < C::KV; ++i) w0[i] = R == 4 && g >= 4 ? 0.0f : w[i];
+            l_run[m] = fmaf(terms(s[m], local, w0, x), factor, l_run[m]);
+            if constexpr (R == 4) {  // lanes g + 4, which have the scores of lanes g, hold what these lose
+                bool deeper = false;
+                if (__any_sync(0xffffffffu, small)) {
+                    float y[C::KV][4];
+                    terms(s[m], local, w, y);
+#pragma unroll
+                    for (int i = 0; i < C::KV; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float const v = rest(y[i][e]);
+                            deeper |= v != 0.0f && fabsf(v) < kSmall;
+                            if (g >= 4) x[i][e] = v;
+                        }
+                }
+                if (g >= 4) unit[m] *= kFiner;
+                small = deeper;
+            }
+            fragments(x, pa[m]);
+        }
+        if (__any_sync(0xffffffffu, small) && lane == min(k, kMarks) / 32) marks |= 1u << (min(k, kMarks) % 32);
+        if (tile + W < t1_seen) scales(tile + W);
+        copies_landed<3>();
+        uint32_t vr[C::KV][4][C::VW];
+        load_v(tk + C::TILE, vr);
+        __syncwarp();
+        if (tile + 2 * W < t1_seen) fetch(ring_u + (stage * 2 + 1) * C::TILE, vb, a.v_t, tile + 2 * W);
+        copies_close();
+        multiply(pa, unit, vr);
+    }
+    copies_landed<0>();
+
+    // Two fp16 parts hold x from 2^-16 on (2^-30 of the tile's largest) to 22 bits and lose up
+    // to 2^-38 of what is smaller. What marked tiles lost is added here, in finer units.
+    if (__any_sync(0xffffffffu, marks != 0)) {
+        int const count = k, first_tile = tile - k * W;
+        auto marked = [&](int k) {  // the first marked tile from the k-th on, or `count`
+            if (k >= kMarks) return __shfl_sync(0xffffffffu, marks, 31) >> 31 ? min(k, count) : count;
+            unsigned const own = lane < k / 32 ? 0u : lane == k / 32 ? marks & ~0u << k % 32 : marks;
+            unsigned const lanes = __ballot_sync(0xffffffffu, own != 0);
+            int const from = __ffs(static_cast<int>(lanes)) - 1;
+            unsigned const bits = __shfl_sync(0xffffffffu, own, max(from, 0));
+            return lanes == 0 ? count : 32 * from + __ffs(static_cast<int>(bits)) - 1;
+        };
+        auto fetch_both = [&](int k, int stage) {
+            if (k < count) {
+                fetch(ring_u + stage * 2 * C::TILE, kb, a.k_t, first_tile + k * W);
+                fetch(ring_u + (stage * 2 + 1) * C::TILE, vb, a.v_t, first_tile + k * W);
+            }
+            copies_close();
+        };
+        k = marked(0);
+        fetch_both(k, 0);
+#pragma unroll 1
+        for (int stage = 0; k < count; stage ^= 1) {
+            int const next = marked(k + 1);
+            fetch_both(next, stage ^ 1);
+            unsigned char const* const tk = ring + stage * 2 * C::TILE;
+            float s[MT][C::NK][2], x[MT][C::KV][4], w[C::KV], unit[MT];
+            tile = first_tile + k * W;
+            scales(tile);
+            copies_landed<1>();
+            scores_of(tk, s);
+            mask(tile, s);
+#pragma unroll
+            for (int i = 0; i < C::KV; ++i)
+                if ((__float_as_uint(vsc[i]) & 0x7fffffffu) >= 0x7f800000u) vsc[i] = 0.0f;
+            int const ve = weights(w);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                float const top = largest(s[m]), base = m_run[m] == neg_inf(0.0f) ? 0.0f : m_run[m];
+                float const local = top == neg_inf(0.0f) ? base : ceilf(top);
+                unit[m] = exp2_neg(local - base) * pow2_biased(ve - 13);
+                terms(s[m], local, w, x[m]);
+                if constexpr (R == 4) {
+                    unit[m] *= kFiner;
+#pragma unroll
+                    for (int i = 0; i < C::KV; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[m][i][e] = g < 4 ? rest(x[m][i][e]) : 0.0f;
+                }
+            }
+            uint32_t vr[C::KV][4][C::VW];
+            load_v(tk + C::TILE, vr);
+#pragma unroll 1
+            for (bool more = true; more;) {  // three times at most: 2^-16 2^-51 2^-51 2^-51 < 2^-149
+                more = false;
+                uint32_t pa[MT][C::KV][4];
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    unit[m] *= kFiner;
+#pragma unroll
+                    for (int i = 0; i < C::KV; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float& y = x[m][i][e];
+                            y = rest(y);
+                            more |= y != 0.0f && fabsf(y) < kSmall;
+                        }
+                    fragments(x[m], pa[m]);
+                }
+                multiply(pa, unit, vr);
+                more = __any_sync(0xffffffffu, more);
+            }
+            __syncwarp();  // the tile is read; its place takes another
+            k = next;
+        }
+        copies_landed<0>();
     }
 
     // Warps to CTA: every warp's rows, maxima and sums. Columns 2t and 2t + 1 of
     // n-tile n are elements 32 t + n and 32 t + 16 + n of a 128-element stretch (D =
     // 64: 16 t + n and 16 t + 8 + n).
-    copies_landed<0>();
-    if constexpr (C::INTV) {
-        convert(1.0f, ref);
+    if constexpr (R == 4) {  // both parts of a row: lanes g < 4 write column 2t, the others column 2t + 1
         float* const p = reinterpret_cast<float*>(ring) + (g & 3) * D + 2 * STRETCH * t + (g >> 2) * STRETCH;
 #pragma unroll
-        for (int n = 0; n < D / 8; n += 4)
-            *reinterpret_cast<float4*>(p + n) = make_float4(oh[n], oh[n + 1], oh[n + 2], oh[n + 3]);
+        for (int n = 0; n < D / 8; n += 4) {
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float2 const y = unpair(o[0][n + i]);
+                v[i] = (g < 4 ? y.x : y.y) + __shfl_xor_sync(0xffffffffu, g < 4 ? y.y : y.x, 16);
+            }
+            *reinterpret_cast<float4*>(p + n) = make_float4(v[0], v[1], v[2], v[3]);
+        }
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
@@ -721,7 +798,7 @@ __global__ void __launch_bounds__(32 * W, Q8<D, R, W>::PER_SM) decode_q8_kernel(
             sml[warp * C::ROWS + 8 * m + g] = m_run[m];
             sml[(W + warp) * C::ROWS + 8 * m + g] = l;
         }
-        if constexpr (!C::INTV) {
+        if constexpr (R > 4) {
             float* row = reinterpret_cast<float*>(ring) + (8 * m + g) * D;
 #pragma unroll
             for (int n = 0; n < D / 8; n += 4) {

@@ -543,7 +543,8 @@ int ann_kv_cache_read_q8_f32(ann_stream stream, const ann_view* k_cache, const a
  * [B] keys per sequence, held to [0, Tcap] (NULL = Tcap). causal != 0: query i
  * sees the keys before lengths[b] - Tq + 1 + i (all of them for Tq = 1); else
  * every query sees lengths[b] keys. A query that sees no key gives a row of
- * zeros. Scores, softmax and sums are held to fp32 accuracy, a query vector's
+ * zeros. Scores, softmax and sums are held to fp32 accuracy, each key's part of a sum by
+ * itself, whatever the sizes of V's scales and of other keys' probabilities; a query vector's
  * elements to 2^-31 of its largest. A NaN or infinity in a query vector or in V's
  * scale of keys that it sees, or a NaN in K's, makes its row NaN. ANN_ENOTSUP
  * unless D is 64, 128 or 256, tokens_per_scale a power of two of 16 or more, and
