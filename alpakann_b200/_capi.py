@@ -119,21 +119,6 @@ for _name, (_args, _res) in SIGNATURES.items():
     _fn.restype = _res
 
 
-def _load_binding():
-    """The CPython module of the short calls, built beside the library."""
-    import importlib.util
-    path = os.path.join(HERE, "_build", "_ann_binding.so")
-    if not os.path.exists(path):
-        raise ImportError(f"alpakann_b200: {path} is missing; build it with `python alpakann_b200/build.py`")
-    spec = importlib.util.spec_from_file_location("_ann_binding", path)
-    module = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(module)
-    return module
-
-
-binding = _load_binding()
-
-
 class AnnError(RuntimeError):
     def __init__(self, code, message):
         super().__init__(message)

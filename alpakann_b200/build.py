@@ -2,17 +2,19 @@
 
 alpakann_b200/csrc/*.cu -> alpakann_b200/_build/obj/*.o -> alpakann_b200/_build/libann_b200.so
 alpakann_b200/csrc/*.cpp (host-only code: file loading, hashing) -> g++ -> same library
-alpakann_b200/binding/binding.c -> gcc -> alpakann_b200/_build/_ann_binding.so (CPython module)
+alpakann_b200/binding/binding.c -> alpakann_b200/_build/_ann_binding.<ABI>.so (CPython module, where torch offers DLPack)
 
 nvcc -gencode arch=compute_100a,code=sm_100a -lineinfo -O3, C++20, static
 cudart inside the shared library (no dependency on the runtime version a
 host process such as PyTorch happens to load), cuBLAS resolved at run time.
 """
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -78,19 +80,26 @@ def _compile(src, extra):
 
 
 BINDING_SRC = os.path.join(HERE, "binding", "binding.c")
-BINDING = os.path.join(OUT_DIR, "_ann_binding.so")
+BINDING = os.path.join(OUT_DIR, "_ann_binding" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
-def build_binding() -> str:
-    """The CPython module of the short calls (binding/binding.c), next to the
-    library it links, for the interpreter that runs this build."""
-    import importlib.util
-    import sysconfig
-    torch = importlib.util.find_spec("torch").submodule_search_locations[0]
-    if _stale(BINDING, [BINDING_SRC, __file__, os.path.join(INCLUDE, "ann_b200.h")]):
-        cmd = [cxx().replace("g++", "gcc"), "-O2", "-Wall", "-fPIC", "-shared", "-I", INCLUDE, "-I",
-               sysconfig.get_paths()["include"], "-I", os.path.join(torch, "include"), BINDING_SRC, "-o", BINDING, "-L", OUT_DIR, "-lann_b200",
-               "-Wl,-rpath,$ORIGIN"]
+def build_binding():
+    """The CPython module of the short calls (binding/binding.c), next to the library
+    it links, for the interpreter that runs this build and the torch beside it; None
+    where torch, its DLPack exchange interface or Python's headers are missing (the calls
+    go through ctypes then)."""
+    torch = importlib.util.find_spec("torch")
+    python = os.path.join(sysconfig.get_paths()["include"], "Python.h")
+    dlpack = os.path.join(torch.submodule_search_locations[0], "include", "ATen", "dlpack.h") if torch else ""
+    if not os.path.exists(dlpack) or not os.path.exists(python):
+        return None
+    with open(dlpack) as f:
+        if "DLPackExchangeAPI" not in f.read():
+            return None
+    if _stale(BINDING, [BINDING_SRC, __file__, dlpack, python, os.path.join(INCLUDE, "ann_b200.h")]):
+        cmd = [cxx(), "-x", "c", "-O2", "-Wall", "-fPIC", "-shared", "-I", INCLUDE, "-I", os.path.dirname(python), "-I",
+               os.path.dirname(os.path.dirname(dlpack)), BINDING_SRC, "-x", "none", "-o", BINDING, "-L", OUT_DIR,
+               "-lann_b200", "-Wl,-rpath,$ORIGIN"]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"binding failed:\n{r.stdout}\n{r.stderr}")

@@ -13,7 +13,8 @@ from dataclasses import dataclass
 
 import torch
 
-from .._capi import AnnView, binding, check, lib, ref, view
+from .._capi import AnnView, check, lib, ref, view
+from .._short import ELSEWHERE as _ELSEWHERE, binding
 from ._common import ext, fn, gemm, handle, suffix, trace
 
 BTHD, BHTD = 0, 1
@@ -295,10 +296,6 @@ class RotaryPairs(enum.IntEnum):
     """Elements of a head vector that rotary turns together."""
     interleaved = 0  # (2p, 2p + 1), as rope
     halves = 1       # (p, p + P), P = number of frequencies
-
-
-binding.setup(torch.Tensor, torch._C._cuda_getDevice)
-_MISMATCH, _ELSEWHERE = -1, -3  # the binding called nothing
 
 
 def _refuse(name, dtypes, tensors):
