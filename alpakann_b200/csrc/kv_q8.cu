@@ -4,10 +4,10 @@
 // one fp32 scale s per KV head and block of `block` tokens:
 //   k_cache, v_cache int8 [B, Hkv, Tcap, D] (or BTHD), scales [B, Hkv, ceil(Tcap / block)].
 //
-// append: s' = max(s of the block's earlier rows, max|x| times fp32's 1/127 over
+// append: s' = max(|s| of the block's earlier rows, max|x| times fp32's 1/127 over
 // the new rows in the block); a new value becomes the whole number nearest to the exact
-// quotient x / s' (ties to even); where s' grew, the block's earlier values are
-// rounded anew from n * s / s'. The rounding is exact, not that of a 32-bit
+// quotient x / s' (ties to even); where s' grew, or s was negative, the block's earlier
+// values are rounded anew from n * s / s'. The rounding is exact, not that of a 32-bit
 // quotient, so any implementation of this definition gives the same integers.
 // A NaN or infinity in a new row makes its block's scale NaN or infinite, so
 // the block reads back as NaN / infinity instead of as wrong finite values.
@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) append_kernel(AppendArgs const 
     unsigned int top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
     bool const begun = j * a.block < lo;  // the block holds earlier rows
-    float const old = begun ? fabsf(*scale) : 0.0f;
+    float const stored = begun ? *scale : 0.0f, old = fabsf(stored);  // a caller may have stored a negative one
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < TH / 32; ++w) top = max(top, red[w]);
@@ -184,13 +184,13 @@ __global__ void __launch_bounds__(TH, 1024 / TH) append_kernel(AppendArgs const 
     if (threadIdx.x == 0) *scale = s;  // every thread has read the old one before the barrier above
 
     bool const finite = __float_as_uint(s) < 0x7f800000u && s > 0.0f;
-    if (begun && __float_as_uint(s) != __float_as_uint(old)) {
+    if (begun && __float_as_uint(s) != __float_as_uint(stored)) {
         int64_t const t0 = j * a.block;
         int const early = static_cast<int>(lo - t0);
         for (int i = threadIdx.x; i < early * D; i += TH) {
             int const r = i / D, d = i - r * D;
             int8_t* p = q + (t0 + r) * c.q_t + d * c.q_d;
-            *p = static_cast<int8_t>(finite ? nearest64(static_cast<double>(*p) * old, s) : 0);
+            *p = static_cast<int8_t>(finite ? nearest64(static_cast<double>(*p) * stored, s) : 0);
         }
     }
     // 64-bit rounding for tiny scales: the remainder's ulp argument needs normal numbers

@@ -520,8 +520,9 @@ int ann_rotary_frequencies(ann_stream stream, const ann_view* frequencies, doubl
  * max|x| * (1/127), both in float32, over its new rows and, if it holds tokens
  * before positions[b], its old scale (its absolute value, should a caller have
  * stored a negative one); new values are the whole numbers nearest to the exact
- * quotient x / scale (ties to even, within [-127, 127]); where the scale grew,
- * the block's earlier values are rounded anew from n * old / new. Tokens of a
+ * quotient x / scale (ties to even, within [-127, 127]); where the scale grew or
+ * was negative, the block's earlier values are rounded anew from n * old / new, so
+ * that they go on standing for what they did. Tokens of a
  * touched block after the new rows are left as they were and are not part of
  * the sequence any more. A NaN or infinite input makes its block's scale NaN or
  * infinite and its integers 0. Rows outside [0, Tcap) are dropped and set
