@@ -388,7 +388,7 @@ int append(ann_stream stream, const ann_view* kn, const ann_view* vn, const ann_
     a.D = x[0].ext[3];
     a.cap = q[0].ext[tok];
     a.block = block;
-    if (x[0].numel() == 0 || a.cap == 0) return ANN_OK;
+    if (x[0].numel() == 0) return ANN_OK;
     int64_t const per_block = std::min<int64_t>(block, a.cap) * a.D;
     if (per_block > INT32_MAX - kThreads) return fail(ANN_ENOTSUP, "kvCacheAppendQ8: a block of one head exceeds 2^31 values.");
     a.vec = 1;
@@ -408,7 +408,8 @@ int append(ann_stream stream, const ann_view* kn, const ann_view* vn, const ann_
     int const threads = in_block <= 512 ? 64 : in_block <= 1024 ? 128 : 256;
     a.rows = static_cast<int>(threads / a.row.d);
     // Rows start anywhere in a block: at most this many blocks hold some of them.
-    int64_t const touched = std::min(ceil_div(a.cap, block), ceil_div(a.Tn - 1, block) + 1), grid = B * H * 2 * touched;
+    // (A cache of no tokens has none, and one thread block that reports the rows.)
+    int64_t const touched = std::clamp(ceil_div(a.cap, block), int64_t{1}, ceil_div(a.Tn - 1, block) + 1), grid = B * H * 2 * touched;
     if (a.cap > INT32_MAX) return fail(ANN_ENOTSUP, "kvCacheAppendQ8: more than 2^31 tokens.");
     a.touched = FastDiv::make(static_cast<uint32_t>(touched));
     a.heads = FastDiv::make(static_cast<uint32_t>(H));

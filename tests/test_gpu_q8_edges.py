@@ -42,3 +42,17 @@ def test_append_behind_a_negative_scale(nn, D, grow):
             assert torch.equal(old[:, :n // 16 * 16], new[:, :n // 16 * 16])
         assert ((after[0, b, :, n:n + 3] - x[b].transpose(0, 1)).abs() <= 0.5001 * scale).all()
     assert torch.equal(after[0], after[1])
+
+
+def test_append_into_a_cache_of_no_tokens_is_reported(nn):
+    import alpakann_b200 as ann
+    from alpakann_b200 import _capi
+    queue = ann.Queue()
+    queue.take_device_error()
+    cache, scale = torch.zeros(2, 3, 0, 64, dtype=torch.int8, device="cuda"), torch.zeros(2, 3, 0, device="cuda")
+    x, pos = torch.randn(2, 4, 3, 64, device="cuda"), torch.tensor([0, 5], dtype=torch.int32, device="cuda")
+    args = (x, x, cache, cache, scale, scale, pos, 16)
+    nn.kvCacheAppendQ8(None, None, *args, counts=torch.zeros(2, dtype=torch.int32, device="cuda"))
+    assert queue.take_device_error() == 0  # no rows, none dropped
+    nn.kvCacheAppendQ8(None, None, *args)
+    assert queue.take_device_error() == _capi.ANN_DEVERR_CACHE_RANGE
