@@ -849,22 +849,27 @@ void attentionPrefillMirror(auto& queue, auto /*exec*/, auto const& Q, auto cons
 enum class RotaryPairs { interleaved = ANN_ROTARY_INTERLEAVED, halves = ANN_ROTARY_HALVES };
 
 namespace detail {
-// An optional view and its descriptor (nullptr stays NULL).
+template <typename E, typename V>
+constexpr bool holds = std::is_same_v<alpaka::nn::b200::detail::elem_of<std::remove_cvref_t<V>>, E>;
+// int32 or uint32 words of the same bits
+template <typename V>
+constexpr bool holds_words = holds<int32_t, V> || holds<uint32_t, V>;
+template <typename... V>
+constexpr bool all_float = (holds<float, V> && ...);
+// An optional view of float or int32 elements and its descriptor (nullptr stays NULL).
+template <typename E>
 struct OptionalView {
     ann_view view{};
     bool given = false;
     OptionalView(std::nullptr_t) {}
     template <typename V>
     OptionalView(V const* v) : given(v != nullptr) {
+        static_assert(std::is_same_v<E, int32_t> ? holds_words<V> : holds<E, V>,
+                      "an optional view holds float (bias, residual) or int32 (counts, lengths) elements");
         if (given) view = alpaka::nn::b200::detail::to_ann(*v);
     }
     ann_view const* get() const { return given ? &view : nullptr; }
 };
-template <typename E, typename V>
-constexpr bool holds = std::is_same_v<alpaka::nn::b200::detail::elem_of<V>, E>;
-// int32 or uint32 words of the same bits
-template <typename V>
-constexpr bool holds_words = holds<int32_t, V> || holds<uint32_t, V>;
 }  // namespace detail
 
 // frequencies (double, rank 1) of rotary, scaled for contexts `factor` times the
@@ -872,7 +877,7 @@ constexpr bool holds_words = holds<int32_t, V> || holds<uint32_t, V>;
 void rotaryFrequencies(auto& queue, auto /*exec*/, auto& frequencies, double base = 10000.0, double factor = 1.0,
                        double trainedLength = 0.0, double lowTurns = 1.0, double highTurns = 32.0) {
     namespace d = alpaka::nn::b200::detail;
-    static_assert(detail::holds<double, std::remove_cvref_t<decltype(frequencies)>>, "frequencies are double");
+    static_assert(detail::holds<double, decltype(frequencies)>, "frequencies are double");
     auto f = d::to_ann(frequencies);
     d::check(ann_rotary_frequencies(d::stream_of(queue), &f, base, factor, trainedLength, lowTurns, highTurns));
 }
@@ -886,8 +891,11 @@ void rotary(auto& queue, auto /*exec*/, auto const& q, auto const& k, auto const
             bool inverse = false) {
     namespace d = alpaka::nn::b200::detail;
     d::require_float<T_Type>();
-    static_assert(detail::holds_words<std::remove_cvref_t<decltype(positions)>>, "positions are int32");
-    static_assert(detail::holds<double, std::remove_cvref_t<decltype(frequencies)>>, "frequencies are double");
+    static_assert(detail::holds<T_Type, decltype(q)> && detail::holds<T_Type, decltype(k)> &&
+                      detail::holds<T_Type, decltype(outQ)> && detail::holds<T_Type, decltype(outK)>,
+                  "q, k and the outputs are of the named type");
+    static_assert(detail::holds_words<decltype(positions)>, "positions are int32");
+    static_assert(detail::holds<double, decltype(frequencies)>, "frequencies are double");
     auto a = d::to_ann(q), b = d::to_ann(k), p = d::to_ann(positions), f = d::to_ann(frequencies);
     auto oa = d::to_ann(outQ), ob = d::to_ann(outK);
     auto const pr = static_cast<int32_t>(pairs), lay = static_cast<int32_t>(layout);
@@ -900,11 +908,12 @@ void rotary(auto& queue, auto /*exec*/, auto const& q, auto const& k, auto const
 // New rows (float BTHD) into int8 caches with a scale per head and block of tokens.
 void kvCacheAppendQ8(auto& queue, auto /*exec*/, auto const& kNew, auto const& vNew, auto& kCache, auto& vCache,
                      auto& kScale, auto& vScale, auto const& positions, uint32_t tokensPerScale,
-                     detail::OptionalView counts = nullptr,
+                     detail::OptionalView<int32_t> counts = nullptr,
                      alpaka::nn::AttentionKvLayout kvLayout = alpaka::nn::AttentionKvLayout::BHTD) {
     namespace d = alpaka::nn::b200::detail;
-    static_assert(detail::holds<int8_t, std::remove_cvref_t<decltype(kCache)>>, "the caches are int8");
-    static_assert(detail::holds_words<std::remove_cvref_t<decltype(positions)>>, "positions are int32");
+    static_assert(detail::holds<int8_t, decltype(kCache)> && detail::holds<int8_t, decltype(vCache)>, "the caches are int8");
+    static_assert(detail::all_float<decltype(kNew), decltype(vNew), decltype(kScale), decltype(vScale)>, "rows and scales are float");
+    static_assert(detail::holds_words<decltype(positions)>, "positions are int32");
     auto kn = d::to_ann(kNew), vn = d::to_ann(vNew), kc = d::to_ann(kCache), vc = d::to_ann(vCache);
     auto ks = d::to_ann(kScale), vs = d::to_ann(vScale), p = d::to_ann(positions);
     d::check(ann_kv_cache_append_q8_f32(d::stream_of(queue), &kn, &vn, &kc, &vc, &ks, &vs, &p, counts.get(),
@@ -914,10 +923,11 @@ void kvCacheAppendQ8(auto& queue, auto /*exec*/, auto const& kNew, auto const& v
 // The float rows that an 8-bit cache stands for.
 void kvCacheReadQ8(auto& queue, auto /*exec*/, auto const& kCache, auto const& vCache, auto const& kScale,
                    auto const& vScale, auto& kOut, auto& vOut, uint32_t tokensPerScale,
-                   detail::OptionalView lengths = nullptr,
+                   detail::OptionalView<int32_t> lengths = nullptr,
                    alpaka::nn::AttentionKvLayout kvLayout = alpaka::nn::AttentionKvLayout::BHTD) {
     namespace d = alpaka::nn::b200::detail;
-    static_assert(detail::holds<int8_t, std::remove_cvref_t<decltype(kCache)>>, "the caches are int8");
+    static_assert(detail::holds<int8_t, decltype(kCache)> && detail::holds<int8_t, decltype(vCache)>, "the caches are int8");
+    static_assert(detail::all_float<decltype(kScale), decltype(vScale), decltype(kOut), decltype(vOut)>, "rows and scales are float");
     auto kc = d::to_ann(kCache), vc = d::to_ann(vCache), ks = d::to_ann(kScale), vs = d::to_ann(vScale);
     auto ko = d::to_ann(kOut), vo = d::to_ann(vOut);
     d::check(ann_kv_cache_read_q8_f32(d::stream_of(queue), &kc, &vc, &ks, &vs, &ko, &vo, lengths.get(), tokensPerScale,
@@ -927,11 +937,12 @@ void kvCacheReadQ8(auto& queue, auto /*exec*/, auto const& kCache, auto const& v
 // attentionDecode over an 8-bit cache; Q, out float BTHD, the last Tq tokens.
 void attentionDecodeQ8(auto& queue, auto /*exec*/, auto const& Q, auto const& kCache, auto const& vCache,
                        auto const& kScale, auto const& vScale, auto& out, uint32_t tokensPerScale,
-                       detail::OptionalView lengths, float scale, uint32_t queriesPerKvGroup = 1u,
+                       detail::OptionalView<int32_t> lengths, float scale, uint32_t queriesPerKvGroup = 1u,
                        alpaka::nn::AttentionKvLayout kvLayout = alpaka::nn::AttentionKvLayout::BHTD,
                        bool causal = true) {
     namespace d = alpaka::nn::b200::detail;
-    static_assert(detail::holds<int8_t, std::remove_cvref_t<decltype(kCache)>>, "the caches are int8");
+    static_assert(detail::holds<int8_t, decltype(kCache)> && detail::holds<int8_t, decltype(vCache)>, "the caches are int8");
+    static_assert(detail::all_float<decltype(Q), decltype(kScale), decltype(vScale), decltype(out)>, "rows and scales are float");
     auto q = d::to_ann(Q), kc = d::to_ann(kCache), vc = d::to_ann(vCache), ks = d::to_ann(kScale);
     auto vs = d::to_ann(vScale), o = d::to_ann(out);
     d::check(ann_attention_decode_q8_f32(d::stream_of(queue), &q, &kc, &vc, &ks, &vs, lengths.get(), &o, scale,
@@ -942,17 +953,19 @@ void attentionDecodeQ8(auto& queue, auto /*exec*/, auto const& Q, auto const& kC
 // A float weight [in, out] in 4 bits with a scale per group of inputs and column.
 void packWeightQ4(auto& queue, auto /*exec*/, auto const& weight, auto& packed, auto& scales, uint32_t groupSize) {
     namespace d = alpaka::nn::b200::detail;
-    static_assert(detail::holds_words<std::remove_cvref_t<decltype(packed)>>, "packed weights are 32-bit words");
+    static_assert(detail::holds_words<decltype(packed)>, "packed weights are 32-bit words");
+    static_assert(detail::all_float<decltype(weight), decltype(scales)>, "weight and scales are float");
     auto w = d::to_ann(weight), p = d::to_ann(packed), s = d::to_ann(scales);
     d::check(ann_pack_weight_q4_f32(d::stream_of(queue), &w, &p, &s, groupSize));
 }
 
 // output = activation(input . W + bias) + residual with W in 4 bits.
 void linearQ4(auto& queue, auto /*exec*/, auto const& input, auto const& packed, auto const& scales, auto& output,
-              uint32_t groupSize, detail::OptionalView bias = nullptr, Activation activation = Activation::none,
-              detail::OptionalView residual = nullptr) {
+              uint32_t groupSize, detail::OptionalView<float> bias = nullptr, Activation activation = Activation::none,
+              detail::OptionalView<float> residual = nullptr) {
     namespace d = alpaka::nn::b200::detail;
-    static_assert(detail::holds_words<std::remove_cvref_t<decltype(packed)>>, "packed weights are 32-bit words");
+    static_assert(detail::holds_words<decltype(packed)>, "packed weights are 32-bit words");
+    static_assert(detail::all_float<decltype(input), decltype(scales), decltype(output)>, "input, scales and output are float");
     auto x = d::to_ann(input), p = d::to_ann(packed), s = d::to_ann(scales), o = d::to_ann(output);
     d::check(ann_linear_q4_f32(d::stream_of(queue), &x, &p, &s, bias.get(), residual.get(), &o, groupSize,
                                static_cast<int32_t>(activation)));
