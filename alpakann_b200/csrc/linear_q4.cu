@@ -439,11 +439,12 @@ __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kern
 #pragma unroll
             for (int k = 0; k < CT; ++k) {
                 float v[4];
+                float const unit = (t & 1 ? 0.0625f : 4096.0f) * down[nt];  // first of all, so that nothing overflows on the way
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float2 const d = unpair(acc[nt][k][e]);
-                    float const two = fmaf(d.x, 256.0f, d.y), low = __shfl_down_sync(0xffffffffu, two, 1);
-                    v[e] = fmaf(two, 4096.0f, low * 0.0625f) * down[nt];
+                    float const two = fmaf(d.x, 256.0f * unit, d.y * unit);
+                    v[e] = two + __shfl_down_sync(0xffffffffu, two, 1);
                 }
                 if ((t & 1) == 0)
                     *reinterpret_cast<float4*>(sums + (warp * C::ROWS + 2 * nt + t / 2) * C::COLS + 32 * k + 4 * g) =

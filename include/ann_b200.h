@@ -546,7 +546,7 @@ int ann_kv_cache_read_q8_f32(ann_stream stream, const ann_view* k_cache, const a
  * every query sees lengths[b] keys. A query that sees no key gives a row of
  * zeros. Scores, softmax and sums are held to fp32 accuracy, each key's part of a sum by
  * itself, whatever the sizes of V's scales and of other keys' probabilities; a query vector's
- * elements to 2^-31 of its largest. A NaN or infinity in a query vector or in V's
+ * elements to 2^-31 of its largest (and to 2^-126). A NaN or infinity in a query vector or in V's
  * scale of keys that it sees, or a NaN in K's, makes its row NaN. ANN_ENOTSUP
  * unless D is 64, 128 or 256, tokens_per_scale a power of two of 16 or more, and
  * head vectors unit-stride with 16-byte aligned rows. */
@@ -569,8 +569,9 @@ int ann_pack_weight_q4_f32(ann_stream stream, const ann_view* weight, const ann_
                            uint32_t group_size);
 /* output [M,N] = act(input [M,K] . W + bias) + residual; bias (rank 1 [N]) and
  * residual ([M,N], may be output) may be NULL, act is ANN_ACT_*. Sums are held to
- * fp32 accuracy, inputs to 2^-31 of the largest of their row; a NaN or infinity in
- * a row of the input makes that row's sums NaN (relu makes 0 of them, as elsewhere).
+ * fp32 accuracy for scales below 2^114 / K, inputs to 2^-31 of the largest of their row
+ * (and to 2^-126); a NaN or infinity in a row of the input makes that row's sums NaN (relu
+ * makes 0 of them, as elsewhere), a NaN or infinite scale its column's NaN or infinite.
  * Meant for the few rows of a decode step:
  * the weights are read once for every eight rows, up to 51200 inputs (for four rows up
  * to 122880, else two). ANN_ENOTSUP for K > 364544 and for more than 131070 rows. */
