@@ -248,7 +248,9 @@ struct ReadArgs {
 };
 
 
-constexpr int kReadAtOnce = 4;  // items of a thread whose loads go out together (eight: 23.5 us for 23.0 below)
+// Items of a thread whose loads go out together (eight: 23.0 us for 22.8 below), ahead of the
+// stores of those before (load_input; ordinary loads: 24.4).
+constexpr int kReadAtOnce = 4;
 
 // Signed byte `at` of w as fp32: its bits with the sign flipped, 128 + n, are the low
 // ones of 2^23 + 128 + n.
@@ -286,9 +288,9 @@ __global__ void __launch_bounds__(kThreads) read_kernel(ReadArgs const __grid_co
 #pragma unroll
         for (int u = 0; u < kReadAtOnce; ++u) {
             bool const in = t < all;
-            s[u] = in ? scale[a.block.div(t) * c.s_j] : 0.0f;
+            s[u] = in ? load_input(scale + a.block.div(t) * c.s_j) : 0.0f;
             if constexpr (VEC)
-                n[u] = in ? *reinterpret_cast<uint32_t const*>(p) : 0u;
+                n[u] = in ? load_input(reinterpret_cast<uint32_t const*>(p)) : 0u;
             else
                 n[u] = in ? static_cast<uint32_t>(static_cast<int>(*p)) : 0u;
             if constexpr (STEP) {
@@ -466,7 +468,7 @@ int read_back(ann_stream stream, const ann_view* kc, const ann_view* vc, const a
     bool const step = kThreads % a.row.d == 0;
     a.rows = kThreads / a.row.d;
     // Eight items a thread where that leaves four blocks an SM and more (4 x 3048
-    // tokens, 8 heads of 128: 23.0 us against 27.5; sixteen: 24.5), else four.
+    // tokens, 8 heads of 128: 22.8 us against 27.5; sixteen: 24.5), else four.
     int64_t const heads = q[0].ext[0] * H * 2, items = a.Tout * a.row.d;
     bool const many = heads * ceil_div(items, 8 * kThreads) >= int64_t{4} * sm_count();
     int64_t const chunks = ceil_div(items, (many ? 8 : 4) * kThreads), grid = heads * chunks;

@@ -10,9 +10,22 @@
 
 #include <cuda_runtime.h>
 
+#include <cstdint>
+
 namespace ann {
 
 __device__ __forceinline__ void prior_kernels_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// A load that stays behind prior_kernels_done() (both are volatile) and that ordinary
+// stores before it in the program do not hold up: for inputs that the kernel does not write.
+__device__ __forceinline__ uint32_t load_input(uint32_t const* p) {
+    uint32_t v;
+    asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ float load_input(float const* p) {
+    return __uint_as_float(load_input(reinterpret_cast<uint32_t const*>(p)));
+}
 
 inline cudaLaunchAttribute overlapping() {
     cudaLaunchAttribute attr{};
