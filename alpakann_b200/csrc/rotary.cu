@@ -11,8 +11,8 @@
 // frequency, so a far or irregular position costs nothing extra and the bytes
 // moved are one read and one write of q and k. The 64-bit product is what far
 // positions need (position 100000 leaves 7 bits of fraction in a 32-bit
-// angle); it is brought into [-1/2, 1/2] turns in 64 bits and only then rounded
-// to the tensor's type, so fp32 takes one single-precision sincospi per pair.
+// angle); it is brought within an eighth of a turn of a whole quarter in 64 bits and only
+// then rounded to the tensor's type, so fp32 takes one single-precision sincospi per pair.
 // A thread forms the angles of its pairs once and walks over heads with them. Bound by
 // HBM; measured: 4 x 4096 tokens, 32 + 32 heads of 128 180 us (0.92 of the bytes' time at
 // the copy rate), fp64 2 x 1024 tokens, 16 + 16 heads of 64 12.1 us (0.86), 16 single
@@ -67,9 +67,16 @@ __device__ __forceinline__ int64_t head_out(RotaryArgs const& a, int64_t b, int6
 }
 
 __device__ __forceinline__ void angle_cs(double a, float& c, float& s) {
-    double const turns = a * 0.15915494309189535;  // 1 / (2 pi)
-    float const r = static_cast<float>(turns - rint(turns));
-    sincospif(2.0f * r, &s, &c);
+    double const turns = a * 0.15915494309189535, part = turns - rint(turns);  // 1 / (2 pi)
+    // quarters of a turn are taken off in 64 bits, so that rounding costs 2^-28 turns and not 2^-26
+    float const quarters = rintf(4.0f * static_cast<float>(part));
+    float x, y;
+    sincospif(static_cast<float>(2.0 * part - 0.5 * quarters), &y, &x);
+    int const k = static_cast<int>(quarters) & 3;
+    c = (k & 1) != 0 ? y : x;
+    s = (k & 1) != 0 ? x : y;
+    if (((k + 1) & 2) != 0) c = -c;
+    if ((k & 2) != 0) s = -s;
 }
 __device__ __forceinline__ void angle_cs(double a, double& c, double& s) { sincos(a, &s, &c); }
 
