@@ -89,7 +89,7 @@ struct DecodeQ8Args {
 // caches go in even shares over all CTAs instead, with a second kernel for the parts.
 //
 // Bound by the cache's bytes, 2 D a key and KV head. Measured (us, of the bytes' time
-// at the copy rate): 16 x 32768 keys, 64/8 heads 173 (0.96; 210 with launches back to
+// at the copy rate): 16 x 32768 keys, 64/8 heads 174 (0.96; 213 with launches back to
 // back for seconds, when the power limit lowers the clock), 8 x 2048, 32/32 27.8 (0.75),
 // 1 x 131072, 32/4 37.5 (0.55: ten rounds of tiles a warp where 9.2 would do, and 5 us
 // for the merge), 12 x 4096 of 64, four tokens, 16/4 12.7 (0.16: the start, and 8 warps'
@@ -1149,7 +1149,9 @@ int launch_shares(ann_stream stream, DecodeQ8Args& a, int64_t units) {
     launch_overlapping(kernel, dim3(static_cast<unsigned>(G)), C::THREADS, C::SMEM, as_stream(stream), a);
     int rc = check_launch("attentionDecodeQ8");
     if (rc == ANN_OK) {
-        // few units: many parts each, so all warps of a block to one row
+        // Few units have many parts each, so all warps of a block go to one row; many fill the
+        // GPU with a warp or two a row (rows a block of 1 / 4 / 8, us of both kernels: 4 units, 1 x
+        // 131072 keys, 37.4 / 40.8 / 44.5; 32, 4 x 65536, 101 / 97 / 97; 64, 8 x 32768, 107 / 97 / 96).
         int const rows = static_cast<int>(std::min<int64_t>(C::ROWS, a.Tq * a.g)), per_block = units < G / 8 ? 1 : std::min(8, C::ROWS);
         dim3 const grid(static_cast<unsigned>(units), static_cast<unsigned>(ceil_div(rows, per_block)));
         launch_overlapping(merge_kernel<D, C::ROWS, C::KT>, grid, 32 * kMergeWarps, 0, as_stream(stream), a,
@@ -1168,9 +1170,9 @@ int launch_shares(ann_stream stream, DecodeQ8Args& a, int64_t units) {
 //    does not fill the GPU, though not in proportion, and no less than 0.45.
 //  * Even shares: their tiles a warp, and about 1.5 tiles' times for the second
 //    launch and for each part of a KV head that a CTA meets.
-// Measured (us, clusters at their best S / shares): 8 x 2048 keys, 32 KV heads 25 /
-// 39; 12 x 4096 keys of 64, 4 heads, four tokens 16 / 20; 31 x 7345 keys of 64, 6
-// heads 36 / 43; 16 x 32768 keys, 8 heads 178 / 169; 1 x 131072 keys, 4 heads 72 / 36.
+// Measured (us, clusters at their best S / shares): 8 x 2048 keys, 32 KV heads 28 /
+// 38; 12 x 4096 keys of 64, 4 heads, four tokens 13 / 17; 31 x 7345 keys of 64, 6
+// heads 41 / 47; 16 x 32768 keys, 8 heads 176 / 174; 1 x 131072 keys, 4 heads 69 / 38.
 template <int D, int R>
 struct Plan {
     using C = Q8<D, R, 4>;
@@ -1215,10 +1217,10 @@ int launch(ann_stream stream, DecodeQ8Args& a) {
 // Query rows of a CTA. Sixteen read the cache half as often as eight, but a tile takes
 // a warp 1.1 times as long, the start and the end one microsecond (0.6 tiles) more, and
 // their registers leave 8 warps an SM instead of 12 (16 x 16384 keys of 64, 8 heads of
-// sixteen rows: 90 us against 111; 12 x 4096, 4 heads: 17.0 against 15.9; 1 x 300, 3
-// heads: 6.7 against 5.3). Heads of 256 take eight: sixteen rows' fragments leave no
-// registers for q's (2 x 65536 keys, 2 heads of sixteen rows: 76 us against 53; 16 x
-// 8192, 4 heads: 85 against 93).
+// sixteen rows: 95 us against 113; 12 x 4096, 4 heads: 15.0 against 12.8; 1 x 300, 3
+// heads: 8.2 against 6.2). Heads of 256 take eight: sixteen rows' sums and fragments do
+// not fit the registers (2 x 65536 keys, 2 heads of sixteen rows: 81 us against 57; 16 x
+// 8192, 4 heads: 134 against 94).
 template <int D>
 int launch_rows(ann_stream stream, DecodeQ8Args& a) {
     if (a.Tq > INT32_MAX / 2 / int64_t{a.g}) return fail(ANN_ENOTSUP, "attentionDecodeQ8: more than 2^30 rows.");

@@ -73,10 +73,11 @@ __device__ __forceinline__ float activate(float v, int act) {
 //
 // Bound by the weights' bytes, K N (1/2 + 4 / group), for one row; eight rows' products
 // take the tensor pipes two thirds of the bytes' time, but with two warps a scheduler
-// (256 registers) 0.4 instructions a cycle are issued, and that bounds it. Measured (K x N, groups of 128, us, of the bytes' time at the copy rate): one
-// row 4096 x 65536 25.2 (0.88), 4096 x 16384 9.8 (0.56), 4096 x 4096 5.2 (0.27: launch,
-// digits, one turn of memory); eight rows 4096 x 16384, groups of 64, 18.2 (0.33), 4096 x
-// 65536 54.2 (0.44).
+// (256 registers) 0.4 instructions a cycle are issued, and that bounds it. Measured (K x N,
+// groups of 128, us, of the bytes' time at the copy rate): one row 4096 x 65536 25.3 (0.87),
+// 4096 x 16384 9.3 (0.59), 4096 x 4096 5.2 (0.27: launch, digits, one turn of memory); eight
+// rows 4096 x 16384, groups of 64, 18.5 (0.32), 4096 x 65536 56 (0.42). The weights are read
+// once for every eight rows: 4096 x 16384, 16 rows 28.0, 32 50.9, 64 96.3.
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxCluster = 16;
@@ -127,7 +128,7 @@ __device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
 // rows a CTA); VEC: words and scales of four columns are one aligned load; ENDS: groups
 // that end in a quad, 1 (groups of 128, 256, ..), 2 (64), 4 (32) or 0 (any). Code for one
 // kind of group only is a third of the instructions to fetch (4096 x 65536, one row, groups
-// of 64: 26.5 us against 27.9).
+// of 128, 64 and 32: 25.4, 27.0 and 29.9 us against 28.0, 28.3 and 33.6).
 template <typename C, int CT, int NT, bool VEC, int ENDS>
 __global__ void __launch_bounds__(kThreads, NT * CT >= 4 ? 1 : 2) linear_q4_kernel(LinearQ4Args a) {
     extern __shared__ __align__(16) unsigned char smem[];
@@ -532,12 +533,13 @@ int launch(ann_stream stream, LinearQ4Args& a) {
     if (tiles > INT32_MAX || row_tiles > 65535) return fail(ANN_ENOTSUP, "linearQ4: grid too large.");
     a.ends = a.group == 32 ? 4 : a.group % 128 == 0 ? 1 : 2;
     // How many warps of a CTA and CTAs of a cluster share the inputs: the least of
-    // these estimates (us, fitted to 20 shapes at up to 36 choices each; the estimate's
-    // best is within 3 % of the measured best there). A quad takes a warp its memory's latency
+    // these estimates (us, fitted to measured shapes). A quad takes a warp its memory's latency
     // with two in flight, or its turn among the SM's warps; preparing a quad's digits,
-    // and what a set of tiles costs to sum and store, count beside it. (8 x 4096 x
-    // 16384: two by two 19 us, all eight warps of two CTAs 23, one of four 20; 1 x 4096 x
-    // 4096: 4 by 4 5.8, eight of one CTA 7.6; 1 x 4096 x 65536: one of two 28, eight of one 31.)
+    // and what a set of tiles costs to sum and store, count beside it. (On thirteen shapes at
+    // up to 36 choices each the estimate's is within 3 % of the best; us of it, of all eight
+    // warps to a tile, of a tile a warp, each with its best cluster: 8 x 4096 x 16384 18.5,
+    // 22.6, 19.3; 1 x 4096 x 4096 5.1, 5.1, 6.5; 1 x 4096 x 65536 24.9, 26.3, 25.0; 1 x 16384 x
+    // 4096 9.2, 10.1, 13.9.)
     size_t smem = 0;
     int64_t clusters = 0;
     double best = 1e300;
@@ -695,9 +697,9 @@ int linear_q4(ann_stream stream, const ann_view* x_v, const ann_view* p_v, const
     a.x_vec = a.x_k == 1 && a.x_m % 4 == 0 && aligned(x.data, 16);
     bool const vec = a.w_n == 1 && a.w_r % 4 == 0 && aligned(p.data, 16) && a.s_n == 1 && a.s_g % 4 == 0 &&
                      aligned(s.data, 16) && a.N % 4 == 0;
-    // Few columns: tiles of 32 give twice the CTAs (1024 x 1024: 3.5 us against 3.7,
+    // Few columns: tiles of 32 give twice the CTAs (1024 x 1024: 3.0 us against 3.6,
     // eight rows 5.4 against 6.2); else 64, whose copies, digits and loops serve twice
-    // the weights (4096 x 65536: 27.4 us against 31.9; 4096 x 2048: 4.5 against 5.1).
+    // the weights (4096 x 65536: 25.4 us against 26.2; 4096 x 2048: 4.5 against 4.8).
     return a.N < 2048 ? launch_rows<1>(stream, a, vec) : launch_rows<2>(stream, a, vec);
 }
 
