@@ -545,8 +545,9 @@ int ann_kv_cache_read_q8_f32(ann_stream stream, const ann_view* k_cache, const a
  * sees the keys before lengths[b] - Tq + 1 + i (all of them for Tq = 1); else
  * every query sees lengths[b] keys. A query that sees no key gives a row of
  * zeros. Scores, softmax and sums are held to fp32 accuracy, each key's part of a sum by
- * itself, whatever the sizes of V's scales and of other keys' probabilities; a query vector's
- * elements to 2^-31 of its largest (and to 2^-126). A NaN or infinity in a query vector or in V's
+ * itself, whatever the sizes of V's scales and of other keys' probabilities, as long as the sum
+ * of p |v|, p relative to the row's largest, fits fp32; a query vector's elements to 2^-31
+ * of its largest (and to 2^-126). A NaN or infinity in a query vector or in V's
  * scale of keys that it sees, or a NaN in K's, makes its row NaN. ANN_ENOTSUP
  * unless D is 64, 128 or 256, tokens_per_scale a power of two of 16 or more, and
  * head vectors unit-stride with 16-byte aligned rows. */

@@ -154,3 +154,38 @@ def test_columns_that_only_small_contributions_reach(nn, rows, D):
         for ratio in (1.0, 1e6):
             vs = (g.uniform(0.5, 1, (1, n)) * np.where(np.arange(n) % 2, ratio, 1) / 127).astype(np.float32)
             check(nn, q, kc, vc, ks, vs, block, gap / 40.0, rows, f"gap {gap} ratio {ratio}")
+
+
+@pytest.mark.parametrize("D,g_,Tq", [(128, 1, 3), (64, 2, 2), (128, 2, 4), (64, 5, 3), (256, 2, 3)])
+@pytest.mark.parametrize("T", [90, 15000])
+def test_several_tokens_over_scores_far_apart(nn, D, g_, Tq, T):
+    """Causal queries of ragged sequences, one key of V = 0 far above the others: every
+    query by itself, over the keys that it sees."""
+    g = np.random.default_rng(D + Tq + T)
+    lengths, block, Hkv = [T, 41, Tq - 1, 0], 16, 2
+    B, n = len(lengths), -(-T // block)
+    level = np.full((B * Hkv, T), -120) + g.integers(-1, 2, (B * Hkv, T))
+    level[:, 7] = 0
+    level[:, 20:T:33] = -60
+    kc = keys(g, B * Hkv, T, D, level).reshape(B, Hkv, T, D)
+    vc = g.integers(-127, 128, (B, Hkv, T, D)).astype(np.int8)
+    kc[:, :, 7], vc[:, :, 7] = 0, 0
+    vc[:, :, 20:T:33, ::2] = 0
+    ks = np.full((B, Hkv, n), 0.125, np.float32)
+    vs = (g.uniform(0.5, 1, (B, Hkv, n)) / 127).astype(np.float32)
+    q = queries(g, B * Tq * Hkv * g_, D).reshape(B, Tq, Hkv * g_, D)
+    dev = [torch.from_numpy(a).cuda() for a in (q, kc, vc, ks, vs)]
+    for gap in (10, 22, 50):
+        out = torch.full(q.shape, float("nan"), device="cuda")
+        nn.attentionDecodeQ8(None, None, *dev, out, block, torch.tensor(lengths, dtype=torch.int32, device="cuda"),
+                             gap / 120.0, g_)
+        got = out.cpu().numpy().astype(np.float64)
+        for b in range(B):
+            for i in range(Tq):
+                seen = lengths[b] - Tq + 1 + i
+                if seen <= 0:
+                    assert not got[b, i].any()
+                    continue
+                want, tol, _, _ = attend(q[b, i], kc[b, :, :seen], vc[b, :, :seen], ks[b], vs[b], block, gap / 120.0, g_)
+                off = np.abs(got[b, i] - want)
+                assert (off <= np.maximum(tol, 1e-300)).all(), (gap, b, i, (off / np.maximum(tol, 1e-300)).max())
