@@ -62,11 +62,11 @@ struct DecodeQ8Args {
 // products is left to the tensor core's own rounding. Every key has to keep its own
 // bits: a column of V may be 0 wherever the probabilities are large. The low part is held
 // 2^13 times finer than the high one, so 22 bits reach 2^-30 (20 nats) below the
-// tile's largest; what a tile with scores further apart loses is added in a second turn
-// over such tiles (R = 4: in the rows of the product that four query rows leave free,
-// down to 2^-81). (8 x 2048 keys, 32 heads: 27.8 us for scores of 2 nats' spread, 30.3 for
-// 9; 1 x 131072, eight rows: 37.5, 47 and 58 for 2, 4.5 and 9.)
-// (Digits for p.v too, against one reference for the row, would be 3 us less for 8 x 2048
+// tile's largest. Tiles with scores further apart are marked, and where a sum is so small that
+// what they lost may show, they are multiplied once more. (8 x 2048 keys, 32 heads:
+// 27.6 us for scores of 2 and of 4.5 nats' standard deviation, 44 for 9; 1 x 131072, eight rows:
+// 37.4, 39 and 50.)
+// (Digits for p.v too, against one reference for the row, would be 2 us less for 8 x 2048
 // keys, but hold every key to the same step, 2^-25 of the largest.)
 // (On this GPU an int8 product of depth 32 and an fp16 one of depth 16 take the same
 // time, 2.1 cycles of an SM: 8 KB of cache cost 64 of them, 0.4 of the time that HBM
@@ -445,12 +445,13 @@ __global__ void __launch_bounds__(32 * W, Q8<D, R, W>::PER_SM) decode_q8_kernel(
         seen[m] = r < rows ? visible(r) : 0;
     }
 
+    float lost[MT];              // units of the marked tiles, below
     float m_run[MT], l_run[MT];  // m_run: a whole number at or above the largest score, so that all factors are powers of two
     pair_t o[MT][D / 8];         // columns 2t and 2t + 1 of n-tile n
     constexpr int STRETCH = D == 64 ? 8 : 16;  // n-tiles of a lane's consecutive elements
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-        m_run[m] = neg_inf(0.0f), l_run[m] = 0.0f;
+        m_run[m] = neg_inf(0.0f), l_run[m] = lost[m] = 0.0f;
 #pragma unroll
         for (int n = 0; n < D / 8; ++n) o[m][n] = pair(0.0f, 0.0f);
     }
@@ -511,13 +512,14 @@ __global__ void __launch_bounds__(32 * W, Q8<D, R, W>::PER_SM) decode_q8_kernel(
                     if (tile * C::KT + 8 * j + 2 * t + e >= seen[m]) s[m][j][e] = neg_inf(0.0f);
     };
     // V's scales relative to a power of two, whose biased exponent is returned: w < 2^14.
+    // (R = 4: lanes g + 4 have the scores of lanes g; their rows of the product stay 0.)
     auto weights = [&](float (&w)[C::KV]) {
         unsigned top = 0;  // the largest |scale| on the bit patterns
 #pragma unroll
         for (int i = 0; i < C::KV; ++i) top = max(top, __float_as_uint(vsc[i]) & 0x7fffffffu);
         int const e = min(max(static_cast<int>(top >> 23), 15), 253);
 #pragma unroll
-        for (int i = 0; i < C::KV; ++i) w[i] = vsc[i] * (pow2_biased(254 - e) * 8192.0f);
+        for (int i = 0; i < C::KV; ++i) w[i] = R == 4 && g >= 4 ? 0.0f : vsc[i] * (pow2_biased(254 - e) * 8192.0f);
         return e;
     };
     // a row's largest score of a tile (four lanes share a row)
@@ -653,6 +655,7 @@ __global__ void __launch_bounds__(32 * W, Q8<D, R, W>::PER_SM) decode_q8_kernel(
             if (__any_sync(0xffffffffu, m_new > m_run[m])) {
                 float const alpha = exp2_neg(m_run[m] - base);
                 l_run[m] *= alpha;
+                lost[m] *= alpha;
 #pragma unroll
                 for (int n = 0; n < D / 8; ++n) o[m][n] = mul2(o[m][n], pair(alpha, alpha));
                 m_run[m] = m_new;
@@ -660,30 +663,14 @@ __global__ void __launch_bounds__(32 * W, Q8<D, R, W>::PER_SM) decode_q8_kernel(
             float const local = top == neg_inf(0.0f) ? base : ceilf(top), factor = exp2_neg(local - base);
             unit[m] = factor * pow2_biased(ve - 13);
             float x[C::KV][4];
-            float w0[C::KV];
-#pragma unroll
-            for (int i = 0; i < C::KV; ++i) w0[i] = R == 4 && g >= 4 ? 0.0f : w[i];
-            l_run[m] = fmaf(terms(s[m], local, w0, x), factor, l_run[m]);
-            if constexpr (R == 4) {  // lanes g + 4, which have the scores of lanes g, hold what these lose
-                bool deeper = false;
-                if (__any_sync(0xffffffffu, small)) {
-                    float y[C::KV][4];
-                    terms(s[m], local, w, y);
-#pragma unroll
-                    for (int i = 0; i < C::KV; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float const v = rest(y[i][e]);
-                            deeper |= v != 0.0f && fabsf(v) < kSmall;
-                            if (g >= 4) x[i][e] = v;
-                        }
-                }
-                if (g >= 4) unit[m] *= kFiner;
-                small = deeper;
-            }
+            l_run[m] = fmaf(terms(s[m], local, w, x), factor, l_run[m]);
             fragments(x, pa[m]);
         }
-        if (__any_sync(0xffffffffu, small) && lane == min(k, kMarks) / 32) marks |= 1u << (min(k, kMarks) % 32);
+        if (__any_sync(0xffffffffu, small)) {
+            if (lane == min(k, kMarks) / 32) marks |= 1u << (min(k, kMarks) % 32);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) lost[m] += unit[m];
+        }
         if (tile + W < t1_seen) scales(tile + W);
         copies_landed<3>();
         uint32_t vr[C::KV][4][C::VW];
@@ -696,8 +683,23 @@ __global__ void __launch_bounds__(32 * W, Q8<D, R, W>::PER_SM) decode_q8_kernel(
     copies_landed<0>();
 
     // Two fp16 parts hold x from 2^-16 on (2^-30 of the tile's largest) to 22 bits and lose up
-    // to 2^-38 of what is smaller. What marked tiles lost is added here, in finer units.
+    // to 2^-38 of what is smaller: of a marked tile, less than 2^-38 KT 128 units. Where that
+    // may be more than 2^-22 of a sum (a column of V that is 0 at the keys of larger x), what the
+    // marked tiles lost is added, in finer units.
+    bool again = false;
     if (__any_sync(0xffffffffu, marks != 0)) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            float const limit = lost[m] * (C::KT * 128.0f / 65536.0f);
+            if (seen[m] == 0 || m_run[m] == neg_inf(0.0f) || (R == 4 && g >= 4)) continue;
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) {
+                float2 const y = unpair(o[m][n]);
+                again |= fminf(fabsf(y.x), fabsf(y.y)) < limit;
+            }
+        }
+    }
+    if (__any_sync(0xffffffffu, again)) {
         int const count = k, first_tile = tile - k * W;
         auto marked = [&](int k) {  // the first marked tile from the k-th on, or `count`
             if (k >= kMarks) return __shfl_sync(0xffffffffu, marks, 31) >> 31 ? min(k, count) : count;
@@ -737,13 +739,6 @@ __global__ void __launch_bounds__(32 * W, Q8<D, R, W>::PER_SM) decode_q8_kernel(
                 float const local = top == neg_inf(0.0f) ? base : ceilf(top);
                 unit[m] = exp2_neg(local - base) * pow2_biased(ve - 13);
                 terms(s[m], local, w, x[m]);
-                if constexpr (R == 4) {
-                    unit[m] *= kFiner;
-#pragma unroll
-                    for (int i = 0; i < C::KV; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) x[m][i][e] = g < 4 ? rest(x[m][i][e]) : 0.0f;
-                }
             }
             uint32_t vr[C::KV][4][C::VW];
             load_v(tk + C::TILE, vr);
@@ -776,19 +771,6 @@ __global__ void __launch_bounds__(32 * W, Q8<D, R, W>::PER_SM) decode_q8_kernel(
     // Warps to CTA: every warp's rows, maxima and sums. Columns 2t and 2t + 1 of
     // n-tile n are elements 32 t + n and 32 t + 16 + n of a 128-element stretch (D =
     // 64: 16 t + n and 16 t + 8 + n).
-    if constexpr (R == 4) {  // both parts of a row: lanes g < 4 write column 2t, the others column 2t + 1
-        float* const p = reinterpret_cast<float*>(ring) + (g & 3) * D + 2 * STRETCH * t + (g >> 2) * STRETCH;
-#pragma unroll
-        for (int n = 0; n < D / 8; n += 4) {
-            float v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float2 const y = unpair(o[0][n + i]);
-                v[i] = (g < 4 ? y.x : y.y) + __shfl_xor_sync(0xffffffffu, g < 4 ? y.y : y.x, 16);
-            }
-            *reinterpret_cast<float4*>(p + n) = make_float4(v[0], v[1], v[2], v[3]);
-        }
-    }
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         float l = l_run[m];
@@ -798,7 +780,7 @@ __global__ void __launch_bounds__(32 * W, Q8<D, R, W>::PER_SM) decode_q8_kernel(
             sml[warp * C::ROWS + 8 * m + g] = m_run[m];
             sml[(W + warp) * C::ROWS + 8 * m + g] = l;
         }
-        if constexpr (R > 4) {
+        if (R > 4 || g < 4) {
             float* row = reinterpret_cast<float*>(ring) + (8 * m + g) * D;
 #pragma unroll
             for (int n = 0; n < D / 8; n += 4) {
